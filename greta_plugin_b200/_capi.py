@@ -64,6 +64,13 @@ def options():
     return None if o is None else ctypes.byref(o)
 
 
+def token_ranges() -> int:
+    """rows_ranges of the enclosing launch_options block (0 = built-in): the
+    selective scan takes it as the number of token ranges of its stream."""
+    o = getattr(_local, "opts", None)
+    return 0 if o is None else int(o.rows_ranges)
+
+
 class GretaKernelError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 
@@ -104,6 +111,28 @@ def lib() -> ctypes.CDLL:
     L.greta_dynconv_bwd_ld_ex.argtypes = [I32, P, I64, P, I64, P, I64, P, P, P, I64, P, I64, P, I64, P, I32, I64,
                                           I64, I64, I64, I64, I32, F, P, P]
     L.greta_dynconv_bwd_ld_ex.restype = I32
+    # state-space operators (include/greta_ssm.h)
+    conv = [I32, P, I64, P, I64, I64, P]  # dtype, x, ldx, w, sw_k, sw_d, bias
+    seqs = [P, I32, I64]                  # cu_seqlens, cu_int64, num_seqs
+    state = [P, I64, I64, I64, I64, P, P, P, I64]  # state, num_slots, strides, starts, slots, has_initial, num_reqs
+    scan = [I32, P, I64, P, I64, P, I64, P, I64, P, I64, P, P, P]  # dtype, u, delta, gate, B, C, A, skip, delta_bias
+    ssm = {
+        "conv_fwd": conv + [P] + seqs + [I64, I64, I64, I32, P],
+        "conv_bwd": conv + [P, P, P, P] + seqs + [I64, I64, I64, I32, P, I64, P],
+        "conv_packed": conv + [P] + state + [I64, I64, I64, I32, I32, P, P],
+        "scan_fwd": scan + [P, P] + seqs + [I64, I64, I64, I64, I32, I32, P, I64, P],
+        "scan_bwd": scan + [P] * 10 + seqs + [I64, I64, I64, I64, I32, I32, P, I64, P],
+        "scan_packed": scan + [P] + state + [I64, I64, I64, I64, I32, I32, I32, P, P, I64, P],
+    }
+    ssm["batch_metadata"] = [P, P, I64, I64, P, P, P, P, P, I64, I64, I64, P, I64, P, P, P]
+    for name, args in ssm.items():
+        getattr(L, f"greta_ssm_{name}").argtypes = args
+        getattr(L, f"greta_ssm_{name}").restype = I32
+    sizes = {"conv_bwd_workspace": [I64] * 3, "scan_workspace": [I64] * 5 + [I32],
+             "scan_bwd_workspace": [I64] * 5 + [I32]}
+    for name, args in sizes.items():
+        getattr(L, f"greta_ssm_{name}").argtypes = args
+        getattr(L, f"greta_ssm_{name}").restype = I64
     L.greta_dynconv_supports.argtypes = [I64, I64]
     L.greta_dynconv_device_errors.argtypes = [I32]
     L.greta_dynconv_status_string.argtypes = [I32]

@@ -1,0 +1,230 @@
+"""Short causal depthwise convolution with static filters (the one ahead of a
+selective scan), for training and for packed serving batches.
+
+  pre[t, d] = bias[d] + sum_k weight[k, d] x[t + k - W + 1, d]   (tap W-1 = current token)
+  out[t, d] = SiLU(pre) or pre
+
+  causal_conv1d          packed sequences (cu_seqlens), zero history, with autograd
+                         -> greta_ssm_conv_fwd / greta_ssm_conv_bwd
+  packed_causal_conv1d   a serving batch with cache-slot state, prompts and single
+                         tokens in any mix -> greta_ssm_conv_packed
+
+Filters are tap-major [W, D], as this package's per-token filters are
+[T, W, D/G]; a checkpoint's [D, 1, W] weight is passed as
+`weight.squeeze(1).t()`, which the kernels read in place. x may be a column
+view of a wider projection output (contiguous channels, any row stride). The
+reference has no such convolution; its dynamic one is dynamic_conv.py.
+
+There is no CPU fallback: non-CUDA tensors raise ValueError.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _capi
+from .dynamic_conv import _cu
+
+MAX_WIDTH = 16
+
+
+def _activation(activation) -> int:
+    if activation not in (None, "silu"):
+        raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+    return int(activation == "silu")
+
+
+def channel_rows(t):
+    """[T, D] as (tensor, row stride): read in place when the channels are
+    contiguous and rows do not overlap, else made contiguous. Rows that start
+    on whole vectors take the vector path; others are read by element."""
+    T, D = t.shape
+    if (t.stride(1) == 1 or D == 1) and (t.stride(0) >= D or T == 1):
+        return t, max(t.stride(0), D)
+    return t.contiguous(), D
+
+
+def _check_weight(x, weight, bias):
+    D = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[1] != D:
+        raise ValueError(f"weight must be [W, {D}] (taps, channels), got {tuple(weight.shape)}")
+    if not 1 <= weight.shape[0] <= MAX_WIDTH:
+        raise ValueError(f"kernel size must be between 1 and {MAX_WIDTH}, got {weight.shape[0]}")
+    if bias is not None and tuple(bias.shape) != (D,):
+        raise ValueError(f"bias must be [{D}], got {tuple(bias.shape)}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    return weight.shape[0]
+
+
+def _as_type(t, dtype):
+    return t if t is None or t.dtype == dtype else t.to(dtype)
+
+
+class CausalConv1dFunction(torch.autograd.Function):
+    """x [T, D] (rows may be strided), weight [W, D], bias [D] or None."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, cu_seqlens, silu):
+        x, ldx = channel_rows(x)
+        w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
+        b = None if b is None else b.contiguous()
+        T, D = x.shape
+        y = torch.empty(T, D, dtype=x.dtype, device=x.device)
+        cu, cu64, nseq = _cu(cu_seqlens, x.device)
+        with torch.cuda.device(x.device.index):
+            st = _capi.lib().greta_ssm_conv_fwd(
+                _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
+                _capi.ptr(y), _capi.ptr(cu), cu64, nseq, T, D, w.shape[0], silu, _capi.stream_of(x))
+        _capi.check("greta_ssm_conv_fwd", st)
+        ctx.save_for_backward(x, weight, bias, cu)
+        ctx.silu = silu
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, weight, bias, cu = ctx.saved_tensors
+        x, ldx = channel_rows(x)
+        w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
+        b = None if b is None else b.contiguous()
+        T, D = x.shape
+        W = w.shape[0]
+        dout = _as_type(dout, x.dtype).contiguous()
+        dev = x.device
+        dx = torch.empty(T, D, dtype=x.dtype, device=dev)
+        dw = torch.empty(W, D, dtype=x.dtype, device=dev)
+        db = None if b is None else torch.empty(D, dtype=x.dtype, device=dev)
+        L = _capi.lib()
+        ws = torch.empty(L.greta_ssm_conv_bwd_workspace(T, D, W), dtype=torch.uint8, device=dev)
+        cu, cu64, nseq = _cu(cu, dev)
+        with torch.cuda.device(dev.index):
+            st = L.greta_ssm_conv_bwd(
+                _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
+                _capi.ptr(dout), _capi.ptr(dx), _capi.ptr(dw), _capi.ptr(db), _capi.ptr(cu), cu64, nseq, T, D, W,
+                ctx.silu, _capi.ptr(ws), ws.numel(), _capi.stream_of(x))
+        _capi.check("greta_ssm_conv_bwd", st)
+        return dx, _as_type(dw, weight.dtype), None if bias is None else _as_type(db, bias.dtype), None, None
+
+
+@torch.compiler.disable(recursive=True)
+def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  cu_seqlens: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
+    """Convolution of packed sequences, differentiable in x, weight and bias.
+
+    x: [1, T, D]; weight: [W, D]; bias: [D] or None; cu_seqlens: [N + 1]
+    offsets (None: one sequence); activation: None or "silu". Returns
+    [1, T, D] contiguous. Each sequence starts with zero history; rows that no
+    sequence holds give zeros and zero gradients. weight and bias are used in
+    x's type; their gradients are summed in fp32 and come back in their own.
+    """
+    if x.dim() != 3 or x.shape[0] != 1:
+        raise ValueError(f"x must be [1, T, D], got {tuple(x.shape)}")
+    _check_weight(x, weight, bias)
+    silu = _activation(activation)
+    _capi.dtype_code(x)
+    if not x.is_cuda:
+        raise ValueError("causal_conv1d requires CUDA tensors")
+    if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
+        raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
+    return CausalConv1dFunction.apply(x[0], weight, bias, cu_seqlens, silu)[None]
+
+
+def packed_metadata(x, state, starts, slots, has_initial):
+    """The request tensors on x's device in the kernels' types, checked against
+    one another."""
+    n = slots.numel()
+    if starts.numel() != n + 1 or has_initial.numel() != n:
+        raise ValueError(f"starts must hold one offset more than slots ({n}) and has_initial as many, got "
+                         f"{starts.numel()} and {has_initial.numel()}")
+    if state.device != x.device:
+        raise ValueError(f"state is on {state.device}, x on {x.device}")
+    return (starts.to(device=x.device, dtype=torch.int32).contiguous(),
+            slots.to(device=x.device, dtype=torch.int32).reshape(-1).contiguous(),
+            has_initial.to(device=x.device, dtype=torch.int8).reshape(-1).contiguous())
+
+
+def packed_out(x, out):
+    """(output of a packed call, whether it is new): `out`, checked, whose rows
+    outside every request stay as they were, or a new tensor, where the kernel
+    writes zeros to them."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device), 1
+    if out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous() or out.device != x.device:
+        raise ValueError("out must be a contiguous tensor shaped and typed like the input, on its device")
+    return out, 0
+
+
+def check_disjoint(out, **inputs):
+    """`out` is written while other rows of the inputs are still read."""
+    a0 = out.data_ptr()
+    a1 = a0 + out.numel() * out.element_size()
+    for name, t in inputs.items():
+        if t is None or t.numel() == 0 or a0 == a1:
+            continue
+        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        b0 = t.data_ptr()
+        if a0 < b0 + span * t.element_size() and b0 < a1:
+            raise ValueError(f"out must not overlap {name}")
+
+
+def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, flags):
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, D], got {tuple(x.shape)}")
+    T, D = x.shape
+    W = _check_weight(x, weight, bias)
+    silu = _activation(activation)
+    if state.dim() != 3 or tuple(state.shape[1:]) != (D, W - 1):
+        raise ValueError(f"state must be [slots, {D}, {W - 1}], got {tuple(state.shape)}")
+    if state.dtype != x.dtype:
+        raise ValueError(f"state dtype {state.dtype} must match x dtype {x.dtype}")
+    _capi.dtype_code(x)
+    if not x.is_cuda:
+        raise ValueError("packed_causal_conv1d requires CUDA tensors")
+    starts, slots, has_initial = packed_metadata(x, state, starts, slots, has_initial)
+    out, new = packed_out(x, out)
+    if T == 0:
+        return out
+    check_disjoint(out, x=x, state=state)
+    x, ldx = channel_rows(x)
+    w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
+    b = None if b is None else b.contiguous()
+    s_slot, s_d, s_h = state.stride()
+    with torch.cuda.device(x.device.index):
+        st = _capi.lib().greta_ssm_conv_packed(
+            _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
+            _capi.ptr(out), _capi.ptr(state) if state.numel() else None, state.shape[0], s_slot, s_d, s_h,
+            _capi.ptr(starts), _capi.ptr(slots), _capi.ptr(has_initial), slots.numel(), T, D, W, silu,
+            new, _capi.ptr(flags), _capi.stream_of(x))
+    _capi.check("greta_ssm_conv_packed", st)
+    return out
+
+
+def packed_causal_conv1d(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None):
+    """Convolution of a packed serving batch with cache-slot history, in one launch.
+
+    x: [T, D]; weight: [W, D]; bias: [D] or None; state: [slots, D, W-1] of x's
+    type, any strides, updated in place. starts: [N+1] offsets of the N
+    requests, prompts and single tokens in any mix; slots, has_initial: [N],
+    with the meaning they have in packed_dynamic_conv_triton (a negative slot
+    has no history and is not written). A request without tokens leaves its
+    slot as it was, and the requests of one batch have different slots. Returns
+    [T, D]: `out` when given, whose rows behind the last request stay as they
+    were (they are zeros in a new tensor).
+    """
+    return _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, None)
+
+
+def packed_causal_conv1d_checked(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None):
+    """packed_causal_conv1d, reporting slots >= state.shape[0] (which the kernel
+    skips) as IndexError. Waits for the device: for debugging and tests."""
+    flags = torch.zeros(1, dtype=torch.int32, device=x.device)
+    out = _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, flags)
+    if int(flags.item()) & 1:
+        raise IndexError(f"a cache slot index is >= the number of cache slots ({state.shape[0]})")
+    return out
+
+
+__all__ = ["causal_conv1d", "packed_causal_conv1d", "packed_causal_conv1d_checked", "CausalConv1dFunction"]

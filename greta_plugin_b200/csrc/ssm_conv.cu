@@ -1,0 +1,227 @@
+// C ABI of the short causal convolution: checks, launch shapes, dispatch.
+#include "ssm_conv.cuh"
+#include "ssm_launch.cuh"
+
+namespace greta {
+namespace ssm {
+
+int sm_count() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (cache[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
+
+namespace {
+
+constexpr int kRuns = 4;  // runs per block (one warp each)
+
+int check(int dtype, const void* x, int64_t ldx, const void* w, const void* y, const void* cu, int64_t num_seqs,
+          int64_t T, int64_t D, int64_t W) {
+  if (esize(dtype) == 0) return GRETA_ERR_UNSUPPORTED;
+  if (T < 0 || D <= 0 || W <= 0 || num_seqs < 0) return GRETA_ERR_INVALID_ARG;
+  if (T >= INT_MAX - 1024 || D > INT_MAX / 64 || num_seqs >= INT_MAX - 64) return GRETA_ERR_INVALID_ARG;
+  if (W > kMaxWGeneric) return GRETA_ERR_UNSUPPORTED;
+  if (T == 0) return GRETA_OK;
+  if (x == nullptr || w == nullptr || y == nullptr) return GRETA_ERR_INVALID_ARG;
+  if (ldx < D) return GRETA_ERR_INVALID_ARG;
+  if (cu == nullptr && num_seqs != 0) return GRETA_ERR_INVALID_ARG;
+  return GRETA_OK;
+}
+
+// Tokens per run: as many as leave each SM 16 warps (enough rows in flight to
+// fill HBM), a power of two between lo and hi.
+int run_tokens(int64_t T, int64_t warps_per_run, int lo, int hi) {
+  const int64_t want = T * warps_per_run / ((int64_t)sm_count() * 16);
+  int L = lo;
+  while (L < hi && 2 * L <= want) L *= 2;
+  return L;
+}
+
+template <typename T, int NV, int WT, bool PACKED>
+cudaError_t fwd_one(const ConvParams& p, dim3 grid, cudaStream_t st) {
+  return launch(ssm_conv_fwd_kernel<T, NV, WT, PACKED>, grid, dim3(32, kRuns), 0, st, p);
+}
+
+template <typename T, int NV, bool PACKED>
+cudaError_t fwd_w(const ConvParams& p, dim3 grid, cudaStream_t st) {
+  if constexpr (NV > 1) {
+    switch (p.W) {
+      case 2: return fwd_one<T, NV, 2, PACKED>(p, grid, st);
+      case 3: return fwd_one<T, NV, 3, PACKED>(p, grid, st);
+      case 4: return fwd_one<T, NV, 4, PACKED>(p, grid, st);
+    }
+  }
+  if (p.W <= 8) return fwd_one<T, NV, -8, PACKED>(p, grid, st);
+  return fwd_one<T, NV, -kMaxWGeneric, PACKED>(p, grid, st);
+}
+
+// Vectors of 16 bytes where every row starts on one; else single elements.
+template <typename T, bool PACKED>
+int fwd_type(ConvParams p, cudaStream_t st) {
+  constexpr int NV = 16 / sizeof(T);
+  p.vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, 16) && aligned(p.y, 16);
+  const int nv = p.vec ? NV : 1;
+  p.vec_w = p.sw_d == 1 && p.sw_k % nv == 0 && aligned(p.w, nv * sizeof(T));
+  if (p.state != nullptr) p.st_layout = state_layout(p.state, p.s_slot, p.s_d, p.s_h, p.W - 1, nv, sizeof(T));
+  const int64_t cw = cdiv(cdiv(p.D, nv), 32);
+  p.L = run_tokens(p.q.T, cw, 1, 64);
+  p.nblk = (int)cw;
+  const int64_t blocks = cdiv(cdiv(p.q.T, p.L), kRuns) * cw;
+  if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
+  const dim3 grid((unsigned)blocks);
+  return finish(p.vec ? fwd_w<T, NV, PACKED>(p, grid, st) : fwd_w<T, 1, PACKED>(p, grid, st));
+}
+
+template <bool PACKED>
+int fwd(int dtype, const ConvParams& p, void* stream) {
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case GRETA_DT_F32: return fwd_type<float, PACKED>(p, st);
+    case GRETA_DT_F16: return fwd_type<__half, PACKED>(p, st);
+    default: return fwd_type<__nv_bfloat16, PACKED>(p, st);
+  }
+}
+
+// Backward runs: four channels a thread (its sums take 2 W + 1 registers each).
+constexpr int kBwdVec = 4;
+constexpr int kBwdMinRun = 8, kBwdMaxRun = 64;
+
+// Blocks of runs of the backward, an upper bound for any channel vector.
+int64_t bwd_rows(int64_t T, int L) { return cdiv(cdiv(T, L), kRuns); }
+
+template <typename T, int NV, int WT>
+cudaError_t bwd_one(const ConvParams& p, dim3 grid, size_t smem, cudaStream_t st) {
+  auto k = ssm_conv_bwd_kernel<T, NV, WT>;
+  cudaError_t e = allow_smem(k, smem);
+  if (e != cudaSuccess) return e;
+  return launch(k, grid, dim3(32, kRuns), smem, st, p);
+}
+
+template <typename T, int NV>
+cudaError_t bwd_w(const ConvParams& p, dim3 grid, size_t smem, cudaStream_t st) {
+  if constexpr (NV > 1) {
+    switch (p.W) {
+      case 2: return bwd_one<T, NV, 2>(p, grid, smem, st);
+      case 3: return bwd_one<T, NV, 3>(p, grid, smem, st);
+      case 4: return bwd_one<T, NV, 4>(p, grid, smem, st);
+    }
+  }
+  if (p.W <= 8) return bwd_one<T, NV, -8>(p, grid, smem, st);
+  return bwd_one<T, NV, -kMaxWGeneric>(p, grid, smem, st);
+}
+
+template <typename T>
+int bwd_type(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
+  constexpr int NV = kBwdVec;
+  p.vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) && aligned(p.dout, NV * sizeof(T)) &&
+          aligned(p.dx, NV * sizeof(T));
+  const int nv = p.vec ? NV : 1;
+  p.vec_w = p.sw_d == 1 && p.sw_k % nv == 0 && aligned(p.w, nv * sizeof(T));
+  const int64_t cw = cdiv(cdiv(p.D, nv), 32);
+  p.L = run_tokens(p.q.T, cw, kBwdMinRun, kBwdMaxRun);
+  p.nblk = (int)cw;
+  const int64_t rows = bwd_rows(p.q.T, p.L);
+  if (rows * cw > INT_MAX) return GRETA_ERR_INVALID_ARG;
+  const size_t smem = (size_t)kRuns * (p.W + 1) * 32 * nv * sizeof(float);
+  const dim3 grid((unsigned)(rows * cw));
+  cudaError_t e = p.vec ? bwd_w<T, NV>(p, grid, smem, st) : bwd_w<T, 1>(p, grid, smem, st);
+  if (e != cudaSuccess) return GRETA_ERR_LAUNCH;
+  const int64_t cols = cdiv((int64_t)(p.W + 1) * p.D, 32);
+  return finish(launch(ssm_conv_reduce_kernel<T>, dim3((unsigned)cols), dim3(32, 8), 0, st, (const float*)p.part,
+                       reinterpret_cast<T*>(dw), reinterpret_cast<T*>(dbias), (long long)rows, p.D, p.W));
+}
+
+ConvParams base(const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d, const void* bias,
+                const void* cu, int cu64, int64_t num_seqs, int64_t T, int64_t D, int64_t W, int silu) {
+  ConvParams p{};
+  p.x = x; p.w = w; p.bias = bias;
+  p.q = Seqs{cu, cu64, cu == nullptr ? 1 : (int)num_seqs, (int)T};
+  p.ldx = ldx; p.sw_k = sw_k; p.sw_d = sw_d;
+  p.D = (int)D; p.W = (int)W;
+  p.silu = silu != 0;
+  return p;
+}
+
+}  // namespace
+}  // namespace ssm
+}  // namespace greta
+
+using namespace greta;
+using namespace greta::ssm;
+
+extern "C" {
+
+int greta_ssm_conv_fwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,
+                       const void* bias, void* y, const void* cu_seqlens, int cu_int64, int64_t num_seqs, int64_t T,
+                       int64_t D, int64_t W, int silu, void* stream) {
+  const int c = check(dtype, x, ldx, w, y, cu_seqlens, num_seqs, T, D, W);
+  if (c != GRETA_OK || T == 0) return c;
+  ConvParams p = base(x, ldx, w, sw_k, sw_d, bias, cu_seqlens, cu_int64, num_seqs, T, D, W, silu);
+  p.y = y;
+  p.zero_rest = 1;
+  return fwd<false>(dtype, p, stream);
+}
+
+int64_t greta_ssm_conv_bwd_workspace(int64_t T, int64_t D, int64_t W) {
+  if (T <= 0 || D <= 0 || W <= 0) return 0;
+  return bwd_rows(T, kBwdMinRun) * (W + 1) * D * (int64_t)sizeof(float);
+}
+
+int greta_ssm_conv_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,
+                       const void* bias, const void* dout, void* dx, void* dw, void* dbias, const void* cu_seqlens,
+                       int cu_int64, int64_t num_seqs, int64_t T, int64_t D, int64_t W, int silu, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+  const int c = check(dtype, x, ldx, w, dx, cu_seqlens, num_seqs, T, D, W);
+  if (c != GRETA_OK) return c;
+  if (dw == nullptr || (bias == nullptr) != (dbias == nullptr)) return GRETA_ERR_INVALID_ARG;
+  if (T > 0 && dout == nullptr) return GRETA_ERR_INVALID_ARG;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (T == 0) {  // sums over no tokens
+    const int es = esize(dtype);
+    cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)(W * D) * es, st);
+    if (e == cudaSuccess && dbias != nullptr) e = cudaMemsetAsync(dbias, 0, (size_t)D * es, st);
+    return finish(e);
+  }
+  if (workspace == nullptr || workspace_bytes < greta_ssm_conv_bwd_workspace(T, D, W)) return GRETA_ERR_INVALID_ARG;
+  if (!aligned(workspace, 16)) return GRETA_ERR_ALIGNMENT;
+  ConvParams p = base(x, ldx, w, sw_k, sw_d, bias, cu_seqlens, cu_int64, num_seqs, T, D, W, silu);
+  p.dout = dout;
+  p.dx = dx;
+  p.part = reinterpret_cast<float*>(workspace);
+  switch (dtype) {
+    case GRETA_DT_F32: return bwd_type<float>(p, dw, dbias, st);
+    case GRETA_DT_F16: return bwd_type<__half>(p, dw, dbias, st);
+    default: return bwd_type<__nv_bfloat16>(p, dw, dbias, st);
+  }
+}
+
+int greta_ssm_conv_packed(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,
+                          const void* bias, void* y, void* state, int64_t num_slots, int64_t s_slot, int64_t s_d,
+                          int64_t s_h, const int32_t* starts, const int32_t* slots, const int8_t* has_initial,
+                          int64_t num_reqs, int64_t T, int64_t D, int64_t W, int silu, int zero_rest,
+                          int32_t* error_flags, void* stream) {
+  const int c = check(dtype, x, ldx, w, y, starts, num_reqs, T, D, W);
+  if (c != GRETA_OK || T == 0) return c;
+  if (starts == nullptr || num_slots < 0) return GRETA_ERR_INVALID_ARG;
+  if (num_reqs > 0 && (slots == nullptr || has_initial == nullptr)) return GRETA_ERR_INVALID_ARG;
+  if (W > 1 && num_slots > 0 && state == nullptr) return GRETA_ERR_INVALID_ARG;
+  ConvParams p = base(x, ldx, w, sw_k, sw_d, bias, starts, 0, num_reqs, T, D, W, silu);
+  p.y = y;
+  if (W > 1 && num_slots > 0) {
+    p.state = state;
+    p.s_slot = s_slot; p.s_d = s_d; p.s_h = s_h; p.num_slots = num_slots;
+  }
+  p.slots = slots;
+  p.initial = reinterpret_cast<const signed char*>(has_initial);
+  p.err = error_flags;
+  p.zero_rest = zero_rest != 0;
+  return fwd<true>(dtype, p, stream);
+}
+
+}  // extern "C"

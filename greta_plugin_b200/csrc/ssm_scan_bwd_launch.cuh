@@ -1,0 +1,39 @@
+// The backward's launches for one element type (ssm_scan_bwd_<dtype>.cu).
+#pragma once
+
+#include "ssm_scan_bwd.cuh"
+#include "ssm_scan_launch.cuh"
+
+namespace greta {
+namespace ssm {
+
+template <typename T>
+cudaError_t scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st) {
+  const int bpg = (int)cdiv(p.spg, kScanWarps);
+  cudaError_t e = with_lanes(p.N, [&](auto ln) {
+    constexpr int LN = decltype(ln)::value;
+    const dim3 block(kScanWarps * 32);
+    if (p.R > 1) {
+      auto k = ssm_scan_bwd_carry_kernel<T, LN>;
+      const size_t smem = sizeof(float) * kScanWarps * FwdSmem<LN>::kWarp;
+      cudaError_t e = allow_smem(k, smem);
+      if (e == cudaSuccess) e = launch(k, slices_grid(p, p.R), block, smem, st, p);
+      if (e != cudaSuccess) return e;
+    }
+    auto k = ssm_scan_bwd_kernel<T, LN>;
+    const size_t smem = sizeof(float) * BwdSmem<LN>::kTotal;
+    static_assert(sizeof(float) * BwdSmem<LN>::kTotal <= 227 * 1024, "shared memory of a CTA");
+    cudaError_t e = allow_smem(k, smem);
+    if (e != cudaSuccess) return e;
+    return launch(k, dim3((unsigned)(p.F * bpg), (unsigned)p.R), block, smem, st, p);
+  });
+  if (e != cudaSuccess) return e;
+  e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), (unsigned)p.F),
+             dim3(256), 0, st, (const float*)p.part_bc, (T*)g.dB, (T*)g.dC, bpg, p.q.T, p.N, p.F);
+  if (e != cudaSuccess) return e;
+  return launch(ssm_scan_reduce_a_kernel<4>, dim3((unsigned)cdiv((int64_t)p.D * (p.N + 2), 256)), dim3(256), 0, st,
+                (const float*)p.part_a, (const float*)p.part_d, g.dA, g.dskip, g.dbias, p.R, p.D, p.N);
+}
+
+}  // namespace ssm
+}  // namespace greta

@@ -1,0 +1,269 @@
+// C ABI of the selective scan: checks, ranges and workspaces, dispatch.
+
+#include "ssm_scan_launch.cuh"
+
+namespace greta {
+namespace ssm {
+namespace {
+
+constexpr int64_t kMaxStates = 128;
+constexpr int kMaxRanges = 64;
+constexpr int kMinRange = 32;  // tokens
+
+int64_t slices(int64_t D, int64_t N, int64_t F) { return F * cdiv(D / F, 128 / lanes_of(N)); }
+
+// Ranges the stream is cut into: enough that each SM has kWarpsPerSm warps,
+// none shorter than kMinRange tokens. Returns the tokens per range (a multiple
+// of kTile) and sets R.
+constexpr int kWarpsPerSm = 8;
+int64_t plan_ranges(int64_t T, int64_t D, int64_t N, int64_t F, int asked, int& R) {
+  int64_t r = asked > 0 ? asked : cdiv((int64_t)sm_count() * kWarpsPerSm, slices(D, N, F));
+  if (r > kMaxRanges) r = kMaxRanges;
+  const int64_t least = asked > 0 ? kTile : kMinRange;
+  int64_t L = cdiv(cdiv(T, r), kTile) * kTile;
+  if (L < least) L = least;
+  R = (int)cdiv(T, L);
+  return L;
+}
+
+int64_t a16(int64_t v) { return (v + 15) / 16 * 16; }
+
+struct Workspace {
+  int64_t carry, hinit, dsum, reset, total;
+  Workspace(int64_t R, int64_t D, int64_t N) {
+    const int64_t states = R > 1 ? a16(R * D * N * 4) : 0;
+    carry = 0;
+    hinit = states;
+    dsum = 2 * states;
+    reset = dsum + (R > 1 ? a16(R * D * 4) : 0);
+    total = reset + (R > 1 ? a16(R * 4) : 0);
+  }
+};
+
+int check(int dtype, const ScanParams& p, const void* cu, int64_t num_seqs, int64_t T, int64_t D, int64_t N,
+          int64_t F, int ranges) {
+  if (esize(dtype) == 0) return GRETA_ERR_UNSUPPORTED;
+  if (T < 0 || D <= 0 || N <= 0 || F <= 0 || num_seqs < 0 || ranges < 0) return GRETA_ERR_INVALID_ARG;
+  if (T >= INT_MAX - 1024 || D > INT_MAX / 256 || num_seqs >= INT_MAX - 64) return GRETA_ERR_INVALID_ARG;
+  if (D % F != 0) return GRETA_ERR_INVALID_ARG;
+  if (N > kMaxStates) return GRETA_ERR_UNSUPPORTED;
+  if (T == 0) return GRETA_OK;
+  if (p.u == nullptr || p.delta == nullptr || p.A == nullptr || p.B == nullptr || p.C == nullptr)
+    return GRETA_ERR_INVALID_ARG;
+  if (p.ldu < D || p.ldd < D || (p.gate != nullptr && p.ldg < D) || p.ldb < F * N || p.ldc < F * N)
+    return GRETA_ERR_INVALID_ARG;
+  if (cu == nullptr && num_seqs != 0) return GRETA_ERR_INVALID_ARG;
+  if (!aligned(p.A, 16)) return GRETA_ERR_ALIGNMENT;
+  return GRETA_OK;
+}
+
+// Vector paths: a lane's loads of V channels (4 or 8) and of 4 states start on
+// whole aligned vectors in every row and group.
+void plan_vectors(ScanParams& p, int es, std::initializer_list<const void*> rows) {
+  const int CHW = 128 / lanes_of(p.N), V = CHW < 8 ? CHW : 8;
+  const int64_t a = (int64_t)V * es < 16 ? (int64_t)V * es : 16;
+  bool ok = p.Dg % V == 0 && p.D % V == 0 && p.ldu % V == 0 && p.ldd % V == 0 &&
+            (p.gate == nullptr || p.ldg % V == 0);
+  for (const void* q : rows) ok = ok && aligned(q, a);
+  p.vec = ok;
+  p.vec_bc = p.N % 4 == 0 && p.ldb % 4 == 0 && p.ldc % 4 == 0 && aligned(p.B, 4 * es) && aligned(p.C, 4 * es);
+}
+
+ScanParams base(const void* u, int64_t ldu, const void* delta, int64_t ldd, const void* gate, int64_t ldg,
+                const void* B, int64_t ldb, const void* C, int64_t ldc, const float* A, const float* skip,
+                const float* dbias, void* out, const void* cu, int cu64, int64_t num_seqs, int64_t T, int64_t D,
+                int64_t N, int64_t F, int softplus) {
+  ScanParams p{};
+  p.u = u; p.delta = delta; p.gate = gate; p.B = B; p.C = C;
+  p.A = A; p.skip = skip; p.dbias = dbias;
+  p.out = out;
+  p.ldu = ldu; p.ldd = ldd; p.ldg = gate == nullptr ? 0 : ldg; p.ldb = ldb; p.ldc = ldc;
+  p.q = Seqs{cu, cu64, cu == nullptr ? 1 : (int)num_seqs, (int)T};
+  p.D = (int)D; p.N = (int)N; p.F = (int)F;
+  if (D > 0 && F > 0 && N > 0) {
+    p.Dg = (int)(D / F);
+    p.spg = (int)cdiv(p.Dg, 128 / lanes_of(N));
+  }
+  p.softplus = softplus != 0;
+  return p;
+}
+
+int set_workspace(ScanParams& p, void* ws, int64_t bytes) {
+  const Workspace w(p.R, p.D, p.N);
+  if (w.total == 0) return GRETA_OK;
+  if (ws == nullptr || bytes < w.total) return GRETA_ERR_INVALID_ARG;
+  if (!aligned(ws, 16)) return GRETA_ERR_ALIGNMENT;
+  char* b = reinterpret_cast<char*>(ws);
+  p.carry = reinterpret_cast<float*>(b + w.carry);
+  p.hinit = reinterpret_cast<float*>(b + w.hinit);
+  p.dsum = reinterpret_cast<float*>(b + w.dsum);
+  p.reset = reinterpret_cast<int*>(b + w.reset);
+  return GRETA_OK;
+}
+
+int run_fwd(int dtype, const ScanParams& p, void* stream) {
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case GRETA_DT_F32: return finish(scan_fwd_f32(p, st));
+    case GRETA_DT_F16: return finish(scan_fwd_f16(p, st));
+    default: return finish(scan_fwd_bf16(p, st));
+  }
+}
+
+int run_decode(int dtype, const ScanParams& p, int rq, void* stream) {
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case GRETA_DT_F32: return finish(scan_decode_f32(p, rq, st));
+    case GRETA_DT_F16: return finish(scan_decode_f16(p, rq, st));
+    default: return finish(scan_decode_bf16(p, rq, st));
+  }
+}
+
+// The backward's workspace: the carries', then the parts of the sums.
+struct BwdWorkspace {
+  int64_t bc, a, d, total;
+  BwdWorkspace(int64_t R, int64_t T, int64_t D, int64_t N, int64_t F) {
+    const int64_t blocks = F * cdiv(slices(D, N, F) / F, kScanWarps);
+    bc = a16(Workspace(R, D, N).total);
+    a = bc + a16(blocks * T * 2 * N * 4);
+    d = a + a16(R * D * N * 4);
+    total = d + a16(R * 2 * D * 4);
+  }
+};
+
+int run_bwd(int dtype, const ScanParams& p, const ScanGrads& g, void* stream) {
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case GRETA_DT_F32: return finish(scan_bwd_f32(p, g, st));
+    case GRETA_DT_F16: return finish(scan_bwd_f16(p, g, st));
+    default: return finish(scan_bwd_bf16(p, g, st));
+  }
+}
+
+// Tokens beyond one per request up to which a batch is a decode batch: its
+// longest request then has at most kDecodeExtra + 1 tokens, walked one after
+// another.
+constexpr int64_t kDecodeExtra = 8;
+
+}  // namespace
+}  // namespace ssm
+}  // namespace greta
+
+using namespace greta;
+using namespace greta::ssm;
+
+extern "C" {
+
+int64_t greta_ssm_scan_workspace(int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F, int ranges) {
+  (void)num_seqs;
+  if (T <= 0 || D <= 0 || N <= 0 || F <= 0 || D % F != 0 || N > kMaxStates || ranges < 0) return 0;
+  int R = 1;
+  plan_ranges(T, D, N, F, ranges, R);
+  return Workspace(R, D, N).total;
+}
+
+int greta_ssm_scan_fwd(int dtype, const void* u, int64_t ldu, const void* delta, int64_t ldd, const void* gate,
+                       int64_t ldg, const void* B, int64_t ldb, const void* C, int64_t ldc, const float* A,
+                       const float* skip, const float* delta_bias, void* out, float* saved, const void* cu_seqlens,
+                       int cu_int64, int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F, int softplus,
+                       int ranges, void* workspace, int64_t workspace_bytes, void* stream) {
+  ScanParams p = base(u, ldu, delta, ldd, gate, ldg, B, ldb, C, ldc, A, skip, delta_bias, out, cu_seqlens, cu_int64,
+                      num_seqs, T, D, N, F, softplus);
+  int c = check(dtype, p, cu_seqlens, num_seqs, T, D, N, F, ranges);
+  if (c != GRETA_OK || T == 0) return c;
+  if (out == nullptr) return GRETA_ERR_INVALID_ARG;
+  if (!aligned(saved, 16)) return GRETA_ERR_ALIGNMENT;
+  p.ckpt = saved;
+  p.zero_rest = 1;
+  plan_vectors(p, esize(dtype), {u, delta, gate, out});
+  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  c = set_workspace(p, workspace, workspace_bytes);
+  if (c != GRETA_OK) return c;
+  return run_fwd(dtype, p, stream);
+}
+
+int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* delta, int64_t ldd, const void* gate,
+                          int64_t ldg, const void* B, int64_t ldb, const void* C, int64_t ldc, const float* A,
+                          const float* skip, const float* delta_bias, void* out, float* state, int64_t num_slots,
+                          int64_t s_slot, int64_t s_d, int64_t s_n, const int32_t* starts, const int32_t* slots,
+                          const int8_t* has_initial, int64_t num_reqs, int64_t T, int64_t D, int64_t N, int64_t F,
+                          int softplus, int zero_rest, int ranges, int32_t* error_flags, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  ScanParams p = base(u, ldu, delta, ldd, gate, ldg, B, ldb, C, ldc, A, skip, delta_bias, out, starts, 0, num_reqs,
+                      T, D, N, F, softplus);
+  int c = check(dtype, p, starts, num_reqs, T, D, N, F, ranges);
+  if (c != GRETA_OK || T == 0) return c;
+  if (out == nullptr || starts == nullptr || num_slots < 0) return GRETA_ERR_INVALID_ARG;
+  if (num_reqs > 0 && (slots == nullptr || has_initial == nullptr)) return GRETA_ERR_INVALID_ARG;
+  if (num_slots > 0 && state == nullptr) return GRETA_ERR_INVALID_ARG;
+  p.zero_rest = zero_rest != 0;
+  if (num_slots > 0) {
+    p.state = state;
+    p.s_slot = s_slot; p.s_d = s_d; p.s_n = s_n; p.num_slots = num_slots;
+    p.st_vec = s_n == 1 && s_d % 4 == 0 && s_slot % 4 == 0 && N % 4 == 0 && aligned(state, 16);
+  }
+  p.slots = slots;
+  p.initial = reinterpret_cast<const signed char*>(has_initial);
+  p.err = error_flags;
+  plan_vectors(p, esize(dtype), {u, delta, gate, out});
+  if (ranges == 0 && num_reqs > 0 && T <= num_reqs + kDecodeExtra) {
+    // one request a warp while that is what it takes to give every SM work
+    const int64_t warps = slices(D, N, F) * num_reqs;
+    const int rq = warps >= (int64_t)sm_count() * 64 ? 2 : 1;
+    if (cdiv(num_reqs, rq) <= 65535) return run_decode(dtype, p, rq, stream);
+  }
+  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  c = set_workspace(p, workspace, workspace_bytes);
+  if (c != GRETA_OK) return c;
+  return run_fwd(dtype, p, stream);
+}
+
+int64_t greta_ssm_scan_bwd_workspace(int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F, int ranges) {
+  (void)num_seqs;
+  if (T <= 0 || D <= 0 || N <= 0 || F <= 0 || D % F != 0 || N > kMaxStates || ranges < 0) return 0;
+  int R = 1;
+  plan_ranges(T, D, N, F, ranges, R);
+  return BwdWorkspace(R, T, D, N, F).total;
+}
+
+int greta_ssm_scan_bwd(int dtype, const void* u, int64_t ldu, const void* delta, int64_t ldd, const void* gate,
+                       int64_t ldg, const void* B, int64_t ldb, const void* C, int64_t ldc, const float* A,
+                       const float* skip, const float* delta_bias, const float* saved, const void* dout, void* du,
+                       void* ddelta, void* dgate, void* dB, void* dC, float* dA, float* dskip, float* ddelta_bias,
+                       const void* cu_seqlens, int cu_int64, int64_t num_seqs, int64_t T, int64_t D, int64_t N,
+                       int64_t F, int softplus, int ranges, void* workspace, int64_t workspace_bytes, void* stream) {
+  ScanParams p = base(u, ldu, delta, ldd, gate, ldg, B, ldb, C, ldc, A, skip, delta_bias, nullptr, cu_seqlens,
+                      cu_int64, num_seqs, T, D, N, F, softplus);
+  int c = check(dtype, p, cu_seqlens, num_seqs, T, D, N, F, ranges);
+  if (c != GRETA_OK) return c;
+  if (dA == nullptr || (skip != nullptr && dskip == nullptr) || (delta_bias != nullptr && ddelta_bias == nullptr))
+    return GRETA_ERR_INVALID_ARG;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (T == 0) {  // sums over no tokens
+    cudaError_t e = cudaMemsetAsync(dA, 0, (size_t)(D * N) * 4, st);
+    if (e == cudaSuccess && dskip != nullptr) e = cudaMemsetAsync(dskip, 0, (size_t)D * 4, st);
+    if (e == cudaSuccess && ddelta_bias != nullptr) e = cudaMemsetAsync(ddelta_bias, 0, (size_t)D * 4, st);
+    return finish(e);
+  }
+  if (saved == nullptr || dout == nullptr || du == nullptr || ddelta == nullptr || dB == nullptr || dC == nullptr ||
+      (gate != nullptr && dgate == nullptr))
+    return GRETA_ERR_INVALID_ARG;
+  if (!aligned(saved, 16)) return GRETA_ERR_ALIGNMENT;
+  p.ckpt = const_cast<float*>(saved);
+  p.dout = dout;
+  p.du = du; p.ddelta = ddelta; p.dgate = dgate;
+  plan_vectors(p, esize(dtype), {u, delta, gate, dout, du, ddelta, dgate});
+  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  const BwdWorkspace w(p.R, T, D, N, F);
+  if (workspace == nullptr || workspace_bytes < w.total) return GRETA_ERR_INVALID_ARG;
+  if (!aligned(workspace, 16)) return GRETA_ERR_ALIGNMENT;
+  c = set_workspace(p, workspace, workspace_bytes);
+  if (c != GRETA_OK) return c;
+  char* b = reinterpret_cast<char*>(workspace);
+  p.part_bc = reinterpret_cast<float*>(b + w.bc);
+  p.part_a = reinterpret_cast<float*>(b + w.a);
+  p.part_d = reinterpret_cast<float*>(b + w.d);
+  return run_bwd(dtype, p, ScanGrads{dA, dskip, ddelta_bias, dB, dC}, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,9 @@
+// Selective scan, f16 instantiations.
+#include "ssm_scan_launch.cuh"
+
+namespace greta {
+namespace ssm {
+cudaError_t scan_fwd_f16(const ScanParams& p, cudaStream_t st) { return scan_fwd<__half>(p, st); }
+cudaError_t scan_decode_f16(const ScanParams& p, int rq, cudaStream_t st) { return scan_decode<__half>(p, rq, st); }
+}  // namespace ssm
+}  // namespace greta
