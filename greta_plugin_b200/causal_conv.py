@@ -129,7 +129,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise ValueError("causal_conv1d requires CUDA tensors")
     if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
         raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
-    return CausalConv1dFunction.apply(x[0], weight, bias, cu_seqlens, silu)[None]
+    # squeeze, not x[0], whose gradient would be copied into zeros
+    return CausalConv1dFunction.apply(x.squeeze(0), weight, bias, cu_seqlens, silu).unsqueeze(0)
 
 
 def packed_metadata(x, state, starts, slots, has_initial):

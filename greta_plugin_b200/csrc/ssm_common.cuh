@@ -134,6 +134,42 @@ __device__ __forceinline__ void store_part(T* ptr, const Pack<T, NV>& r, int n, 
   }
 }
 
+// Asynchronous copies of 4, 8 or 16 bytes into shared memory; zeros where !ok
+// (the address is not read then, but has to be one).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool ok) {
+  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+  const int n = ok ? BYTES : 0;
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All of this thread's copies have landed.
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// NV elements of a row into shared memory: asynchronously when the row is
+// there in whole aligned vectors, else n of them one by one and zeros.
+template <typename T, int NV>
+__device__ __forceinline__ void copy_part(T* dst, const T* src, const T* base, int n, bool vec) {
+  constexpr int kBytes = sizeof(T) * NV;
+  if (vec || n <= 0) {
+    const bool ok = n > 0;
+    const T* s = ok ? src : base;
+    if constexpr (kBytes <= 16) {
+      copy_async<kBytes>(dst, s, ok);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i)
+        copy_async<16>(dst + i * (16 / sizeof(T)), ok ? s + i * (16 / sizeof(T)) : s, ok);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) dst[c] = c < n ? src[c] : from_f<T>(0.f);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // fp32 pairs in 64-bit registers (one instruction for two lanes; each lane is
 // rounded like the scalar operation)
@@ -186,31 +222,55 @@ __device__ __forceinline__ float exp_neg(float x) {
   return fmaf(e, lost * kLn2, e);
 }
 
-// log(1 + e^x), with a small relative error also where it is small (steps of
-// 1e-3 and less): max(x, 0) + log1p(e) for e = e^-|x| in (0, 1], and
-// log1p(e) = 2 atanh(v), v = e / (2 + e) <= 1/3, by atanh's series up to v^15
-// (the next term is below 2^-28 of the sum). x itself above 20, where the
-// rest is less than half an ulp, and for NaN the NaN.
-__device__ __forceinline__ float softplusf_(float x) {
-  const float e = exp_neg(-fabsf(x));
-  const float v = __fdividef(e, 2.f + e);
-  const float q = v * v;
-  float s = 1.f / 15.f;
-  s = fmaf(s, q, 1.f / 13.f);
-  s = fmaf(s, q, 1.f / 11.f);
-  s = fmaf(s, q, 1.f / 9.f);
-  s = fmaf(s, q, 1.f / 7.f);
-  s = fmaf(s, q, 1.f / 5.f);
-  s = fmaf(s, q, 1.f / 3.f);
-  const float l = 2.f * fmaf(s * q, v, v);
-  return x > 20.f ? x : (x > 0.f ? x + l : l);
+// max(x, 0) that keeps NaN.
+__device__ __forceinline__ float max0(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// 1 / (1 + e^-x), to a few ulp at both ends.
+// log(1 + e^x) of two values, with a small relative error also where it is
+// small (steps of 1e-3 and less): max(x, 0) + log1p(e) for e = e^-|x| in
+// (0, 1], and log1p(e) = e P(e) with the polynomial of degree 9 that fits
+// log1p(e) / e on [0, 1] best (5e-9; 1.2e-7 with the fp32 roundings). e as in
+// exp_neg; beyond 87 it is nothing next to the sum.
+__device__ __forceinline__ f2 softplus2(float x0, float x1) {
+  const f2 x = pack2(fminf(fabsf(x0), 87.f), fminf(fabsf(x1), 87.f));
+  const f2 t = f2_mul(x, pack2(-kLog2e, -kLog2e));  // rounded -|x| log2(e)
+  // what it lost: -(|x| log2(e) + t) - |x| (log2(e) - kLog2e)
+  f2 lost = f2_fma(x, pack2(-kLog2e, -kLog2e), f2_mul(t, pack2(-1.f, -1.f)));
+  lost = f2_fma(x, pack2(-1.925963033e-8f, -1.925963033e-8f), lost);
+  f2 e = f2_ex2(t);
+  e = f2_fma(e, f2_mul(lost, pack2(kLn2, kLn2)), e);
+  constexpr float c[9] = {-0.4999990165233612f, 0.3332996070384979f,  -0.2495412975549698f,
+                          0.1967591792345047f,  -0.1530553102493286f, 0.106035515666008f,
+                          -0.05695851147174835f, 0.019850919023156166f, -0.003243904560804367f};
+  f2 q = pack2(c[8], c[8]);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) q = f2_fma(q, e, pack2(c[i], c[i]));
+  q = f2_fma(q, e, pack2(1.f, 1.f));
+  return f2_fma(q, e, pack2(max0(x0), max0(x1)));
+}
+
+// 1 / (1 + e^-x), to a few ulp at both ends; sigmoid_fast to about 1e-6, for
+// results that are rounded to 16 bits (2^-12 and more).
 __device__ __forceinline__ float sigmoid_exact(float x) {
   const float e = exp_neg(-fabsf(x));
   const float r = __fdividef(1.f, 1.f + e);
   return x >= 0.f ? r : e * r;
+}
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(-kLog2e * x)));
+  return r;
+}
+// The sigmoid for inputs and outputs of type T.
+template <typename T>
+__device__ __forceinline__ float sigmoid_t(float x) {
+  if constexpr (sizeof(T) == 4)
+    return sigmoid_exact(x);
+  else
+    return sigmoid_fast(x);
 }
 
 }  // namespace greta

@@ -9,19 +9,22 @@
 // What bounds it: one exponential per (token, channel, state). The SM's
 // special-function unit takes 16 a clock, so T D N / (148 * 16) clocks, three
 // times what the reads and writes need at N = 16. The other work per state
-// (three multiplications, two fused additions) is half of that on the fp32
-// pipe, issued two states an instruction.
+// (two multiplications, two fused additions) is half of that on the fp32 pipe,
+// issued for two channels an instruction.
 //
-// Split. A warp works alone: CHW = 128 / LN channels of one group and all
-// their states, LN lanes a channel and four states a lane (LN = N / 4 rounded
-// up to a power of two from 4 on), four channels a lane. So a lane keeps 16
-// states and their 16 decay rates in registers, a token's B and C are read by
-// four channels at a time, and sums over n take log2(LN) shuffles for four
+// Split. A warp works alone: LN lanes a channel with four states each (LN =
+// N / 4 rounded up to a power of two from 4 on) and KD channels a lane, so a
+// lane keeps 4 KD states and their decay rates in registers, a token's B and C
+// are read once for KD channels, and sums over n take log2(LN) shuffles for KD
 // channels together. The packed stream is cut into ranges by position
-// (ssm_common.cuh); a warp walks its range in tiles of 16 tokens: it loads the
-// tile's rows as vectors, computes (dt, dt u) once per token and channel into
-// shared memory, runs the recurrence from there, and applies skip and gate to
-// the tile's y, again as vectors.
+// (ssm_common.cuh); a warp walks its range in tiles of 8 tokens, whose rows are
+// copied to shared memory as vectors while the tile before is computed (the
+// copies hold no registers: loads that did were moved behind the computation,
+// and a third of the time was spent waiting for them); (dt, dt u) are computed
+// once per token and channel, the recurrence runs from shared memory, and skip
+// and gate are applied to the tile's y, again as vectors. Two channels of a
+// lane share an instruction, so dt, dt u, states and y are register pairs as
+// they come, and only B and C are doubled when they are widened.
 //
 // A range that begins inside a sequence needs the state at its first token.
 // The first kernel (kPhaseCarry) runs the recurrence of each range that such a
@@ -36,9 +39,9 @@
 
 namespace greta {
 
-constexpr int kTile = 16;        // tokens per tile, and per saved state
+constexpr int kTile = 8;         // tokens per tile, and per saved state
 constexpr int kLaneStates = 4;   // states per lane
-constexpr int kLaneChans = 4;    // channels per lane
+constexpr int kFwdChans = 4;     // channels per lane of the forward kernels
 constexpr int kScanWarps = 4;    // warps per CTA
 
 struct ScanParams {
@@ -58,7 +61,7 @@ struct ScanParams {
   // the carry holds a sequence start [R], copies of initial states [R][D][N]
   float *carry, *dsum, *hinit;
   int* reset;
-  float* ckpt;  // [T / 16 + 1][D][N]: state ahead of every 16th token, or null
+  float* ckpt;  // [T / 8 + 1][D][N]: state ahead of every 8th token, or null
   // cache-slot state (packed batches)
   float* state;
   long long s_slot, s_d, s_n, num_slots;
@@ -75,11 +78,12 @@ struct ScanParams {
 };
 
 // Which channels and states a lane has.
-template <int LN>
+template <int LN, int KD_ = kFwdChans>
 struct Lanes {
-  static constexpr int CHW = 128 / LN;  // channels per warp
+  static constexpr int KD = KD_;
+  static constexpr int CHW = 32 / LN * KD;  // channels per warp
   static constexpr int NP = LN * kLaneStates;
-  int lane, dg, nq;  // channel group of four and states' quarter
+  int lane, dg, nq;  // the lane's KD channels and its four states
   int f, c0, nch;    // group, first channel, channels of the slice
   __device__ __forceinline__ Lanes(const ScanParams& p, int slice, int lane_) {
     lane = lane_;
@@ -89,103 +93,101 @@ struct Lanes {
     c0 = f * p.Dg + (slice % p.spg) * CHW;
     nch = min(CHW, (f + 1) * p.Dg - c0);
   }
-  __device__ __forceinline__ int ch(int j) const { return dg * kLaneChans + j; }
+  __device__ __forceinline__ int ch(int j) const { return dg * KD + j; }
   __device__ __forceinline__ int n0() const { return nq * kLaneStates; }
 };
 
-// Values of a lane: [channel][pair of states]
-using LaneStates = f2[kLaneChans][kLaneStates / 2];
+// Values of a lane: [pair of channels][state]
+template <int KD>
+using LaneStates = f2[KD / 2][kLaneStates];
 
-// p[(c0 + ch) * N + n] of this lane (rows of N floats), zeros where there is
-// no such channel or state.
-template <int LN>
-__device__ __forceinline__ void load_states(const float* p, const Lanes<LN>& l, int N, float (&v)[4][4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool okc = l.ch(j) < l.nch;
-    const float* r = p + (long long)(l.c0 + l.ch(j)) * N + l.n0();
-    if (okc && N % 4 == 0 && l.n0() < N) {
-      const float4 x = *reinterpret_cast<const float4*>(r);
-      v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[j][i] = okc && l.n0() + i < N ? r[i] : 0.f;
-    }
+__device__ __forceinline__ void pack_pair(const float4& a, const float4& b, f2 (&h)[4]) {
+  h[0] = pack2(a.x, b.x);
+  h[1] = pack2(a.y, b.y);
+  h[2] = pack2(a.z, b.z);
+  h[3] = pack2(a.w, b.w);
+}
+__device__ __forceinline__ void unpack_pair(const f2 (&h)[4], float4& a, float4& b) {
+  unpack2(h[0], a.x, b.x);
+  unpack2(h[1], a.y, b.y);
+  unpack2(h[2], a.z, b.z);
+  unpack2(h[3], a.w, b.w);
+}
+
+// Up to four states (n of them, s apart; vec: one aligned float4), else zeros.
+__device__ __forceinline__ float4 load_four(const float* r, long long s, int n, bool vec) {
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vec) {
+    if (n > 0) x = *reinterpret_cast<const float4*>(r);
+  } else {
+    if (n > 0) x.x = r[0];
+    if (n > 1) x.y = r[s];
+    if (n > 2) x.z = r[2 * s];
+    if (n > 3) x.w = r[3 * s];
+  }
+  return x;
+}
+__device__ __forceinline__ void store_four(float* r, long long s, int n, bool vec, const float4& x) {
+  if (vec) {
+    if (n > 0) *reinterpret_cast<float4*>(r) = x;
+  } else {
+    if (n > 0) r[0] = x.x;
+    if (n > 1) r[s] = x.y;
+    if (n > 2) r[2 * s] = x.z;
+    if (n > 3) r[3 * s] = x.w;
   }
 }
 
-template <int LN>
-__device__ __forceinline__ void store_states(float* p, const Lanes<LN>& l, int N, const LaneStates& h) {
+// The lane's part of an fp32 [D, N] array with element strides (s_d, s_n).
+template <int LN, int KD>
+__device__ __forceinline__ void load_states(const float* p, const Lanes<LN, KD>& l, int N, long long s_d,
+                                            long long s_n, bool vec, LaneStates<KD>& h) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (l.ch(j) >= l.nch) continue;
-    float* r = p + (long long)(l.c0 + l.ch(j)) * N + l.n0();
-    float4 x;
-    unpack2(h[j][0], x.x, x.y);
-    unpack2(h[j][1], x.z, x.w);
-    if (N % 4 == 0) {
-      if (l.n0() < N) *reinterpret_cast<float4*>(r) = x;
-    } else {
-      const float v[4] = {x.x, x.y, x.z, x.w};
+  for (int j = 0; j < KD; j += 2) {
+    float4 x[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (l.n0() + i < N) r[i] = v[i];
-    }
+    for (int i = 0; i < 2; ++i)
+      x[i] = load_four(p + (l.c0 + l.ch(j + i)) * s_d + l.n0() * s_n, s_n, l.ch(j + i) < l.nch ? N - l.n0() : 0, vec);
+    pack_pair(x[0], x[1], h[j / 2]);
   }
 }
-
-__device__ __forceinline__ void pack_states(const float (&v)[4][4], LaneStates& h) {
+template <int LN, int KD>
+__device__ __forceinline__ void store_states(float* p, const Lanes<LN, KD>& l, int N, long long s_d, long long s_n,
+                                             bool vec, const LaneStates<KD>& h) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    h[j][0] = pack2(v[j][0], v[j][1]);
-    h[j][1] = pack2(v[j][2], v[j][3]);
+  for (int j = 0; j < KD; j += 2) {
+    float4 x[2];
+    unpack_pair(h[j / 2], x[0], x[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      store_four(p + (l.c0 + l.ch(j + i)) * s_d + l.n0() * s_n, s_n, l.ch(j + i) < l.nch ? N - l.n0() : 0, vec, x[i]);
   }
 }
+// ... contiguous, on 16-byte boundaries where N % 4 == 0.
+template <int LN, int KD>
+__device__ __forceinline__ void load_states(const float* p, const Lanes<LN, KD>& l, int N, LaneStates<KD>& h) {
+  load_states(p, l, N, N, 1, N % 4 == 0, h);
+}
+template <int LN, int KD>
+__device__ __forceinline__ void store_states(float* p, const Lanes<LN, KD>& l, int N, const LaneStates<KD>& h) {
+  store_states(p, l, N, N, 1, N % 4 == 0, h);
+}
 
-__device__ __forceinline__ void zero_states(LaneStates& h) {
+template <int KD>
+__device__ __forceinline__ void zero_states(LaneStates<KD>& h) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) h[j][0] = h[j][1] = 0ull;
+  for (int j = 0; j < KD / 2; ++j) h[j][0] = h[j][1] = h[j][2] = h[j][3] = 0ull;
 }
 
 // A slot's states of this lane, through the cache's strides.
-template <int LN>
-__device__ __forceinline__ void load_slot(const ScanParams& p, int slot, const Lanes<LN>& l, LaneStates& h) {
-  const float* b = p.state + slot * p.s_slot;
-  float v[4][4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool okc = l.ch(j) < l.nch;
-    const float* r = b + (l.c0 + l.ch(j)) * p.s_d + l.n0() * p.s_n;
-    if (p.st_vec && okc && l.n0() < p.N) {
-      const float4 x = *reinterpret_cast<const float4*>(r);
-      v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[j][i] = okc && l.n0() + i < p.N ? r[i * p.s_n] : 0.f;
-    }
-  }
-  pack_states(v, h);
+template <int LN, int KD>
+__device__ __forceinline__ void load_slot(const ScanParams& p, int slot, const Lanes<LN, KD>& l, LaneStates<KD>& h) {
+  load_states(p.state + slot * p.s_slot, l, p.N, p.s_d, p.s_n, p.st_vec, h);
 }
-
-template <int LN>
-__device__ __forceinline__ void store_slot(const ScanParams& p, int slot, const Lanes<LN>& l, const LaneStates& h) {
-  float* b = p.state + slot * p.s_slot;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (l.ch(j) >= l.nch) continue;
-    float* r = b + (l.c0 + l.ch(j)) * p.s_d + l.n0() * p.s_n;
-    float4 x;
-    unpack2(h[j][0], x.x, x.y);
-    unpack2(h[j][1], x.z, x.w);
-    if (p.st_vec) {
-      if (l.n0() < p.N) *reinterpret_cast<float4*>(r) = x;
-    } else {
-      const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (l.n0() + i < p.N) r[i * p.s_n] = v[i];
-    }
-  }
+template <int LN, int KD>
+__device__ __forceinline__ void store_slot(const ScanParams& p, int slot, const Lanes<LN, KD>& l,
+                                           const LaneStates<KD>& h) {
+  store_states(p.state + slot * p.s_slot, l, p.N, p.s_d, p.s_n, p.st_vec, h);
 }
 
 // The request's slot, or -1 for none (negative or out of range, which is
@@ -197,84 +199,152 @@ __device__ __forceinline__ int slot_of(const ScanParams& p, int s, bool flag) {
   return raw >= 0 && raw < p.num_slots ? raw : -1;
 }
 
-// Vectors of a tile: V channels of a token's row, NVEC of them per lane.
-template <int LN>
+// A tile's rows of channels as vectors: V channels of a token, NVEC of them per
+// lane.
+template <int CHW>
 struct TileVecs {
-  static constexpr int CHW = Lanes<LN>::CHW;
-  static constexpr int V = CHW < 8 ? CHW : 8;
+  static constexpr int V = CHW < 4 ? CHW : (kTile * CHW >= 256 ? 8 : 4);
   static constexpr int VPR = CHW / V;  // vectors per row
   static constexpr int COUNT = kTile * VPR;
   static constexpr int NVEC = (COUNT + 31) / 32;
+  // vector k of a lane: its row and first channel
+  static __device__ __forceinline__ bool has(int k, int lane) { return COUNT % 32 == 0 || k * 32 + lane < COUNT; }
+  static __device__ __forceinline__ int row(int k, int lane) { return (k * 32 + lane) / VPR; }
+  static __device__ __forceinline__ int chan(int lane) { return lane % VPR * V; }
 };
 
-// Shared memory of a warp, in floats.
-template <int LN>
-struct FwdSmem {
-  static constexpr int kDl = kTile * Lanes<LN>::CHW * 2;  // (dt, dt u)
-  static constexpr int kY = kTile * Lanes<LN>::CHW;
-  static constexpr int kBC = kTile * Lanes<LN>::NP * 2;   // [token][B | C]
-  static constexpr int kWarp = kDl + kY + kBC;
-};
-
-template <typename T, int LN>
-__device__ __forceinline__ void stage_bc(const ScanParams& p, const Lanes<LN>& l, int tile0, int ta, int tb,
-                                         float* bc, bool with_c) {
-  constexpr int NP = Lanes<LN>::NP;
-  const T* bg = reinterpret_cast<const T*>(p.B) + (long long)l.f * p.N;
-  const T* cg = reinterpret_cast<const T*>(p.C) + (long long)l.f * p.N;
-  // four states at a time
-  for (int i = l.lane; i < kTile * LN * 2; i += 32) {
-    const int which = i / (kTile * LN);
-    const int r = (i / LN) % kTile, n = (i % LN) * 4, t = tile0 + r;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (t >= ta && t < tb && (which == 0 || with_c)) {
-      const T* s = (which == 0 ? bg + (long long)t * p.ldb : cg + (long long)t * p.ldc) + n;
-      const Pack<T, 4> v = load_part<T, 4>(s, p.N - n, p.vec_bc && n < p.N);
-      o = make_float4(to_f(v.v[0]), to_f(v.v[1]), to_f(v.v[2]), to_f(v.v[3]));
-    }
-    *reinterpret_cast<float4*>(bc + (r * 2 + which) * NP + n) = o;
-  }
-}
-
-__device__ __forceinline__ float step_size(const ScanParams& p, float raw) { return p.softplus ? softplusf_(raw) : raw; }
-
-// One token of the recurrence for the lane's states; y[j] += the lane's part
-// of sum_n C h.
-template <bool WITH_Y>
-__device__ __forceinline__ void scan_step(LaneStates& h, const LaneStates& A2, const float2 (&dl)[4], float4 b,
-                                          float4 c, float (&y)[4]) {
-  const f2 b2[2] = {pack2(b.x, b.y), pack2(b.z, b.w)};
-  const f2 c2[2] = {pack2(c.x, c.y), pack2(c.z, c.w)};
+// Rows [ta, tb) of a tile of a [T, D] operand into shared memory ([token][CHW]);
+// zeros elsewhere. A lane copies the vectors that it reads itself.
+template <typename T, int LN, int KD>
+__device__ __forceinline__ void copy_tile(const void* base, long long ld, bool vec, const Lanes<LN, KD>& l, int tile0,
+                                          int ta, int tb, T* s) {
+  constexpr int CHW = Lanes<LN, KD>::CHW;
+  using TV = TileVecs<CHW>;
+  const T* b = reinterpret_cast<const T*>(base);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const f2 d = pack2(dl[j].x, dl[j].x), du = pack2(dl[j].y, dl[j].y);
-    const f2 a0 = f2_ex2(f2_mul(d, A2[j][0])), a1 = f2_ex2(f2_mul(d, A2[j][1]));
-    h[j][0] = f2_fma(a0, h[j][0], f2_mul(du, b2[0]));
-    h[j][1] = f2_fma(a1, h[j][1], f2_mul(du, b2[1]));
-    if (WITH_Y) y[j] = f2_sum(f2_fma(c2[0], h[j][0], f2_mul(c2[1], h[j][1])));
+  for (int k = 0; k < TV::NVEC; ++k) {
+    if (!TV::has(k, l.lane)) continue;
+    const int r = TV::row(k, l.lane), t = tile0 + r, c = TV::chan(l.lane);
+    const int n = t >= ta && t < tb ? l.nch - c : 0;
+    copy_part<T, TV::V>(s + r * CHW + c, b + t * ld + l.c0 + c, b, n, vec && n >= TV::V);
   }
 }
 
-// y[j] summed over the LN lanes of the channels; lane nq of the group keeps
-// channel (bit 0 of nq) * 2 + (bit 1 of nq).
+// A lane's vector k of a tile in shared memory.
+template <typename T, int CHW>
+__device__ __forceinline__ Pack<T, TileVecs<CHW>::V> tile_vec(const T* s, int k, int lane) {
+  using TV = TileVecs<CHW>;
+  return load_part<T, TV::V>(s + TV::row(k, lane) * CHW + TV::chan(lane), TV::V, true);
+}
+
+// B and C of a tile into shared memory, [token][B | C][states], by `lanes`
+// lanes of which this is number `at`.
+template <typename T, int LN, int KD>
+__device__ __forceinline__ void copy_bc(const ScanParams& p, const Lanes<LN, KD>& l, int tile0, int ta, int tb, T* s,
+                                        int at, int lanes) {
+  const T* bg = reinterpret_cast<const T*>(p.B);
+  const T* cg = reinterpret_cast<const T*>(p.C);
+#pragma unroll
+  for (int i = at; i < kTile * 2 * LN; i += lanes) {
+    const int n = i % LN * 4, t = tile0 + i / (2 * LN);
+    const bool b = i / LN % 2 == 0;
+    const T* base = b ? bg : cg;
+    copy_part<T, 4>(s + i * 4, base + t * (b ? p.ldb : p.ldc) + (long long)l.f * p.N + n, base,
+                    t >= ta && t < tb ? p.N - n : 0, p.vec_bc);
+  }
+}
+
+// Four states of B or C in fp32, each twice (for two channels).
+template <typename T>
+__device__ __forceinline__ void read_four(const T* s, f2 (&o)[4]) {
+  const Pack<T, 4> v = load_part<T, 4>(s, 4, true);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = pack2(to_f(v.v[i]), to_f(v.v[i]));
+}
+
+__device__ __forceinline__ f2 step_sizes(const ScanParams& p, float x0, float x1) {
+  return p.softplus ? softplus2(x0, x1) : pack2(x0, x1);
+}
+
+// One token of the recurrence for the lane's states, dl = (dt, dt u) of its
+// pairs of channels; y: the lane's part of sum_n C h.
+template <bool WITH_Y, int KD>
+__device__ __forceinline__ void scan_step(LaneStates<KD>& h, const LaneStates<KD>& A2, const ulonglong2 (&dl)[KD / 2],
+                                          const f2 (&b)[4], const f2 (&c)[4], f2 (&y)[KD / 2]) {
+#pragma unroll
+  for (int j = 0; j < KD / 2; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f2 a = f2_ex2(f2_mul(dl[j].x, A2[j][i]));
+      h[j][i] = f2_fma(a, h[j][i], f2_mul(dl[j].y, b[i]));
+      if (WITH_Y) y[j] = i == 0 ? f2_mul(c[i], h[j][i]) : f2_fma(c[i], h[j][i], y[j]);
+    }
+  }
+}
+
+// v (pairs of channels) summed over the LN lanes of the channels: the first
+// exchanges give each lane one channel, sum_channel, the rest add it up. Lanes
+// with nq < KD hold the sums.
 template <int LN>
-__device__ __forceinline__ float sum_over_states(const float (&y)[4], int lane) {
+__device__ __forceinline__ float sum_over_states(const f2 (&v)[2], int lane) {
   const bool b0 = lane & 1, b1 = lane & 2;
-  const float s0 = (b0 ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, b0 ? y[0] : y[2], 1);
-  const float s1 = (b0 ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, b0 ? y[1] : y[3], 1);
-  float s = (b1 ? s1 : s0) + __shfl_xor_sync(0xffffffffu, b1 ? s0 : s1, 2);
+  float k0, k1, s0, s1;
+  unpack2(b0 ? v[1] : v[0], k0, k1);
+  unpack2(b0 ? v[0] : v[1], s0, s1);
+  k0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+  k1 += __shfl_xor_sync(0xffffffffu, s1, 1);
+  float s = (b1 ? k1 : k0) + __shfl_xor_sync(0xffffffffu, b1 ? k0 : k1, 2);
 #pragma unroll
   for (int o = 4; o < LN; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
-__device__ __forceinline__ int sum_channel(int lane) { return (lane & 1) * 2 + ((lane >> 1) & 1); }
-
-// The state at the start of range i, which lies inside a sequence that began
-// in range j0 < i (j0: the last range whose carry holds a sequence start).
 template <int LN>
-__device__ __forceinline__ void carry_in(const ScanParams& p, const Lanes<LN>& l, int i, const LaneStates& A2,
-                                         LaneStates& h) {
-  int j0 = i - 1;
+__device__ __forceinline__ float sum_over_states(const f2 (&v)[1], int lane) {
+  const bool b0 = lane & 1;
+  float v0, v1;
+  unpack2(v[0], v0, v1);
+  float s = (b0 ? v1 : v0) + __shfl_xor_sync(0xffffffffu, b0 ? v0 : v1, 1);
+#pragma unroll
+  for (int o = 2; o < LN; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+template <int KD>
+__device__ __forceinline__ int sum_channel(int lane) {
+  return KD == 4 ? (lane & 1) * 2 + ((lane >> 1) & 1) : lane & 1;
+}
+
+// A state (or adjoint) brought through the ranges `from`, .., `to` (in that
+// direction): the first one's carry, then carry + exp(A sum dt) times what came.
+template <int LN, int KD>
+__device__ __forceinline__ void carry_through(const ScanParams& p, const Lanes<LN, KD>& l, int from, int to, int step,
+                                              const LaneStates<KD>& A2, LaneStates<KD>& h) {
+  const long long DN = (long long)p.D * p.N;
+  zero_states<KD>(h);
+#pragma unroll 2
+  for (int j = from; j != to + step; j += step) {
+    LaneStates<KD> s;
+    load_states(p.carry + j * DN, l, p.N, s);
+#pragma unroll
+    for (int c = 0; c < KD / 2; ++c) {
+      float d[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int ch = l.ch(2 * c + i);
+        d[i] = ch < l.nch ? p.dsum[(long long)j * p.D + l.c0 + ch] : 0.f;
+      }
+      const f2 d2 = pack2(d[0], d[1]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) h[c][k] = f2_fma(f2_ex2(f2_mul(d2, A2[c][k])), h[c][k], s[c][k]);
+    }
+  }
+}
+
+// The state at the start of range i, which lies inside a sequence: from the
+// last range before whose carry holds that sequence's start.
+template <int LN, int KD>
+__device__ __forceinline__ void carry_in(const ScanParams& p, const Lanes<LN, KD>& l, int i, const LaneStates<KD>& A2,
+                                         LaneStates<KD>& h) {
+  int j0 = 0;
   for (int hi = i - 1; hi >= 0; hi -= 32) {
     const int k = hi - l.lane;
     const unsigned m = __ballot_sync(0xffffffffu, k >= 0 && p.reset[k] != 0);
@@ -282,120 +352,139 @@ __device__ __forceinline__ void carry_in(const ScanParams& p, const Lanes<LN>& l
       j0 = hi - (__ffs(m) - 1);
       break;
     }
-    j0 = max(0, hi - 31);
   }
-  const long long DN = (long long)p.D * p.N;
-  zero_states(h);
-  for (int j = j0; j < i; ++j) {
-    float s[4][4];
-    load_states(p.carry + j * DN, l, p.N, s);
-    LaneStates s2;
-    pack_states(s, s2);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float d = l.ch(c) < l.nch && j > j0 ? p.dsum[(long long)j * p.D + l.c0 + l.ch(c)] : 0.f;
-      const f2 d2 = pack2(d, d);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) h[c][k] = f2_fma(f2_ex2(f2_mul(d2, A2[c][k])), h[c][k], s2[c][k]);
-    }
-  }
+  carry_through(p, l, j0, i - 1, 1, A2, h);
 }
 
-template <int LN>
-__device__ __forceinline__ void load_rates(const ScanParams& p, const Lanes<LN>& l, LaneStates& A2) {
-  float v[4][4];
-  load_states(p.A, l, p.N, v);
+// A log2(e): decays are 2^(dt A2).
+template <int LN, int KD>
+__device__ __forceinline__ void load_rates(const ScanParams& p, const Lanes<LN, KD>& l, LaneStates<KD>& A2) {
+  load_states(p.A, l, p.N, A2);
+  const f2 e = pack2(kLog2e, kLog2e);
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < KD / 2; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[j][i] *= kLog2e;
-  pack_states(v, A2);
+    for (int i = 0; i < 4; ++i) A2[j][i] = f2_mul(A2[j][i], e);
 }
 
-// (dt, dt u) of a tile into shared memory; rows outside [ta, tb) and channels
-// that are not there get zeros (a decay of 1 and no input).
-template <typename T, int LN>
-__device__ __forceinline__ void stage_steps(const ScanParams& p, const Lanes<LN>& l, int tile0, int ta, int tb,
-                                            float* dl, Pack<T, TileVecs<LN>::V> (&u)[TileVecs<LN>::NVEC]) {
-  using TV = TileVecs<LN>;
-  constexpr int V = TV::V, CHW = TV::CHW;
+// A per-channel operand for the lane's vector column (zeros without one).
+template <int V>
+__device__ __forceinline__ void load_column(const float* v, int c0, int n, float (&o)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = v != nullptr && e < n ? v[c0 + e] : 0.f;
+}
+
+// Bits of the tile's rows [ta, tb).
+__device__ __forceinline__ unsigned tile_rows(int tile0, int ta, int tb) {
+  return ((1u << (tb - ta)) - 1) << (ta - tile0);
+}
+
+// (dt, dt u) of a tile into shared memory, [token][pair of channels] as (dt0,
+// dt1, dt0 u0, dt1 u1). Rows without their bit and channels that are not there
+// get zeros: a decay of 1 and no input.
+template <typename T, int LN, int KD>
+__device__ __forceinline__ void stage_steps(const ScanParams& p, const Lanes<LN, KD>& l, unsigned rows, const T* u,
+                                            const T* d, const float (&bias)[TileVecs<Lanes<LN, KD>::CHW>::V],
+                                            float4* dl) {
+  constexpr int CHW = Lanes<LN, KD>::CHW;
+  using TV = TileVecs<CHW>;
+  constexpr int V = TV::V;
 #pragma unroll
   for (int k = 0; k < TV::NVEC; ++k) {
-    const int i = k * 32 + l.lane;
-    if (TV::COUNT % 32 != 0 && i >= TV::COUNT) continue;
-    const int r = i / TV::VPR, c = (i % TV::VPR) * V, t = tile0 + r;
-    const int n = l.nch - c;
-    zero(u[k]);
-    float2 o[V];
+    if (!TV::has(k, l.lane)) continue;
+    const int r = TV::row(k, l.lane), c = TV::chan(l.lane);
+    const bool in = (rows >> r) & 1;
+    const Pack<T, V> uv = tile_vec<T, CHW>(u, k, l.lane), dv = tile_vec<T, CHW>(d, k, l.lane);
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = make_float2(0.f, 0.f);
-    if (t >= ta && t < tb && n > 0) {
-      const bool vec = p.vec && n >= V;
-      u[k] = load_part<T, V>(reinterpret_cast<const T*>(p.u) + t * p.ldu + l.c0 + c, n, vec);
-      const Pack<T, V> d = load_part<T, V>(reinterpret_cast<const T*>(p.delta) + t * p.ldd + l.c0 + c, n, vec);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (e < n) {
-          const float bias = p.dbias != nullptr ? p.dbias[l.c0 + c + e] : 0.f;
-          const float s = step_size(p, to_f(d.v[e]) + bias);
-          o[e] = make_float2(s, s * to_f(u[k].v[e]));
-        }
-      }
+    for (int e = 0; e < V; e += 2) {
+      const f2 s = step_sizes(p, to_f(dv.v[e]) + bias[e], to_f(dv.v[e + 1]) + bias[e + 1]);
+      const f2 x = f2_mul(s, pack2(to_f(uv.v[e]), to_f(uv.v[e + 1])));
+      float4 o;
+      unpack2(s, o.x, o.y);
+      unpack2(x, o.z, o.w);
+      const bool c0 = in && c + e < l.nch, c1 = in && c + e + 1 < l.nch;
+      dl[(r * CHW + c + e) / 2] = make_float4(c0 ? o.x : 0.f, c1 ? o.y : 0.f, c0 ? o.z : 0.f, c1 ? o.w : 0.f);
     }
-    float4* w = reinterpret_cast<float4*>(dl + (r * CHW + c) * 2);
-#pragma unroll
-    for (int e = 0; e < V; e += 2) w[e / 2] = make_float4(o[e].x, o[e].y, o[e + 1].x, o[e + 1].y);
   }
 }
 
-template <int LN>
-__device__ __forceinline__ void read_steps(const float* dl, const Lanes<LN>& l, int r, float2 (&v)[4]) {
-  const float4* s = reinterpret_cast<const float4*>(dl + (r * Lanes<LN>::CHW + l.ch(0)) * 2);
-  const float4 a = s[0], b = s[1];
-  v[0] = make_float2(a.x, a.y);
-  v[1] = make_float2(a.z, a.w);
-  v[2] = make_float2(b.x, b.y);
-  v[3] = make_float2(b.z, b.w);
+template <int KD>
+__device__ __forceinline__ void read_steps(const float4* dl, int at, ulonglong2 (&v)[KD / 2]) {
+  const ulonglong2* s = reinterpret_cast<const ulonglong2*>(dl + at / 2);
+#pragma unroll
+  for (int j = 0; j < KD / 2; ++j) v[j] = s[j];
 }
+
+// The sums of dt of a range.
+template <int LN, int KD>
+__device__ __forceinline__ void store_sums(const ScanParams& p, const Lanes<LN, KD>& l, int range,
+                                           const f2 (&dsum)[KD / 2]) {
+#pragma unroll
+  for (int j = 0; j < KD; ++j) {
+    float v[2];
+    unpack2(dsum[j / 2], v[0], v[1]);
+    if (l.ch(j) < l.nch) p.dsum[(long long)range * p.D + l.c0 + l.ch(j)] = v[j % 2];
+  }
+}
+
+// Shared memory of a warp of the forward, in bytes.
+template <typename T, int LN, int KD>
+struct FwdSmem {
+  static constexpr int CHW = Lanes<LN, KD>::CHW;
+  static constexpr int kDl = kTile * CHW * 8;  // (dt, dt u)
+  static constexpr int kY = kTile * CHW * 4;
+  static constexpr int kRow = kTile * CHW * (int)sizeof(T);        // a tile of an operand
+  static constexpr int kBC = kTile * 2 * LN * 4 * (int)sizeof(T);  // [token][B | C]
+  static constexpr int kStage = 3 * kRow + kBC;                    // u, delta, gate; B, C
+  static constexpr int kWarp = kDl + kY + 2 * kStage;
+};
 
 // kPhaseCarry: the end state and sum of dt of a range that a range inside the
 // same sequence follows. kPhaseMain: outputs, saved states, slots.
 enum ScanPhase { kPhaseCarry = 0, kPhaseMain = 1 };
 
 template <typename T, int LN, int PHASE>
-__global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_fwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const ScanParams p) {
   extern __shared__ float4 smem4[];
-  using TV = TileVecs<LN>;
-  constexpr int CHW = TV::CHW, V = TV::V, NP = Lanes<LN>::NP;
+  constexpr int KD = kFwdChans;
+  using L = Lanes<LN, KD>;
+  using S = FwdSmem<T, LN, KD>;
+  constexpr int CHW = L::CHW, NP = L::NP;
+  using TV = TileVecs<CHW>;
+  constexpr int V = TV::V;
+  constexpr bool kMain = PHASE == kPhaseMain;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* dl = reinterpret_cast<float*>(smem4) + warp * FwdSmem<LN>::kWarp;
-  float* ys = dl + FwdSmem<LN>::kDl;
-  float* bc = ys + FwdSmem<LN>::kY;
+  char* mine = reinterpret_cast<char*>(smem4) + warp * S::kWarp;
+  float4* dl = reinterpret_cast<float4*>(mine);
+  float* ys = reinterpret_cast<float*>(mine + S::kDl);
+  auto stage = [&](int s, int part) {  // part: u, delta, gate, (B, C)
+    return reinterpret_cast<T*>(mine + S::kDl + S::kY + s * S::kStage + part * S::kRow);
+  };
   pdl_wait();
   pdl_trigger();
   const int slice = blockIdx.x * (blockDim.x >> 5) + warp;
   if (slice >= p.F * p.spg) return;
-  const Lanes<LN> l(p, slice, lane);
+  const L l(p, slice, lane);
   const int ri = blockIdx.y;
   int t0 = range_begin(p.q, ri, p.R, p.L, lane);
   const int t1 = range_begin(p.q, ri + 1, p.R, p.L, lane);
-  if (t0 >= t1 && PHASE == kPhaseMain) return;
+  if (t0 >= t1) return;
 
-  LaneStates A2, h;
-  load_rates(p, l, A2);
-  zero_states(h);
+  LaneStates<KD> A2, h;
   const long long DN = (long long)p.D * p.N;
-  float dsum[4] = {0.f, 0.f, 0.f, 0.f};
   Seg g;
-  if (PHASE == kPhaseCarry) {
-    if (ri + 1 >= p.R || t1 >= p.q.T) return;
+  int slot = -1;
+  if (!kMain) {
+    if (t1 >= p.q.T) return;
     g = seg_at(p.q, t1, lane);
     if (!g.in || g.b >= t1) return;  // the next range begins with a sequence, or outside
+    load_rates(p, l, A2);
+    zero_states<KD>(h);
     const bool reset = g.b >= t0;
     if (slice == 0 && lane == 0) p.reset[ri] = reset;
     if (reset) {
       t0 = g.b;
-      const int slot = slot_of(p, g.s, false);
+      slot = slot_of(p, g.s, false);
       if (slot >= 0 && p.initial[g.s] != 0) {
         load_slot(p, slot, l, h);
         store_states(p.hinit + ri * DN, l, p.N, h);
@@ -403,101 +492,111 @@ __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_fwd_kernel(const Sca
     }
   } else {
     g = seg_at(p.q, t0, lane);
-    if (g.in && g.b < t0) carry_in(p, l, ri, A2, h);
+    load_rates(p, l, A2);
+    zero_states<KD>(h);
+    if (g.in && g.b < t0) {
+      carry_in(p, l, ri, A2, h);
+      slot = slot_of(p, g.s, false);
+    }
   }
-  int slot = -1;
-  if (PHASE == kPhaseMain && g.in && g.b < t0) slot = slot_of(p, g.s, false);
+  float bias[V], skip[V];
+  load_column<V>(p.dbias, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), bias);
+  if (kMain) load_column<V>(p.skip, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), skip);
+  f2 dsum[KD / 2];
+#pragma unroll
+  for (int j = 0; j < KD / 2; ++j) dsum[j] = 0ull;
 
-  for (int tile0 = t0 / kTile * kTile; tile0 < t1; tile0 += kTile) {
+  int cur = 0;
+  const T* bc;
+  auto fetch = [&](int tile0, int s) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
-    Pack<T, V> u[TV::NVEC];
-    stage_steps<T, LN>(p, l, tile0, ta, tb, dl, u);
-    stage_bc<T, LN>(p, l, tile0, ta, tb, bc, PHASE == kPhaseMain);
+    copy_tile<T>(p.u, p.ldu, p.vec, l, tile0, ta, tb, stage(s, 0));
+    copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
+    if (kMain && p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
+    copy_bc<T>(p, l, tile0, ta, tb, stage(s, 3), lane, 32);
+    copy_commit();
+  };
+  // token r of the tile
+  auto step = [&](int r) {
+    ulonglong2 dv[KD / 2];
+    f2 b[4], c[4], y[KD / 2];
+    read_steps<KD>(dl, r * CHW + l.ch(0), dv);
+    read_four(bc + r * 2 * NP + l.n0(), b);
+    if (kMain) read_four(bc + (r * 2 + 1) * NP + l.n0(), c);
+    scan_step<kMain, KD>(h, A2, dv, b, c, y);
+    if (kMain) {
+      const float s = sum_over_states<LN>(y, lane);
+      if (l.nq < KD) ys[r * CHW + l.ch(sum_channel<KD>(lane))] = s;
+    } else {
+#pragma unroll
+      for (int j = 0; j < KD / 2; ++j) dsum[j] = f2_add(dsum[j], dv[j].x);
+    }
+  };
+
+  fetch(t0 / kTile * kTile, 0);
+  for (int tile0 = t0 / kTile * kTile; tile0 < t1; tile0 += kTile, cur ^= 1) {
+    const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
+    copy_wait();
+    bc = stage(cur, 3);
+    stage_steps<T>(p, l, tile_rows(tile0, ta, tb), stage(cur, 0), stage(cur, 1), bias, dl);
     __syncwarp();
-    if (PHASE == kPhaseMain && p.ckpt != nullptr && ta == tile0)
-      store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
+    // (the other stage's B and C were last read ahead of the barrier before)
+    if (tile0 + kTile < t1) fetch(tile0 + kTile, cur ^ 1);
+    if (kMain && p.ckpt != nullptr && ta == tile0) store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
     unsigned live = 0;  // tokens of the tile that a sequence holds
     int t = ta;
     while (t < tb) {
       const int stop = min(g.e, tb);
       if (g.in) {
-        if (PHASE == kPhaseMain && t == g.b) {
-          zero_states(h);
+        if (kMain && t == g.b) {
+          zero_states<KD>(h);
           slot = slot_of(p, g.s, slice == 0 && lane == 0);
           if (slot >= 0 && p.initial[g.s] != 0) {
             // a sequence that goes on in a later range: its last range may have
             // written the slot by now, so the copy of the first kernel
-            if (g.e > t1) {
-              float v[4][4];
-              load_states(p.hinit + ri * DN, l, p.N, v);
-              pack_states(v, h);
-            } else {
+            if (g.e > t1)
+              load_states(p.hinit + ri * DN, l, p.N, h);
+            else
               load_slot(p, slot, l, h);
-            }
           }
         }
-#pragma unroll 2
-        for (int r = t - tile0; r < stop - tile0; ++r) {
-          float2 d[4];
-          read_steps(dl, l, r, d);
-          const float4 b = *reinterpret_cast<const float4*>(bc + (r * 2) * NP + l.n0());
-          float y[4];
-          if (PHASE == kPhaseMain) {
-            const float4 c = *reinterpret_cast<const float4*>(bc + (r * 2 + 1) * NP + l.n0());
-            scan_step<true>(h, A2, d, b, c, y);
-            const float s = sum_over_states<LN>(y, lane);
-            if (l.nq < 4) ys[r * CHW + l.ch(sum_channel(lane))] = s;
-          } else {
-            scan_step<false>(h, A2, d, b, b, y);
+        if (stop - t == kTile) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dsum[j] += d[j].x;
-          }
+          for (int r = 0; r < kTile; ++r) step(r);
+        } else {
+          for (int r = t - tile0; r < stop - tile0; ++r) step(r);
         }
-        live |= (0xffffu >> (kTile - (stop - t))) << (t - tile0);
-        if (PHASE == kPhaseMain && stop == g.e && slot >= 0) store_slot(p, slot, l, h);
+        live |= tile_rows(tile0, t, stop);
+        if (kMain && stop == g.e && slot >= 0) store_slot(p, slot, l, h);
       }
       t = stop;
       if (t == g.e && t < t1) g = seg_next(p.q, g);
     }
     __syncwarp();
-    if (PHASE == kPhaseMain) {
+    if (kMain) {
 #pragma unroll
       for (int k = 0; k < TV::NVEC; ++k) {
-        const int i = k * 32 + lane;
-        if (TV::COUNT % 32 != 0 && i >= TV::COUNT) continue;
-        const int r = i / TV::VPR, c = (i % TV::VPR) * V, tt = tile0 + r;
-        const int n = l.nch - c;
-        if (tt < ta || tt >= tb || n <= 0) continue;
+        const int r = TV::row(k, lane), c = TV::chan(lane), tt = tile0 + r, n = l.nch - c;
+        if (!TV::has(k, lane) || tt < ta || tt >= tb || n <= 0) continue;
         const bool in = (live >> r) & 1;
         if (!in && !p.zero_rest) continue;
-        const bool vec = p.vec && n >= V;
-        Pack<T, V> o;
-        zero(o);
-        if (in) {
-          Pack<T, V> z;
-          if (p.gate != nullptr)
-            z = load_part<T, V>(reinterpret_cast<const T*>(p.gate) + tt * p.ldg + l.c0 + c, n, vec);
+        const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane);
+        const Pack<float, V> y = load_part<float, V>(ys + r * CHW + c, V, true);
+        Pack<T, V> z, o;
+        if (p.gate != nullptr) z = tile_vec<T, CHW>(stage(cur, 2), k, lane);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (e < n) {
-              float y = ys[r * CHW + c + e];
-              if (p.skip != nullptr) y = fmaf(p.skip[l.c0 + c + e], to_f(u[k].v[e]), y);
-              if (p.gate != nullptr) y *= to_f(z.v[e]) * sigmoid_exact(to_f(z.v[e]));
-              o.v[e] = from_f<T>(y);
-            }
-          }
+        for (int e = 0; e < V; ++e) {
+          float v = fmaf(skip[e], to_f(u.v[e]), y.v[e]);
+          if (p.gate != nullptr) v *= to_f(z.v[e]) * sigmoid_t<T>(to_f(z.v[e]));
+          o.v[e] = from_f<T>(in ? v : 0.f);
         }
-        store_part<T, V>(reinterpret_cast<T*>(p.out) + (long long)tt * p.D + l.c0 + c, o, n, vec);
+        store_part<T, V>(reinterpret_cast<T*>(p.out) + (long long)tt * p.D + l.c0 + c, o, n, p.vec && n >= V);
       }
     }
   }
-  if (PHASE == kPhaseCarry) {
+  if (!kMain) {
     store_states(p.carry + ri * DN, l, p.N, h);
-    if (l.nq == 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (l.ch(j) < l.nch) p.dsum[(long long)ri * p.D + l.c0 + l.ch(j)] = dsum[j];
-    }
+    if (l.nq == 0) store_sums(p, l, ri, dsum);
   }
 }
 
@@ -511,10 +610,11 @@ __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = blockIdx.x * (blockDim.x >> 5) + warp;
   if (slice >= p.F * p.spg) return;
-  const Lanes<LN> l(p, slice, lane);
+  constexpr int KD = kFwdChans;
+  const Lanes<LN, KD> l(p, slice, lane);
   // the channel whose step and output this lane computes
-  const int cj = l.ch(sum_channel(lane));
-  const bool mine = l.nq < 4 && cj < l.nch;
+  const int cj = l.ch(sum_channel<KD>(lane));
+  const bool mine = l.nq < KD && cj < l.nch;
   const int c = l.c0 + cj;
   const T* ug = reinterpret_cast<const T*>(p.u);
   const T* dg = reinterpret_cast<const T*>(p.delta);
@@ -524,11 +624,11 @@ __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const 
   T* og = reinterpret_cast<T*>(p.out);
   pdl_wait();
   pdl_trigger();
-  LaneStates A2;
+  LaneStates<KD> A2;
   load_rates(p, l, A2);
   const float bias = p.dbias != nullptr && mine ? p.dbias[c] : 0.f;
   const float skip = p.skip != nullptr && mine ? p.skip[c] : 0.f;
-  LaneStates h[RQ];
+  LaneStates<KD> h[RQ];
   int tb[RQ], te[RQ], slot[RQ];
   struct Row {
     T u, d, z;
@@ -551,7 +651,7 @@ __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const 
     tb[q] = ok ? seq_start(p.q, r) : 0;
     te[q] = ok ? seq_start(p.q, r + 1) : 0;
     slot[q] = tb[q] < te[q] ? slot_of(p, r, slice == 0 && lane == 0) : -1;
-    zero_states(h[q]);
+    zero_states<KD>(h[q]);
     if (slot[q] >= 0 && p.initial[r] != 0) load_slot(p, slot[q], l, h[q]);
     if (tb[q] < te[q]) load_row(tb[q], row[q]);
   }
@@ -559,28 +659,34 @@ __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const 
   for (int q = 0; q < RQ; ++q) {
     for (int t = tb[q]; t < te[q]; ++t) {
       if (t > tb[q]) load_row(t, row[q]);
-      float2 own = make_float2(0.f, 0.f);
       const float u = mine ? to_f(row[q].u) : 0.f;
-      if (mine) {
-        own.x = step_size(p, to_f(row[q].d) + bias);
-        own.y = own.x * u;
-      }
-      float2 d[4];
+      float dt = 0.f, other;
+      if (mine) unpack2(step_sizes(p, to_f(row[q].d) + bias, 0.f), dt, other);
+      ulonglong2 d[KD / 2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // channel j's lane: sum_channel is its own inverse on two bits
-        const int src = l.dg * LN + sum_channel(j);
-        d[j].x = __shfl_sync(0xffffffffu, own.x, src);
-        d[j].y = __shfl_sync(0xffffffffu, own.y, src);
+      for (int j = 0; j < KD / 2; ++j) {
+        float s[2], x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // that channel's lane: sum_channel is its own inverse
+          const int src = l.dg * LN + sum_channel<KD>(2 * j + i);
+          s[i] = __shfl_sync(0xffffffffu, dt, src);
+          x[i] = __shfl_sync(0xffffffffu, dt * u, src);
+        }
+        d[j].x = pack2(s[0], s[1]);
+        d[j].y = pack2(x[0], x[1]);
       }
-      const Pack<T, 4>&b = row[q].b, &cc = row[q].c;
-      float y[4];
-      scan_step<true>(h[q], A2, d, make_float4(to_f(b.v[0]), to_f(b.v[1]), to_f(b.v[2]), to_f(b.v[3])),
-                      make_float4(to_f(cc.v[0]), to_f(cc.v[1]), to_f(cc.v[2]), to_f(cc.v[3])), y);
+      f2 b2[4], c2[4], y[KD / 2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b2[i] = pack2(to_f(row[q].b.v[i]), to_f(row[q].b.v[i]));
+        c2[i] = pack2(to_f(row[q].c.v[i]), to_f(row[q].c.v[i]));
+      }
+      scan_step<true, KD>(h[q], A2, d, b2, c2, y);
       float o = sum_over_states<LN>(y, lane);
       if (mine) {
         o = fmaf(skip, u, o);
-        if (zg != nullptr) o *= to_f(row[q].z) * sigmoid_exact(to_f(row[q].z));
+        if (zg != nullptr) o *= to_f(row[q].z) * sigmoid_t<T>(to_f(row[q].z));
         og[(long long)t * p.D + c] = from_f<T>(o);
       }
     }

@@ -9,23 +9,26 @@ namespace ssm {
 
 template <typename T>
 cudaError_t scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st) {
-  const int bpg = (int)cdiv(p.spg, kScanWarps);
+  // the main kernel's slices: half as many channels as the carry kernel's
+  ScanParams m = p;
+  m.spg = bwd_slices_per_group(p.D, p.N, p.F);
+  const int bpg = (int)cdiv(m.spg, kScanWarps);
   cudaError_t e = with_lanes(p.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
     const dim3 block(kScanWarps * 32);
     if (p.R > 1) {
       auto k = ssm_scan_bwd_carry_kernel<T, LN>;
-      const size_t smem = sizeof(float) * kScanWarps * FwdSmem<LN>::kWarp;
+      const size_t smem = (size_t)kScanWarps * FwdSmem<T, LN, kFwdChans>::kWarp;
       cudaError_t e = allow_smem(k, smem);
       if (e == cudaSuccess) e = launch(k, slices_grid(p, p.R), block, smem, st, p);
       if (e != cudaSuccess) return e;
     }
     auto k = ssm_scan_bwd_kernel<T, LN>;
-    const size_t smem = sizeof(float) * BwdSmem<LN>::kTotal;
-    static_assert(sizeof(float) * BwdSmem<LN>::kTotal <= 227 * 1024, "shared memory of a CTA");
+    const size_t smem = BwdSmem<T, LN>::kTotal;
+    static_assert(BwdSmem<T, LN>::kTotal <= 227 * 1024, "shared memory of a CTA");
     cudaError_t e = allow_smem(k, smem);
     if (e != cudaSuccess) return e;
-    return launch(k, dim3((unsigned)(p.F * bpg), (unsigned)p.R), block, smem, st, p);
+    return launch(k, dim3((unsigned)(p.F * bpg), (unsigned)p.R), block, smem, st, m);
   });
   if (e != cudaSuccess) return e;
   e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), (unsigned)p.F),

@@ -10,12 +10,12 @@ constexpr int64_t kMaxStates = 128;
 constexpr int kMaxRanges = 64;
 constexpr int kMinRange = 32;  // tokens
 
-int64_t slices(int64_t D, int64_t N, int64_t F) { return F * cdiv(D / F, 128 / lanes_of(N)); }
+int64_t slices(int64_t D, int64_t N, int64_t F) { return F * fwd_slices_per_group(D, N, F); }
 
 // Ranges the stream is cut into: enough that each SM has kWarpsPerSm warps,
 // none shorter than kMinRange tokens. Returns the tokens per range (a multiple
 // of kTile) and sets R.
-constexpr int kWarpsPerSm = 8;
+constexpr int kWarpsPerSm = 16;
 int64_t plan_ranges(int64_t T, int64_t D, int64_t N, int64_t F, int asked, int& R) {
   int64_t r = asked > 0 ? asked : cdiv((int64_t)sm_count() * kWarpsPerSm, slices(D, N, F));
   if (r > kMaxRanges) r = kMaxRanges;
@@ -57,10 +57,11 @@ int check(int dtype, const ScanParams& p, const void* cu, int64_t num_seqs, int6
   return GRETA_OK;
 }
 
-// Vector paths: a lane's loads of V channels (4 or 8) and of 4 states start on
-// whole aligned vectors in every row and group.
-void plan_vectors(ScanParams& p, int es, std::initializer_list<const void*> rows) {
-  const int CHW = 128 / lanes_of(p.N), V = CHW < 8 ? CHW : 8;
+// Vector paths: a lane's loads of V channels and of 4 states start on whole
+// aligned vectors in every row and group.
+void plan_vectors(ScanParams& p, int es, int chans, std::initializer_list<const void*> rows) {
+  const int CHW = 32 / lanes_of(p.N) * chans;
+  const int V = CHW < 4 ? CHW : kTile * CHW >= 256 ? 8 : 4;  // TileVecs::V
   const int64_t a = (int64_t)V * es < 16 ? (int64_t)V * es : 16;
   bool ok = p.Dg % V == 0 && p.D % V == 0 && p.ldu % V == 0 && p.ldd % V == 0 &&
             (p.gate == nullptr || p.ldg % V == 0);
@@ -82,7 +83,7 @@ ScanParams base(const void* u, int64_t ldu, const void* delta, int64_t ldd, cons
   p.D = (int)D; p.N = (int)N; p.F = (int)F;
   if (D > 0 && F > 0 && N > 0) {
     p.Dg = (int)(D / F);
-    p.spg = (int)cdiv(p.Dg, 128 / lanes_of(N));
+    p.spg = fwd_slices_per_group(D, N, F);
   }
   p.softplus = softplus != 0;
   return p;
@@ -123,7 +124,7 @@ int run_decode(int dtype, const ScanParams& p, int rq, void* stream) {
 struct BwdWorkspace {
   int64_t bc, a, d, total;
   BwdWorkspace(int64_t R, int64_t T, int64_t D, int64_t N, int64_t F) {
-    const int64_t blocks = F * cdiv(slices(D, N, F) / F, kScanWarps);
+    const int64_t blocks = F * cdiv(bwd_slices_per_group(D, N, F), kScanWarps);
     bc = a16(Workspace(R, D, N).total);
     a = bc + a16(blocks * T * 2 * N * 4);
     d = a + a16(R * D * N * 4);
@@ -175,7 +176,7 @@ int greta_ssm_scan_fwd(int dtype, const void* u, int64_t ldu, const void* delta,
   if (!aligned(saved, 16)) return GRETA_ERR_ALIGNMENT;
   p.ckpt = saved;
   p.zero_rest = 1;
-  plan_vectors(p, esize(dtype), {u, delta, gate, out});
+  plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, out});
   p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
   c = set_workspace(p, workspace, workspace_bytes);
   if (c != GRETA_OK) return c;
@@ -205,7 +206,7 @@ int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* del
   p.slots = slots;
   p.initial = reinterpret_cast<const signed char*>(has_initial);
   p.err = error_flags;
-  plan_vectors(p, esize(dtype), {u, delta, gate, out});
+  plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, out});
   if (ranges == 0 && num_reqs > 0 && T <= num_reqs + kDecodeExtra) {
     // one request a warp while that is what it takes to give every SM work
     const int64_t warps = slices(D, N, F) * num_reqs;
@@ -252,7 +253,7 @@ int greta_ssm_scan_bwd(int dtype, const void* u, int64_t ldu, const void* delta,
   p.ckpt = const_cast<float*>(saved);
   p.dout = dout;
   p.du = du; p.ddelta = ddelta; p.dgate = dgate;
-  plan_vectors(p, esize(dtype), {u, delta, gate, dout, du, ddelta, dgate});
+  plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, dout, du, ddelta, dgate});
   p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
   const BwdWorkspace w(p.R, T, D, N, F);
   if (workspace == nullptr || workspace_bytes < w.total) return GRETA_ERR_INVALID_ARG;

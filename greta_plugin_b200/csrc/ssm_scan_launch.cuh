@@ -11,6 +11,15 @@ namespace ssm {
 // Lanes per channel: N / 4 rounded up to 4, 8, 16 or 32.
 inline int lanes_of(int64_t N) { return N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
 
+// Channel slices (one warp each) per group of the forward and carry kernels and
+// of the backward kernel.
+inline int fwd_slices_per_group(int64_t D, int64_t N, int64_t F) {
+  return (int)cdiv(D / F, 32 / lanes_of(N) * 4);
+}
+inline int bwd_slices_per_group(int64_t D, int64_t N, int64_t F) {
+  return (int)cdiv(D / F, 32 / lanes_of(N) * 2);
+}
+
 template <typename F>
 auto with_lanes(int N, F f) {
   switch (lanes_of(N)) {
@@ -30,7 +39,7 @@ template <typename T>
 cudaError_t scan_fwd(const ScanParams& p, cudaStream_t st) {
   return with_lanes(p.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    const size_t smem = sizeof(float) * kScanWarps * FwdSmem<LN>::kWarp;
+    const size_t smem = (size_t)kScanWarps * FwdSmem<T, LN, kFwdChans>::kWarp;
     const dim3 grid = slices_grid(p, p.R), block(kScanWarps * 32);
     if (p.R > 1) {
       auto k = ssm_scan_fwd_kernel<T, LN, kPhaseCarry>;

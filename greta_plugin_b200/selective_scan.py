@@ -32,7 +32,7 @@ from .causal_conv import channel_rows, check_disjoint, packed_metadata, packed_o
 from .dynamic_conv import _cu
 
 MAX_STATES = 128
-SAVE_EVERY = 16  # tokens per saved state
+SAVE_EVERY = 8  # tokens per saved state
 
 
 def _check(u, delta, A, B, C, skip, gate, delta_bias):
@@ -173,21 +173,23 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     each; skip, delta_bias: [D] or None; cu_seqlens: [N + 1] offsets (None: one
     sequence). Returns [1, T, D] contiguous. Every sequence starts from a zero
     state; rows that no sequence holds give zeros and zero gradients. When a
-    gradient is needed, the forward keeps the states ahead of every 16th token
-    (fp32 [T / 16 + 1, D, N]) for the backward.
+    gradient is needed, the forward keeps the states ahead of every 8th token
+    (fp32 [T / 8 + 1, D, N]) for the backward.
     """
     if u.dim() != 3 or u.shape[0] != 1:
         raise ValueError(f"u must be [1, T, D], got {tuple(u.shape)}")
     for name, t in (("delta", delta), ("gate", gate)):
         if t is not None and tuple(t.shape) != tuple(u.shape):
             raise ValueError(f"{name} shape {tuple(t.shape)} must match u's {tuple(u.shape)}")
-    _check(u[0], delta[0], A, B, C, skip, None if gate is None else gate[0], delta_bias)
+    # squeeze, not u[0], whose gradient would be copied into zeros
+    u, delta, gate = u.squeeze(0), delta.squeeze(0), None if gate is None else gate.squeeze(0)
+    _check(u, delta, A, B, C, skip, gate, delta_bias)
     if not u.is_cuda:
         raise ValueError("selective_scan requires CUDA tensors")
     if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
         raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
-    return SelectiveScanFunction.apply(u[0], delta[0], A, B, C, skip, None if gate is None else gate[0], delta_bias,
-                                       cu_seqlens, delta_softplus)[None]
+    return SelectiveScanFunction.apply(u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens,
+                                       delta_softplus).unsqueeze(0)
 
 
 def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has_initial, delta_softplus, out, flags):

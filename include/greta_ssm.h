@@ -80,8 +80,8 @@ GRETA_API int greta_ssm_conv_packed(int dtype, const void* x, int64_t ldx, const
  *   A              : fp32 [D, N] contiguous; skip, delta_bias: fp32 [D] or NULL
  *   out            : [T, D] contiguous
  *   F divides D; 1 <= N <= 128. States are fp32.
- *   saved          : NULL, or fp32 [T / 16 + 1, D, N]: the states ahead of every
- *                    16th token of the stream, for the backward
+ *   saved          : NULL, or fp32 [T / 8 + 1, D, N]: the states ahead of every
+ *                    8th token of the stream, for the backward
  *   ranges         : 0, or the number of token ranges to cut the stream into
  *                    (tests and tuning; results differ by rounding only)
  */
