@@ -75,22 +75,10 @@ __device__ __forceinline__ Seg seg_next(const Seqs& q, const Seg& g) {
   return n;
 }
 
-// Where range i of R ranges of about L tokens begins: i * L, or the nearest
-// sequence start within half a range of it. A range that begins with a
-// sequence needs nothing from the range before; the moved borders stay in
-// order, since each moves by less than half a range.
-__device__ __forceinline__ int range_begin(const Seqs& q, int i, int R, int L, int lane) {
-  if (i <= 0) return 0;
-  if (i >= R) return q.T;
-  const int p = (int)min((long long)i * L, (long long)q.T);
-  const int s = warp_find(q, p, lane);
-  const int before = s >= 0 ? seq_start(q, s) : 0;
-  const int after = s < q.nseq ? seq_start(q, s + 1) : q.T;
-  const bool nb = before <= p && p - before <= L / 2 && before > 0;
-  const bool na = after > p && after - p < L / 2;
-  if (nb && (!na || p - before <= after - p)) return before;
-  if (na) return after;
-  return p;
+// Where range i of L tokens begins. (Borders moved to sequence starts close by
+// save some carries, but ranges of uneven length cost more than that.)
+__device__ __forceinline__ int range_begin(const Seqs& q, int i, int L) {
+  return (int)min((long long)i * L, (long long)q.T);
 }
 
 // NV consecutive elements of a row as fp32. vec: the row starts on a whole
@@ -170,6 +158,20 @@ __device__ __forceinline__ void copy_part(T* dst, const T* src, const T* base, i
   }
 }
 
+// Four consecutive elements (aligned) in fp32. For bf16 two shifts and two
+// masks, written out.
+template <typename T>
+__device__ __forceinline__ float4 widen4(const T* s) {
+  const Pack<T, 4> v = load_part<T, 4>(s, 4, true);
+  return make_float4(to_f(v.v[0]), to_f(v.v[1]), to_f(v.v[2]), to_f(v.v[3]));
+}
+template <>
+__device__ __forceinline__ float4 widen4(const __nv_bfloat16* s) {
+  const uint2 w = *reinterpret_cast<const uint2*>(s);
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                     __uint_as_float(w.y & 0xffff0000u));
+}
+
 // ---------------------------------------------------------------------------
 // fp32 pairs in 64-bit registers (one instruction for two lanes; each lane is
 // rounded like the scalar operation)
@@ -233,14 +235,15 @@ __device__ __forceinline__ float max0(float x) {
 // small (steps of 1e-3 and less): max(x, 0) + log1p(e) for e = e^-|x| in
 // (0, 1], and log1p(e) = e P(e) with the polynomial of degree 9 that fits
 // log1p(e) / e on [0, 1] best (5e-9; 1.2e-7 with the fp32 roundings). e as in
-// exp_neg; beyond 87 it is nothing next to the sum.
-__device__ __forceinline__ f2 softplus2(float x0, float x1) {
-  const f2 x = pack2(fminf(fabsf(x0), 87.f), fminf(fabsf(x1), 87.f));
+// exp_neg (0 from 120 on at the latest, so that -inf gives 0 and no NaN).
+// e: the two values of e.
+__device__ __forceinline__ f2 softplus2(float x0, float x1, f2& e) {
+  const f2 x = pack2(fminf(fabsf(x0), 120.f), fminf(fabsf(x1), 120.f));
   const f2 t = f2_mul(x, pack2(-kLog2e, -kLog2e));  // rounded -|x| log2(e)
   // what it lost: -(|x| log2(e) + t) - |x| (log2(e) - kLog2e)
   f2 lost = f2_fma(x, pack2(-kLog2e, -kLog2e), f2_mul(t, pack2(-1.f, -1.f)));
   lost = f2_fma(x, pack2(-1.925963033e-8f, -1.925963033e-8f), lost);
-  f2 e = f2_ex2(t);
+  e = f2_ex2(t);
   e = f2_fma(e, f2_mul(lost, pack2(kLn2, kLn2)), e);
   constexpr float c[9] = {-0.4999990165233612f, 0.3332996070384979f,  -0.2495412975549698f,
                           0.1967591792345047f,  -0.1530553102493286f, 0.106035515666008f,
@@ -250,6 +253,13 @@ __device__ __forceinline__ f2 softplus2(float x0, float x1) {
   for (int i = 7; i >= 0; --i) q = f2_fma(q, e, pack2(c[i], c[i]));
   q = f2_fma(q, e, pack2(1.f, 1.f));
   return f2_fma(q, e, pack2(max0(x0), max0(x1)));
+}
+
+// Its derivative, 1 / (1 + e^-x), from that e.
+__device__ __forceinline__ float softplus_slope(float x, float e) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return x >= 0.f ? r : e * r;
 }
 
 // 1 / (1 + e^-x), to a few ulp at both ends; sigmoid_fast to about 1e-6, for

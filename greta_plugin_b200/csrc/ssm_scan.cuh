@@ -37,7 +37,14 @@
 
 #include "ssm_common.cuh"
 
+#ifndef FB
+#define FB 4
+#endif
+#ifndef FU
+#define FU 8
+#endif
 namespace greta {
+constexpr int kFU = FU;
 
 constexpr int kTile = 8;         // tokens per tile, and per saved state
 constexpr int kLaneStates = 4;   // states per lane
@@ -257,13 +264,16 @@ __device__ __forceinline__ void copy_bc(const ScanParams& p, const Lanes<LN, KD>
 // Four states of B or C in fp32, each twice (for two channels).
 template <typename T>
 __device__ __forceinline__ void read_four(const T* s, f2 (&o)[4]) {
-  const Pack<T, 4> v = load_part<T, 4>(s, 4, true);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = pack2(to_f(v.v[i]), to_f(v.v[i]));
+  const float4 v = widen4(s);
+  o[0] = pack2(v.x, v.x);
+  o[1] = pack2(v.y, v.y);
+  o[2] = pack2(v.z, v.z);
+  o[3] = pack2(v.w, v.w);
 }
 
 __device__ __forceinline__ f2 step_sizes(const ScanParams& p, float x0, float x1) {
-  return p.softplus ? softplus2(x0, x1) : pack2(x0, x1);
+  f2 e;
+  return p.softplus ? softplus2(x0, x1, e) : pack2(x0, x1);
 }
 
 // One token of the recurrence for the lane's states, dl = (dt, dt u) of its
@@ -444,7 +454,7 @@ struct FwdSmem {
 enum ScanPhase { kPhaseCarry = 0, kPhaseMain = 1 };
 
 template <typename T, int LN, int PHASE>
-__global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, FB) ssm_scan_fwd_kernel(const ScanParams p) {
   extern __shared__ float4 smem4[];
   constexpr int KD = kFwdChans;
   using L = Lanes<LN, KD>;
@@ -466,8 +476,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
   if (slice >= p.F * p.spg) return;
   const L l(p, slice, lane);
   const int ri = blockIdx.y;
-  int t0 = range_begin(p.q, ri, p.R, p.L, lane);
-  const int t1 = range_begin(p.q, ri + 1, p.R, p.L, lane);
+  int t0 = range_begin(p.q, ri, p.L);
+  const int t1 = range_begin(p.q, ri + 1, p.L);
   if (t0 >= t1) return;
 
   LaneStates<KD> A2, h;
@@ -533,8 +543,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
     }
   };
 
-  fetch(t0 / kTile * kTile, 0);
-  for (int tile0 = t0 / kTile * kTile; tile0 < t1; tile0 += kTile, cur ^= 1) {
+  // (the carry of a range begins where its last sequence does)
+  const int tile_first = t0 / kTile * kTile;
+  fetch(tile_first, 0);
+  for (int tile0 = tile_first; tile0 < t1; tile0 += kTile, cur ^= 1) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
     copy_wait();
     bc = stage(cur, 3);
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
     __syncwarp();
     // (the other stage's B and C were last read ahead of the barrier before)
     if (tile0 + kTile < t1) fetch(tile0 + kTile, cur ^ 1);
-    if (kMain && p.ckpt != nullptr && ta == tile0) store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
+    if (kMain && p.ckpt != nullptr) store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
     unsigned live = 0;  // tokens of the tile that a sequence holds
     int t = ta;
     while (t < tb) {
@@ -561,7 +573,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
           }
         }
         if (stop - t == kTile) {
-#pragma unroll
+#pragma unroll kFU
           for (int r = 0; r < kTile; ++r) step(r);
         } else {
           for (int r = t - tile0; r < stop - tile0; ++r) step(r);

@@ -12,13 +12,16 @@
 // its range's tiles of 8 tokens from the last to the first: it runs a tile's
 // recurrence again from the saved state with the tile's states in registers,
 // and goes back through them with g. So two exponentials and some thirteen fp32
-// operations per (token, channel, state): 16 and 14 clocks a warp, both pipes
-// about equally full, and as many issue slots again for the sums over states
-// and channels. A lane has two channels of four states: 8 x 8 states, and
-// their rates, adjoints and sums, are what its registers hold (with four
-// channels the saved states would be ahead of every 4th token). The
-// CTA's warps take neighbouring channels of one group; their parts of dB
-// and dC are added in shared memory and go, one row per token and CTA, to
+// operations per (token, channel, state), 16 and 13 clocks a warp. A lane has
+// two channels of four states: 8 x 8 states, and their rates, adjoints and
+// sums, are what its registers hold (with four channels the saved states would
+// be ahead of every 4th token). What bounds it is the issue of instructions and
+// the shared memory beside them, so: two states of a channel share an
+// instruction here (doubling dt, dt u and dy takes fewer moves than doubling B
+// and C, and the sums over channels need no adding of halves), and the lanes'
+// parts of dB and dC are not exchanged but stored, two vectors a token, and
+// added for all of the CTA's channels at once. The CTA's warps take
+// neighbouring channels of one group; its dB and dC go, one row per token, to
 // `part_bc`; dA, dskip and d(delta_bias) of the range stay with the lane,
 // added tile by tile to keep long sums short. Small kernels add the parts in a
 // fixed order, so the same call gives the same bits.
@@ -130,8 +133,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   const L l(p, slice, lane);
   const int ri = blockIdx.y;
   if (ri == 0) return;
-  const int t0 = range_begin(p.q, ri, p.R, p.L, lane);
-  int t1 = range_begin(p.q, ri + 1, p.R, p.L, lane);
+  const int t0 = range_begin(p.q, ri, p.L);
+  int t1 = range_begin(p.q, ri + 1, p.L);
   if (t0 >= t1) return;
   const Seg g = seg_at(p.q, t0, lane);
   if (!g.in || g.b >= t0) return;
@@ -193,45 +196,45 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   if (l.nq == 0) store_sums(p, l, ri, dsum);
 }
 
-// The eight values of a lane summed over the channel groups of the warp (lane
-// bits LN, 2 LN, .. 16): halves are exchanged while there are some, so that
-// M = LN / 4 values, from index `base`, stay with a lane.
-template <int LN>
-__device__ __forceinline__ void sum_over_channels(float (&v)[8], int lane, int& base) {
-  base = 0;
-  int m = 8;
-#pragma unroll
-  for (int o = LN; o < 32; o <<= 1) {
-    const bool hi = lane & o;
-    m >>= 1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i < m) {
-        const float send = hi ? v[i] : v[m + i], keep = hi ? v[m + i] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-      }
-    }
-    if (hi) base += m;
-  }
-}
-
 // Shared memory of the backward, in bytes: of a warp, and what the CTA shares.
 template <typename T, int LN>
 struct BwdSmem {
-  static constexpr int CHW = Lanes<LN, kBwdChans>::CHW, NP = Lanes<LN, kBwdChans>::NP;
-  static constexpr int kDl = kTile * CHW * 8;    // (dt, dt u)
-  static constexpr int kDy = kTile * CHW * 4;
-  static constexpr int kY = kTile * CHW * 4;
-  static constexpr int kPair = kTile * CHW * 8;  // (sum kept A2, sum g B)
-  static constexpr int kSum = 32 * TileVecs<CHW>::V * 8;     // dskip, d(delta_bias) of the lanes
-  static constexpr int kPart = kTile * 2 * NP * 4;           // dB, dC of the warp's channels
+  static constexpr int CHW = Lanes<LN, kBwdChans>::CHW, NP = Lanes<LN, kBwdChans>::NP, V = TileVecs<CHW>::V;
   static constexpr int kRow = kTile * CHW * (int)sizeof(T);  // a tile of an operand
-  static constexpr int kH = 32 * kBwdChans * 16;             // saved states
-  static constexpr int kStage = 4 * kRow + kH;               // u, delta, gate, dout; states
-  static constexpr int kWarp = kDl + kDy + kY + kPair + kSum + kPart + 2 * kStage;
+  static constexpr int kRowF = kTile * CHW * 4;
+  static constexpr int kDl = 0;                       // (dt, dt u)
+  static constexpr int kDy = kDl + 2 * kRowF;         // dy
+  static constexpr int kSlope = kDy + kRowF;          // d(dt) / d(raw step)
+  static constexpr int kGk = kSlope + kRowF;          // dout SiLU'(gate)
+  static constexpr int kY = kGk + kRowF;              // sum C h
+  static constexpr int kPair = kY + kRowF;            // (sum kept A2, sum g B)
+  static constexpr int kCols = kPair + 2 * kRowF;     // [bias | skip][lane] V floats
+  static constexpr int kSum = kCols + 2 * 32 * V * 4;  // [dskip | d(delta_bias)][lane] V floats
+  static constexpr int kPart = kSum + 2 * 32 * V * 4;  // [token][dB | dC][lane] float4
+  static constexpr int kStage0 = kPart + kTile * 2 * 32 * 16;
+  static constexpr int kStage = 4 * kRow + 32 * kBwdChans * 16;  // u, delta, gate, dout; saved states
+  static constexpr int kWarp = kStage0 + 2 * kStage;
   static constexpr int kBC = kTile * 2 * NP * (int)sizeof(T);
   static constexpr int kTotal = kScanWarps * kWarp + 2 * kBC;
 };
+
+// Four states of B or C in fp32, as pairs of states.
+template <typename T>
+__device__ __forceinline__ void read_pairs(const T* s, f2 (&o)[2]) {
+  const float4 v = widen4(s);
+  o[0] = pack2(v.x, v.y);
+  o[1] = pack2(v.z, v.w);
+}
+
+// Pairs of channels to pairs of states.
+__device__ __forceinline__ void by_states(const f2 (&h)[4], f2 (&o)[2][2]) {
+  float4 a, b;
+  unpack_pair(h, a, b);
+  o[0][0] = pack2(a.x, a.y);
+  o[0][1] = pack2(a.z, a.w);
+  o[1][0] = pack2(b.x, b.y);
+  o[1][1] = pack2(b.z, b.w);
+}
 
 template <typename T, int LN>
 __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const ScanParams p) {
@@ -245,18 +248,20 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   char* base = reinterpret_cast<char*>(smem4);
   char* mine = base + 2 * S::kBC + warp * S::kWarp;
-  float4* dl = reinterpret_cast<float4*>(mine);
-  float* dys = reinterpret_cast<float*>(mine + S::kDl);
-  float* ys = reinterpret_cast<float*>(mine + S::kDl + S::kDy);
-  float2* pair = reinterpret_cast<float2*>(mine + S::kDl + S::kDy + S::kY);
-  float2* sums = reinterpret_cast<float2*>(mine + S::kDl + S::kDy + S::kY + S::kPair) + lane;  // [V][32]
-  constexpr int kPartAt = S::kDl + S::kDy + S::kY + S::kPair + S::kSum;
-  float* part = reinterpret_cast<float*>(mine + kPartAt);
-  auto stage = [&](int s, int op) {  // u, delta, gate, dout, (states)
-    return reinterpret_cast<T*>(mine + kPartAt + S::kPart + s * S::kStage + op * S::kRow);
+  float4* dl = reinterpret_cast<float4*>(mine + S::kDl);
+  float* dys = reinterpret_cast<float*>(mine + S::kDy);
+  float* slope = reinterpret_cast<float*>(mine + S::kSlope);
+  float* gk = reinterpret_cast<float*>(mine + S::kGk);
+  float* ys = reinterpret_cast<float*>(mine + S::kY);
+  float2* pair = reinterpret_cast<float2*>(mine + S::kPair);
+  float* cols = reinterpret_cast<float*>(mine + S::kCols) + lane * V;
+  float* sums = reinterpret_cast<float*>(mine + S::kSum) + lane * V;
+  float4* part = reinterpret_cast<float4*>(mine + S::kPart) + lane;
+  auto stage = [&](int s, int op) {  // u, delta, gate, dout
+    return reinterpret_cast<T*>(mine + S::kStage0 + s * S::kStage + op * S::kRow);
   };
   auto saved = [&](int s) {  // [channel][lane]
-    return reinterpret_cast<float4*>(mine + kPartAt + S::kPart + s * S::kStage + 4 * S::kRow) + lane;
+    return reinterpret_cast<float4*>(mine + S::kStage0 + s * S::kStage + 4 * S::kRow) + lane;
   };
   pdl_wait();
   pdl_trigger();
@@ -266,23 +271,36 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   L l(p, f * p.spg + (have ? in_group : 0), lane);
   if (!have) l.nch = 0;
   const int ri = blockIdx.y;
-  const int t0 = range_begin(p.q, ri, p.R, p.L, lane);
-  const int t1 = range_begin(p.q, ri + 1, p.R, p.L, lane);
+  const int t0 = range_begin(p.q, ri, p.L);
+  const int t1 = range_begin(p.q, ri + 1, p.L);
   const long long DN = (long long)p.D * p.N;
-  LaneStates<KD> A2, dA, rr;
-  load_rates(p, l, A2);
-  zero_states<KD>(dA);
-  zero_states<KD>(rr);
-  float bias[V], skip[V];
-  load_column<V>(p.dbias, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), bias);
-  load_column<V>(p.skip, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), skip);
-#pragma unroll
-  for (int e = 0; e < V; ++e) sums[e * 32] = make_float2(0.f, 0.f);
-  Seg g{-1, 0, 0, false};
-  if (t0 < t1 && t1 < p.q.T) {
-    g = seg_at(p.q, t1, lane);
-    if (g.in && g.b < t1) carry_back(p, l, ri, A2, rr);
+  f2 A2[KD][2], dA[KD][2], rr[KD][2];
+  {
+    LaneStates<KD> a, r;
+    load_rates(p, l, a);
+    zero_states<KD>(r);
+    if (t0 < t1 && t1 < p.q.T) {
+      const Seg g = seg_at(p.q, t1, lane);
+      if (g.in && g.b < t1) carry_back(p, l, ri, a, r);
+    }
+    by_states(a[0], A2);
+    by_states(r[0], rr);
   }
+#pragma unroll
+  for (int j = 0; j < KD; ++j) dA[j][0] = dA[j][1] = 0ull;
+  {
+    float v[V];
+    load_column<V>(p.dbias, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) cols[e] = v[e];
+    load_column<V>(p.skip, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      cols[32 * V + e] = v[e];
+      sums[e] = sums[32 * V + e] = 0.f;
+    }
+  }
+  Seg g{-1, 0, 0, false};
 
   auto fetch = [&](int tile0, int s) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
@@ -291,13 +309,12 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     if (p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
     copy_tile<T>(p.dout, p.D, p.vec, l, tile0, ta, tb, stage(s, 3));
     copy_bc<T>(p, l, tile0, ta, tb, reinterpret_cast<T*>(base + s * S::kBC), threadIdx.x, kScanWarps * 32);
-    // a range that begins inside a tile begins there with a sequence, or outside
     const float* c = p.ckpt + (tile0 / kTile) * DN;
 #pragma unroll
     for (int j = 0; j < KD; ++j)
       copy_part<float, 4>(reinterpret_cast<float*>(saved(s) + j * 32),
                           c + (long long)(l.c0 + l.ch(j)) * p.N + l.n0(), p.ckpt,
-                          ta == tile0 && l.ch(j) < l.nch ? p.N - l.n0() : 0, p.N % 4 == 0);
+                          l.ch(j) < l.nch ? p.N - l.n0() : 0, p.N % 4 == 0);
     copy_commit();
   };
   const int last = t1 > t0 ? (t1 - 1) / kTile * kTile : -kTile;
@@ -308,10 +325,59 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     const TileSeqs q = tile_seqs(p.q, tile0, ta, tb, lane, g);
     copy_wait();
     const T* bc = reinterpret_cast<T*>(base + cur * S::kBC);
-    f2 hs[kTile + 1][4];
-    pack_pair(saved(cur)[0], saved(cur)[32], hs[0]);
-    stage_steps<T>(p, l, q.live, stage(cur, 0), stage(cur, 1), bias, dl);
-    stage_dy<T>(p, l, stage(cur, 3), stage(cur, 2), q.live, dys);
+    f2 hs[kTile + 1][KD][2];
+#pragma unroll
+    for (int j = 0; j < KD; ++j) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(saved(cur) + j * 32);
+      hs[0][j][0] = v.x;
+      hs[0][j][1] = v.y;
+    }
+    // per token and channel: (dt, dt u), the step's slope, dy and dout SiLU'
+#pragma unroll
+    for (int k = 0; k < TV::NVEC; ++k) {
+      if (!TV::has(k, lane)) continue;
+      const int r = TV::row(k, lane), c = TV::chan(lane), at = r * CHW + c;
+      const bool in = (q.live >> r) & 1;
+      const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane), d = tile_vec<T, CHW>(stage(cur, 1), k, lane),
+                       go = tile_vec<T, CHW>(stage(cur, 3), k, lane);
+      const Pack<float, V> bias = load_part<float, V>(cols, V, true);
+      Pack<float, V> sl, dy, gs;
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float x0 = to_f(d.v[e]) + bias.v[e], x1 = to_f(d.v[e + 1]) + bias.v[e + 1];
+        f2 s = pack2(x0, x1), ex;
+        sl.v[e] = sl.v[e + 1] = 1.f;
+        if (p.softplus) {
+          s = softplus2(x0, x1, ex);
+          float e0, e1;
+          unpack2(ex, e0, e1);
+          sl.v[e] = softplus_slope(x0, e0);
+          sl.v[e + 1] = softplus_slope(x1, e1);
+        }
+        const f2 su = f2_mul(s, pack2(to_f(u.v[e]), to_f(u.v[e + 1])));
+        float4 o;
+        unpack2(s, o.x, o.y);
+        unpack2(su, o.z, o.w);
+        const bool c0 = in && c + e < l.nch, c1 = in && c + e + 1 < l.nch;
+        dl[(at + e) / 2] = make_float4(c0 ? o.x : 0.f, c1 ? o.y : 0.f, c0 ? o.z : 0.f, c1 ? o.w : 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) dy.v[e] = to_f(go.v[e]);
+      if (p.gate != nullptr) {
+        const Pack<T, V> z = tile_vec<T, CHW>(stage(cur, 2), k, lane);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float zv = to_f(z.v[e]), sg = sigmoid_t<T>(zv), gsg = dy.v[e] * sg;
+          gs.v[e] = gsg * fmaf(zv, 1.f - sg, 1.f);
+          dy.v[e] = gsg * zv;
+        }
+        store_part<float, V>(gk + at, gs, V, true);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) dy.v[e] = in ? dy.v[e] : 0.f;
+      store_part<float, V>(slope + at, sl, V, true);
+      store_part<float, V>(dys + at, dy, V, true);
+    }
     __syncthreads();
     if (tile0 > t0) fetch(tile0 - kTile, cur ^ 1);
 
@@ -321,69 +387,78 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     auto forward = [&](auto general) {
 #pragma unroll
       for (int r = 0; r < kTile; ++r) {
-        ulonglong2 dv[1];
-        f2 b[4], c[4], y[1];
-        read_steps<KD>(dl, r * CHW + l.ch(0), dv);
-        read_four(bc + r * 2 * NP + l.n0(), b);
-        if (p.gate != nullptr) read_four(bc + (r * 2 + 1) * NP + l.n0(), c);
-        LaneStates<KD> h;
+        const float4 dv = dl[(r * CHW + l.ch(0)) / 2];
+        const float dt[KD] = {dv.x, dv.y}, du[KD] = {dv.z, dv.w};
+        f2 b[2], c[2];
+        float y[KD];
+        read_pairs(bc + r * 2 * NP + l.n0(), b);
+        if (p.gate != nullptr) read_pairs(bc + (r * 2 + 1) * NP + l.n0(), c);
         const bool first = decltype(general)::value && ((q.first >> r) & 1);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[0][k] = first ? 0ull : hs[r][k];
-        if (p.gate != nullptr) {
-          scan_step<true, KD>(h, A2, dv, b, c, y);
-          const float s = sum_over_states<LN>(y, lane);
-          if (l.nq < KD) ys[r * CHW + l.ch(sum_channel<KD>(lane))] = s;
-        } else {
-          scan_step<false, KD>(h, A2, dv, b, c, y);
-        }
+        for (int j = 0; j < KD; ++j) {
+          const f2 d2 = pack2(dt[j], dt[j]), du2 = pack2(du[j], du[j]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hs[r + 1][k] = h[0][k];
+          for (int k = 0; k < 2; ++k)
+            hs[r + 1][j][k] = f2_fma(f2_ex2(f2_mul(d2, A2[j][k])), first ? 0ull : hs[r][j][k], f2_mul(du2, b[k]));
+          if (p.gate != nullptr) y[j] = f2_sum(f2_fma(c[1], hs[r + 1][j][1], f2_mul(c[0], hs[r + 1][j][0])));
+        }
+        if (p.gate != nullptr) {
+          const f2 yp[1] = {pack2(y[0], y[1])};
+          const float s = sum_over_states<LN>(yp, lane);
+          if (l.nq < KD) ys[r * CHW + l.ch(sum_channel<KD>(lane))] = s;
+        }
       }
     };
     // the exponentials are taken again: kept from the first pass they would need
     // 64 more registers
     auto again = [&] {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) asm volatile("" : "+l"(A2[0][k])::"memory");
+      for (int j = 0; j < KD; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) asm volatile("" : "+l"(A2[j][k])::"memory");
     };
     // back through them
-    f2 dAt[4] = {0ull, 0ull, 0ull, 0ull};
+    f2 dAt[KD][2];
+#pragma unroll
+    for (int j = 0; j < KD; ++j) dAt[j][0] = dAt[j][1] = 0ull;
     auto backward = [&](auto general) {
 #pragma unroll
       for (int r = kTile - 1; r >= 0; --r) {
         const bool first = decltype(general)::value && ((q.first >> r) & 1);
         const bool none = decltype(general)::value && !((q.live >> r) & 1);
-        ulonglong2 dv[1];
-        f2 b[4], c[4], y[1], s2[1], g2[1];
-        read_steps<KD>(dl, r * CHW + l.ch(0), dv);
-        read_dy<KD>(dys + r * CHW + l.ch(0), y);
-        read_four(bc + r * 2 * NP + l.n0(), b);
-        read_four(bc + (r * 2 + 1) * NP + l.n0(), c);
-        float v[8];
+        const float4 dv = dl[(r * CHW + l.ch(0)) / 2];
+        const float2 dyv = *reinterpret_cast<const float2*>(dys + r * CHW + l.ch(0));
+        const float dt[KD] = {dv.x, dv.y}, du[KD] = {dv.z, dv.w}, dy[KD] = {dyv.x, dyv.y};
+        f2 b[2], c[2], dB[2], dC[2];
+        float sa[KD], gb[KD];
+        read_pairs(bc + r * 2 * NP + l.n0(), b);
+        read_pairs(bc + (r * 2 + 1) * NP + l.n0(), c);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const f2 a = f2_ex2(f2_mul(dv[0].x, A2[0][k]));
-          const f2 gg = f2_fma(c[k], y[0], rr[0][k]);
-          const f2 ag = first ? 0ull : f2_mul(a, gg);
-          // (what is ahead of a first token is another sequence's, maybe NaN)
-          const f2 kept = none ? 0ull : f2_mul(ag, first ? 0ull : hs[r][k]);
-          s2[0] = k == 0 ? f2_mul(kept, A2[0][k]) : f2_fma(kept, A2[0][k], s2[0]);
-          g2[0] = k == 0 ? f2_mul(gg, b[k]) : f2_fma(gg, b[k], g2[0]);
-          dAt[k] = f2_fma(kept, dv[0].x, dAt[k]);
-          v[k] = f2_sum(f2_mul(gg, dv[0].y));
-          v[4 + k] = f2_sum(f2_mul(y[0], hs[r + 1][k]));
-          rr[0][k] = none ? rr[0][k] : ag;
+        for (int j = 0; j < KD; ++j) {
+          const f2 d2 = pack2(dt[j], dt[j]), du2 = pack2(du[j], du[j]), y2 = pack2(dy[j], dy[j]);
+          f2 s2 = 0ull, g2 = 0ull;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const f2 a = f2_ex2(f2_mul(d2, A2[j][k]));
+            const f2 gg = f2_fma(c[k], y2, rr[j][k]);
+            const f2 ag = first ? 0ull : f2_mul(a, gg);
+            // (what is ahead of a first token is another sequence's, maybe NaN)
+            const f2 kept = none ? 0ull : f2_mul(ag, first ? 0ull : hs[r][j][k]);
+            s2 = k == 0 ? f2_mul(kept, A2[j][k]) : f2_fma(kept, A2[j][k], s2);
+            g2 = k == 0 ? f2_mul(gg, b[k]) : f2_fma(gg, b[k], g2);
+            dAt[j][k] = f2_fma(kept, d2, dAt[j][k]);
+            dB[k] = j == 0 ? f2_mul(gg, du2) : f2_fma(gg, du2, dB[k]);
+            dC[k] = j == 0 ? f2_mul(y2, hs[r + 1][j][k]) : f2_fma(y2, hs[r + 1][j][k], dC[k]);
+            rr[j][k] = none ? rr[j][k] : ag;
+          }
+          sa[j] = f2_sum(s2);
+          gb[j] = f2_sum(g2);
         }
-        const float2 s = make_float2(sum_over_states<LN>(s2, lane), sum_over_states<LN>(g2, lane));
+        const f2 sp[1] = {pack2(sa[0], sa[1])}, gp[1] = {pack2(gb[0], gb[1])};
+        const float2 s = make_float2(sum_over_states<LN>(sp, lane), sum_over_states<LN>(gp, lane));
         if (l.nq < KD) pair[r * CHW + l.ch(sum_channel<KD>(lane))] = s;
-        int vb;
-        sum_over_channels<LN>(v, lane, vb);
-#pragma unroll
-        for (int i = 0; i < LN / 4; ++i) {
-          const int k = vb + i;  // 0..3: dB, 4..7: dC of states n0 + k % 4
-          part[(r * 2 + k / 4) * NP + l.n0() + k % 4] = v[i];
-        }
+        reinterpret_cast<ulonglong2*>(part)[(r * 2) * 32] = make_ulonglong2(dB[0], dB[1]);
+        reinterpret_cast<ulonglong2*>(part)[(r * 2 + 1) * 32] = make_ulonglong2(dC[0], dC[1]);
       }
     };
     if (q.first == 0 && q.live == (1u << kTile) - 1) {
@@ -396,65 +471,93 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
       backward(std::true_type());
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) dA[0][k] = f2_add(dA[0][k], dAt[k]);
-    __syncwarp();
+    for (int j = 0; j < KD; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) dA[j][k] = f2_add(dA[j][k], dAt[j][k]);
+    __syncthreads();
     // the tile's gradients by token and channel
 #pragma unroll
     for (int k = 0; k < TV::NVEC; ++k) {
-      const int r = TV::row(k, lane), c = TV::chan(lane), t = tile0 + r, n = l.nch - c;
+      const int r = TV::row(k, lane), c = TV::chan(lane), t = tile0 + r, n = l.nch - c, at = r * CHW + c;
       if (!TV::has(k, lane) || t < ta || t >= tb || n <= 0) continue;
       const bool vec = p.vec && n >= V, in = (q.live >> r) & 1;
-      const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane), d = tile_vec<T, CHW>(stage(cur, 1), k, lane);
-      Pack<T, V> z, go, du, dd, dz;
-      if (p.gate != nullptr) {
-        z = tile_vec<T, CHW>(stage(cur, 2), k, lane);
-        go = tile_vec<T, CHW>(stage(cur, 3), k, lane);
-      }
+      const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane);
+      const Pack<float, V> sl = load_part<float, V>(slope + at, V, true), dy = load_part<float, V>(dys + at, V, true),
+                           skip = load_part<float, V>(cols + 32 * V, V, true);
+      const Pack<float, 2 * V> steps = load_part<float, 2 * V>(reinterpret_cast<const float*>(dl) + at * 2, 2 * V, true),
+                               sp = load_part<float, 2 * V>(reinterpret_cast<const float*>(pair + at), 2 * V, true);
+      Pack<float, V> s0 = load_part<float, V>(sums, V, true), s1 = load_part<float, V>(sums + 32 * V, V, true);
+      Pack<T, V> du, dd, dz;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int at = r * CHW + c + e;
-        const float uv = to_f(u.v[e]), dt = reinterpret_cast<const float*>(dl)[at / 2 * 4 + e % 2], dy = dys[at];
-        const float2 s = pair[at];
-        du.v[e] = from_f<T>(in ? fmaf(dt, s.y, skip[e] * dy) : 0.f);
-        float ddt = fmaf(kLn2, s.x, uv * s.y);
-        if (p.softplus) ddt *= sigmoid_exact(to_f(d.v[e]) + bias[e]);
+        const float uv = to_f(u.v[e]), dt = steps.v[e / 2 * 4 + e % 2], sa = sp.v[2 * e], gb = sp.v[2 * e + 1];
+        const float ddt = fmaf(kLn2, sa, uv * gb) * sl.v[e];
+        du.v[e] = from_f<T>(in ? fmaf(dt, gb, skip.v[e] * dy.v[e]) : 0.f);
         dd.v[e] = from_f<T>(in ? ddt : 0.f);
-        if (in) {
-          const float2 o = sums[e * 32];
-          sums[e * 32] = make_float2(fmaf(dy, uv, o.x), o.y + ddt);
-        }
-        if (p.gate != nullptr) {
-          const float zv = to_f(z.v[e]), sg = sigmoid_t<T>(zv);
-          const float y = fmaf(skip[e], uv, ys[at]);
-          dz.v[e] = from_f<T>(in ? to_f(go.v[e]) * y * sg * (1.f + zv * (1.f - sg)) : 0.f);
-        }
+        s0.v[e] = in ? fmaf(dy.v[e], uv, s0.v[e]) : s0.v[e];
+        s1.v[e] = in ? s1.v[e] + ddt : s1.v[e];
       }
+      store_part<float, V>(sums, s0, V, true);
+      store_part<float, V>(sums + 32 * V, s1, V, true);
       const long long o = (long long)t * p.D + l.c0 + c;
       store_part<T, V>(reinterpret_cast<T*>(p.du) + o, du, n, vec);
       store_part<T, V>(reinterpret_cast<T*>(p.ddelta) + o, dd, n, vec);
-      if (p.gate != nullptr) store_part<T, V>(reinterpret_cast<T*>(p.dgate) + o, dz, n, vec);
-    }
-    __syncthreads();
-    // dB and dC of the CTA's channels, the warps' parts in order (the next
-    // tile's parts are written behind its own barrier)
-    const int warps = min(kScanWarps, p.spg - blockIdx.x % bpg * kScanWarps);
-    float* out = p.part_bc + ((long long)blockIdx.x * p.q.T + tile0) * 2 * p.N;
-    for (int i = threadIdx.x; i < kTile * 2 * NP; i += blockDim.x) {
-      const int r = i / (2 * NP), k = i / NP % 2, n = i % NP;
-      if (r < ta - tile0 || r >= tb - tile0 || n >= p.N) continue;
-      float s = 0.f;
+      if (p.gate != nullptr) {
+        const Pack<float, V> y = load_part<float, V>(ys + at, V, true), gs = load_part<float, V>(gk + at, V, true);
 #pragma unroll
-      for (int w = 0; w < kScanWarps; ++w)
-        if (w < warps) s += reinterpret_cast<float*>(base + 2 * S::kBC + w * S::kWarp + kPartAt)[i];
-      out[(r * 2 + k) * p.N + n] = (q.live >> r) & 1 ? s : 0.f;
+        for (int e = 0; e < V; ++e)
+          dz.v[e] = from_f<T>(in ? gs.v[e] * fmaf(skip.v[e], to_f(u.v[e]), y.v[e]) : 0.f);
+        store_part<T, V>(reinterpret_cast<T*>(p.dgate) + o, dz, n, vec);
+      }
+    }
+    // dB and dC of the CTA's channels: four states of a token's dB or dC per
+    // item, `PER` threads for one, each adding every PER-th channel group of all
+    // warps (the next tile's parts are written behind its own barrier; a warp
+    // without channels has zeros)
+    constexpr int ITEMS = kTile * 2 * LN;
+    constexpr int PER = ITEMS >= kScanWarps * 32 ? 1 : kScanWarps * 32 / ITEMS;
+    constexpr int GROUPS = 32 / LN;
+    static_assert(PER <= 2 && GROUPS % PER == 0, "a thread pair per item at most");
+    float* out = p.part_bc + ((long long)blockIdx.x * p.q.T + tile0) * 2 * p.N;
+#pragma unroll
+    for (int i0 = 0; i0 < ITEMS * PER; i0 += kScanWarps * 32) {
+      const int i = i0 + threadIdx.x, nq = i % LN, sub = i / LN % PER, item = i / (LN * PER), r = item / 2, k = item % 2;
+      f2 s0 = 0ull, s1 = 0ull;
+#pragma unroll
+      for (int w = 0; w < kScanWarps; ++w) {
+        const ulonglong2* b = reinterpret_cast<const ulonglong2*>(base + 2 * S::kBC + w * S::kWarp + S::kPart);
+#pragma unroll
+        for (int dg = 0; dg < GROUPS; dg += PER) {
+          const ulonglong2 v = b[(r * 2 + k) * 32 + (dg + sub) * LN + nq];
+          s0 = f2_add(s0, v.x);
+          s1 = f2_add(s1, v.y);
+        }
+      }
+      if (PER == 2) {
+        s0 = f2_add(s0, __shfl_xor_sync(0xffffffffu, s0, LN));
+        s1 = f2_add(s1, __shfl_xor_sync(0xffffffffu, s1, LN));
+      }
+      float4 v;
+      unpack2(s0, v.x, v.y);
+      unpack2(s1, v.z, v.w);
+      if (!((q.live >> r) & 1)) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (sub == 0 && r >= ta - tile0 && r < tb - tile0)
+        store_four(out + (r * 2 + k) * p.N + nq * 4, 1, p.N - nq * 4, p.N % 4 == 0, v);
     }
   }
   if (!have) return;
-  store_states(p.part_a + ri * DN, l, p.N, dA);
+#pragma unroll
+  for (int j = 0; j < KD; ++j) {
+    float4 v;
+    unpack2(dA[j][0], v.x, v.y);
+    unpack2(dA[j][1], v.z, v.w);
+    store_four(p.part_a + ri * DN + (long long)(l.c0 + l.ch(j)) * p.N + l.n0(), 1, l.ch(j) < l.nch ? p.N - l.n0() : 0,
+               p.N % 4 == 0, v);
+  }
   // lanes of one vector column: the same lane % VPR
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    float2 s = sums[e * 32];
+    float2 s = make_float2(sums[e], sums[32 * V + e]);
 #pragma unroll
     for (int o = TV::VPR; o < 32; o <<= 1) {
       s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
