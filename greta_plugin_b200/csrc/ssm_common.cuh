@@ -233,25 +233,20 @@ __device__ __forceinline__ float max0(float x) {
 
 // log(1 + e^x) of two values, with a small relative error also where it is
 // small (steps of 1e-3 and less): max(x, 0) + log1p(e) for e = e^-|x| in
-// (0, 1], and log1p(e) = e P(e) with the polynomial of degree 9 that fits
-// log1p(e) / e on [0, 1] best (5e-9; 1.2e-7 with the fp32 roundings). e as in
-// exp_neg (0 from 120 on at the latest, so that -inf gives 0 and no NaN).
-// e: the two values of e.
+// (0, 1], and log1p(e) = e P(e) with the polynomial of degree 8 that fits
+// log1p(e) / e on [0, 1] best (3e-8; 1.9e-7 with the fp32 roundings). e is
+// ex2's of the rounded product: off by 2^-24 |x| beside ex2's own ulp, 4e-7 for
+// a step of 1e-3. (0 from |x| = 120 on at the latest, so that -inf gives 0 and
+// no NaN.) e: the two values of e.
 __device__ __forceinline__ f2 softplus2(float x0, float x1, f2& e) {
   const f2 x = pack2(fminf(fabsf(x0), 120.f), fminf(fabsf(x1), 120.f));
-  const f2 t = f2_mul(x, pack2(-kLog2e, -kLog2e));  // rounded -|x| log2(e)
-  // what it lost: -(|x| log2(e) + t) - |x| (log2(e) - kLog2e)
-  f2 lost = f2_fma(x, pack2(-kLog2e, -kLog2e), f2_mul(t, pack2(-1.f, -1.f)));
-  lost = f2_fma(x, pack2(-1.925963033e-8f, -1.925963033e-8f), lost);
-  e = f2_ex2(t);
-  e = f2_fma(e, f2_mul(lost, pack2(kLn2, kLn2)), e);
-  constexpr float c[9] = {-0.4999990165233612f, 0.3332996070384979f,  -0.2495412975549698f,
-                          0.1967591792345047f,  -0.1530553102493286f, 0.106035515666008f,
-                          -0.05695851147174835f, 0.019850919023156166f, -0.003243904560804367f};
+  e = f2_ex2(f2_mul(x, pack2(-kLog2e, -kLog2e)));
+  constexpr float c[9] = {0.9999999403953552f, -0.4999949336051941f, 0.3331909477710724f,
+                          -0.24842970073223114f, 0.19105957448482513f, -0.13663139939308167f,
+                          0.07822470366954803f, -0.029504472389817238f, 0.005232503172010183f};
   f2 q = pack2(c[8], c[8]);
 #pragma unroll
   for (int i = 7; i >= 0; --i) q = f2_fma(q, e, pack2(c[i], c[i]));
-  q = f2_fma(q, e, pack2(1.f, 1.f));
   return f2_fma(q, e, pack2(max0(x0), max0(x1)));
 }
 

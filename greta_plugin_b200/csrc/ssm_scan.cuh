@@ -37,14 +37,7 @@
 
 #include "ssm_common.cuh"
 
-#ifndef FB
-#define FB 4
-#endif
-#ifndef FU
-#define FU 8
-#endif
 namespace greta {
-constexpr int kFU = FU;
 
 constexpr int kTile = 8;         // tokens per tile, and per saved state
 constexpr int kLaneStates = 4;   // states per lane
@@ -389,22 +382,39 @@ __device__ __forceinline__ unsigned tile_rows(int tile0, int ta, int tb) {
   return ((1u << (tb - ta)) - 1) << (ta - tile0);
 }
 
-// (dt, dt u) of a tile into shared memory, [token][pair of channels] as (dt0,
-// dt1, dt0 u0, dt1 u1). Rows without their bit and channels that are not there
-// get zeros: a decay of 1 and no input.
+// The step sizes of a tile in shared memory: [token][pair of channels] (dt0, dt1,
+// dt0 u0, dt1 u1). Lanes write four channels each, two float4: the pairs of a
+// row's upper half are swapped two by two so that the eight lanes of a row
+// write to different banks.
+__device__ __forceinline__ int step_slot(int pair) { return pair ^ ((pair >> 3) & 1); }
+
+// How the steps of a tile are dealt to the lanes: four channels a time (CHW of
+// a narrow slice).
+template <int CHW>
+struct StepVecs {
+  static constexpr int V = CHW < 4 ? CHW : 4;
+  static constexpr int VPR = CHW / V;
+  static constexpr int COUNT = kTile * VPR;
+  static constexpr int NVEC = (COUNT + 31) / 32;
+  static __device__ __forceinline__ bool has(int k, int lane) { return COUNT % 32 == 0 || k * 32 + lane < COUNT; }
+  static __device__ __forceinline__ int row(int k, int lane) { return (k * 32 + lane) / VPR; }
+  static __device__ __forceinline__ int chan(int lane) { return lane % VPR * V; }
+};
+
+// All rows and channels of the tile: those that are not there were copied as
+// zeros, have no input and are not stored (a step that no recurrence takes).
+// The rows were copied by other lanes: a barrier lies ahead.
 template <typename T, int LN, int KD>
-__device__ __forceinline__ void stage_steps(const ScanParams& p, const Lanes<LN, KD>& l, unsigned rows, const T* u,
-                                            const T* d, const float (&bias)[TileVecs<Lanes<LN, KD>::CHW>::V],
-                                            float4* dl) {
+__device__ __forceinline__ void stage_steps(const ScanParams& p, const Lanes<LN, KD>& l, const T* u, const T* d,
+                                            const float (&bias)[StepVecs<Lanes<LN, KD>::CHW>::V], float4* dl) {
   constexpr int CHW = Lanes<LN, KD>::CHW;
-  using TV = TileVecs<CHW>;
-  constexpr int V = TV::V;
+  using SV = StepVecs<CHW>;
+  constexpr int V = SV::V;
 #pragma unroll
-  for (int k = 0; k < TV::NVEC; ++k) {
-    if (!TV::has(k, l.lane)) continue;
-    const int r = TV::row(k, l.lane), c = TV::chan(l.lane);
-    const bool in = (rows >> r) & 1;
-    const Pack<T, V> uv = tile_vec<T, CHW>(u, k, l.lane), dv = tile_vec<T, CHW>(d, k, l.lane);
+  for (int k = 0; k < SV::NVEC; ++k) {
+    if (!SV::has(k, l.lane)) continue;
+    const int at = SV::row(k, l.lane) * CHW + SV::chan(l.lane);
+    const Pack<T, V> uv = load_part<T, V>(u + at, V, true), dv = load_part<T, V>(d + at, V, true);
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
       const f2 s = step_sizes(p, to_f(dv.v[e]) + bias[e], to_f(dv.v[e + 1]) + bias[e + 1]);
@@ -412,17 +422,16 @@ __device__ __forceinline__ void stage_steps(const ScanParams& p, const Lanes<LN,
       float4 o;
       unpack2(s, o.x, o.y);
       unpack2(x, o.z, o.w);
-      const bool c0 = in && c + e < l.nch, c1 = in && c + e + 1 < l.nch;
-      dl[(r * CHW + c + e) / 2] = make_float4(c0 ? o.x : 0.f, c1 ? o.y : 0.f, c0 ? o.z : 0.f, c1 ? o.w : 0.f);
+      dl[step_slot((at + e) / 2)] = o;
     }
   }
 }
 
+// The steps of the lane's channels at `at` = token * CHW + channel.
 template <int KD>
 __device__ __forceinline__ void read_steps(const float4* dl, int at, ulonglong2 (&v)[KD / 2]) {
-  const ulonglong2* s = reinterpret_cast<const ulonglong2*>(dl + at / 2);
 #pragma unroll
-  for (int j = 0; j < KD / 2; ++j) v[j] = s[j];
+  for (int j = 0; j < KD / 2; ++j) v[j] = *reinterpret_cast<const ulonglong2*>(dl + step_slot(at / 2 + j));
 }
 
 // The sums of dt of a range.
@@ -454,7 +463,7 @@ struct FwdSmem {
 enum ScanPhase { kPhaseCarry = 0, kPhaseMain = 1 };
 
 template <typename T, int LN, int PHASE>
-__global__ void __launch_bounds__(kScanWarps * 32, FB) ssm_scan_fwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const ScanParams p) {
   extern __shared__ float4 smem4[];
   constexpr int KD = kFwdChans;
   using L = Lanes<LN, KD>;
@@ -509,8 +518,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, FB) ssm_scan_fwd_kernel(const
       slot = slot_of(p, g.s, false);
     }
   }
-  float bias[V], skip[V];
-  load_column<V>(p.dbias, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), bias);
+  using SV = StepVecs<CHW>;
+  float bias[SV::V], skip[V];
+  load_column<SV::V>(p.dbias, l.c0 + SV::chan(lane), l.nch - SV::chan(lane), bias);
   if (kMain) load_column<V>(p.skip, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), skip);
   f2 dsum[KD / 2];
 #pragma unroll
@@ -549,8 +559,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, FB) ssm_scan_fwd_kernel(const
   for (int tile0 = tile_first; tile0 < t1; tile0 += kTile, cur ^= 1) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
     copy_wait();
+    __syncwarp();
     bc = stage(cur, 3);
-    stage_steps<T>(p, l, tile_rows(tile0, ta, tb), stage(cur, 0), stage(cur, 1), bias, dl);
+    stage_steps<T>(p, l, stage(cur, 0), stage(cur, 1), bias, dl);
     __syncwarp();
     // (the other stage's B and C were last read ahead of the barrier before)
     if (tile0 + kTile < t1) fetch(tile0 + kTile, cur ^ 1);
@@ -573,7 +584,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, FB) ssm_scan_fwd_kernel(const
           }
         }
         if (stop - t == kTile) {
-#pragma unroll kFU
+#pragma unroll
           for (int r = 0; r < kTile; ++r) step(r);
         } else {
           for (int r = t - tile0; r < stop - tile0; ++r) step(r);

@@ -78,28 +78,27 @@ __device__ __forceinline__ void carry_back(const ScanParams& p, const Lanes<LN, 
   carry_through(p, l, j1, i + 1, -1, A2, r);
 }
 
-// dy of a tile into shared memory (zeros in rows without their bit).
+// dy of a tile into shared memory.
 template <typename T, int LN, int KD>
 __device__ __forceinline__ void stage_dy(const ScanParams& p, const Lanes<LN, KD>& l, const T* g, const T* z,
-                                         unsigned rows, float* dy) {
+                                         float* dy) {
   constexpr int CHW = Lanes<LN, KD>::CHW;
-  using TV = TileVecs<CHW>;
-  constexpr int V = TV::V;
+  using SV = StepVecs<CHW>;
+  constexpr int V = SV::V;
 #pragma unroll
-  for (int k = 0; k < TV::NVEC; ++k) {
-    if (!TV::has(k, l.lane)) continue;
-    const int r = TV::row(k, l.lane);
-    const Pack<T, V> gv = tile_vec<T, CHW>(g, k, l.lane);
+  for (int k = 0; k < SV::NVEC; ++k) {
+    if (!SV::has(k, l.lane)) continue;
+    const int at = SV::row(k, l.lane) * CHW + SV::chan(l.lane);
+    const Pack<T, V> gv = load_part<T, V>(g + at, V, true);
     Pack<T, V> zv;
-    if (p.gate != nullptr) zv = tile_vec<T, CHW>(z, k, l.lane);
+    if (p.gate != nullptr) zv = load_part<T, V>(z + at, V, true);
     Pack<float, V> o;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      float v = to_f(gv.v[e]);
-      if (p.gate != nullptr) v *= to_f(zv.v[e]) * sigmoid_t<T>(to_f(zv.v[e]));
-      o.v[e] = (rows >> r) & 1 ? v : 0.f;
+      o.v[e] = to_f(gv.v[e]);
+      if (p.gate != nullptr) o.v[e] *= to_f(zv.v[e]) * sigmoid_t<T>(to_f(zv.v[e]));
     }
-    store_part<float, V>(dy + r * CHW + TV::chan(l.lane), o, V, true);
+    store_part<float, V>(dy + at, o, V, true);
   }
 }
 
@@ -144,8 +143,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   LaneStates<KD> A2, r;
   load_rates(p, l, A2);
   zero_states<KD>(r);
-  float bias[TV::V];
-  load_column<TV::V>(p.dbias, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), bias);
+  using SV = StepVecs<CHW>;
+  float bias[SV::V];
+  load_column<SV::V>(p.dbias, l.c0 + SV::chan(lane), l.nch - SV::chan(lane), bias);
   f2 dsum[KD / 2];
 #pragma unroll
   for (int j = 0; j < KD / 2; ++j) dsum[j] = 0ull;
@@ -178,10 +178,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   for (int tile0 = last; tile0 + kTile > t0; tile0 -= kTile, cur ^= 1) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
     copy_wait();
+    __syncwarp();
     bc = stage(cur, 3);
-    const unsigned rows = tile_rows(tile0, ta, tb);
-    stage_steps<T>(p, l, rows, stage(cur, 0), stage(cur, 1), bias, dl);
-    stage_dy<T>(p, l, stage(cur, 0), stage(cur, 2), rows, dy);
+    stage_steps<T>(p, l, stage(cur, 0), stage(cur, 1), bias, dl);
+    stage_dy<T>(p, l, stage(cur, 0), stage(cur, 2), dy);
     __syncwarp();
     if (tile0 > t0) fetch(tile0 - kTile, cur ^ 1);
     if (tb - ta == kTile) {
@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
         float4 o;
         unpack2(s, o.x, o.y);
         unpack2(su, o.z, o.w);
-        const bool c0 = in && c + e < l.nch, c1 = in && c + e + 1 < l.nch;
-        dl[(at + e) / 2] = make_float4(c0 ? o.x : 0.f, c1 ? o.y : 0.f, c0 ? o.z : 0.f, c1 ? o.w : 0.f);
+        if (!in) o = make_float4(0.f, 0.f, 0.f, 0.f);
+        dl[step_slot((at + e) / 2)] = o;
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) dy.v[e] = to_f(go.v[e]);
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     auto forward = [&](auto general) {
 #pragma unroll
       for (int r = 0; r < kTile; ++r) {
-        const float4 dv = dl[(r * CHW + l.ch(0)) / 2];
+        const float4 dv = dl[step_slot((r * CHW + l.ch(0)) / 2)];
         const float dt[KD] = {dv.x, dv.y}, du[KD] = {dv.z, dv.w};
         f2 b[2], c[2];
         float y[KD];
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
       for (int r = kTile - 1; r >= 0; --r) {
         const bool first = decltype(general)::value && ((q.first >> r) & 1);
         const bool none = decltype(general)::value && !((q.live >> r) & 1);
-        const float4 dv = dl[(r * CHW + l.ch(0)) / 2];
+        const float4 dv = dl[step_slot((r * CHW + l.ch(0)) / 2)];
         const float2 dyv = *reinterpret_cast<const float2*>(dys + r * CHW + l.ch(0));
         const float dt[KD] = {dv.x, dv.y}, du[KD] = {dv.z, dv.w}, dy[KD] = {dyv.x, dyv.y};
         f2 b[2], c[2], dB[2], dC[2];
@@ -484,13 +484,13 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
       const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane);
       const Pack<float, V> sl = load_part<float, V>(slope + at, V, true), dy = load_part<float, V>(dys + at, V, true),
                            skip = load_part<float, V>(cols + 32 * V, V, true);
-      const Pack<float, 2 * V> steps = load_part<float, 2 * V>(reinterpret_cast<const float*>(dl) + at * 2, 2 * V, true),
-                               sp = load_part<float, 2 * V>(reinterpret_cast<const float*>(pair + at), 2 * V, true);
+      const Pack<float, 2 * V> sp = load_part<float, 2 * V>(reinterpret_cast<const float*>(pair + at), 2 * V, true);
       Pack<float, V> s0 = load_part<float, V>(sums, V, true), s1 = load_part<float, V>(sums + 32 * V, V, true);
       Pack<T, V> du, dd, dz;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float uv = to_f(u.v[e]), dt = steps.v[e / 2 * 4 + e % 2], sa = sp.v[2 * e], gb = sp.v[2 * e + 1];
+        const float4 st = dl[step_slot((at + e) / 2)];
+        const float uv = to_f(u.v[e]), dt = e % 2 == 0 ? st.x : st.y, sa = sp.v[2 * e], gb = sp.v[2 * e + 1];
         const float ddt = fmaf(kLn2, sa, uv * gb) * sl.v[e];
         du.v[e] = from_f<T>(in ? fmaf(dt, gb, skip.v[e] * dy.v[e]) : 0.f);
         dd.v[e] = from_f<T>(in ? ddt : 0.f);
