@@ -43,39 +43,47 @@ int run_tokens(int64_t T, int64_t warps_per_run, int lo, int hi) {
   return L;
 }
 
-template <typename T, int NV, int WT, bool PACKED>
-cudaError_t fwd_one(const ConvParams& p, dim3 grid, cudaStream_t st) {
-  return launch(ssm_conv_fwd_kernel<T, NV, WT, PACKED>, grid, dim3(32, kRuns), 0, st, p);
+// Elements of a thread's vector for a kernel of WT taps: 16 bytes for the small
+// kernels, half and a quarter of it for the wide ones, whose windows and
+// filters take W registers a channel each.
+template <typename T, int WT>
+constexpr int vec_of() {
+  constexpr int bytes = WT > 0 ? 16 : WT == -8 ? 8 : 4;
+  return bytes / (int)sizeof(T);
 }
 
-template <typename T, int NV, bool PACKED>
-cudaError_t fwd_w(const ConvParams& p, dim3 grid, cudaStream_t st) {
-  if constexpr (NV > 1) {
-    switch (p.W) {
-      case 2: return fwd_one<T, NV, 2, PACKED>(p, grid, st);
-      case 3: return fwd_one<T, NV, 3, PACKED>(p, grid, st);
-      case 4: return fwd_one<T, NV, 4, PACKED>(p, grid, st);
-    }
+// The kernel's template value for W taps.
+template <typename F>
+int with_taps(int W, F f) {
+  switch (W) {
+    case 2: return f(std::integral_constant<int, 2>());
+    case 3: return f(std::integral_constant<int, 3>());
+    case 4: return f(std::integral_constant<int, 4>());
   }
-  if (p.W <= 8) return fwd_one<T, NV, -8, PACKED>(p, grid, st);
-  return fwd_one<T, NV, -kMaxWGeneric, PACKED>(p, grid, st);
+  return W <= 8 ? f(std::integral_constant<int, -8>()) : f(std::integral_constant<int, -kMaxWGeneric>());
 }
 
-// Vectors of 16 bytes where every row starts on one; else single elements.
-template <typename T, bool PACKED>
-int fwd_type(ConvParams p, cudaStream_t st) {
-  constexpr int NV = 16 / sizeof(T);
-  p.vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, 16) && aligned(p.y, 16);
-  const int nv = p.vec ? NV : 1;
-  p.vec_w = p.sw_d == 1 && p.sw_k % nv == 0 && aligned(p.w, nv * sizeof(T));
-  if (p.state != nullptr) p.st_layout = state_layout(p.state, p.s_slot, p.s_d, p.s_h, p.W - 1, nv, sizeof(T));
-  const int64_t cw = cdiv(cdiv(p.D, nv), 32);
+template <typename T, int NV, int WT, bool PACKED>
+int fwd_one(ConvParams p, cudaStream_t st) {
+  p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
+  if (p.state != nullptr) p.st_layout = state_layout(p.state, p.s_slot, p.s_d, p.s_h, p.W - 1, NV, sizeof(T));
+  const int64_t cw = cdiv(cdiv(p.D, NV), 32);
   p.L = run_tokens(p.q.T, cw, 1, 64);
   p.nblk = (int)cw;
   const int64_t blocks = cdiv(cdiv(p.q.T, p.L), kRuns) * cw;
   if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
-  const dim3 grid((unsigned)blocks);
-  return finish(p.vec ? fwd_w<T, NV, PACKED>(p, grid, st) : fwd_w<T, 1, PACKED>(p, grid, st));
+  const size_t smem = NV > 1 ? (size_t)kRuns * ConvRing<T, NV>::kBytes : 0;
+  return finish(launch(ssm_conv_fwd_kernel<T, NV, WT, PACKED>, dim3((unsigned)blocks), dim3(32, kRuns), smem, st, p));
+}
+
+// Whole vectors where every row starts on one; else single elements.
+template <typename T, bool PACKED>
+int fwd_type(const ConvParams& p, cudaStream_t st) {
+  return with_taps(p.W, [&](auto taps) {
+    constexpr int WT = decltype(taps)::value, NV = vec_of<T, WT>();
+    const bool vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) && aligned(p.y, NV * sizeof(T));
+    return vec ? fwd_one<T, NV, WT, PACKED>(p, st) : fwd_one<T, 1, WT, PACKED>(p, st);
+  });
 }
 
 template <bool PACKED>
@@ -88,53 +96,40 @@ int fwd(int dtype, const ConvParams& p, void* stream) {
   }
 }
 
-// Backward runs: four channels a thread (its sums take 2 W + 1 registers each).
-constexpr int kBwdVec = 4;
 constexpr int kBwdMinRun = 8, kBwdMaxRun = 64;
 
-// Blocks of runs of the backward, an upper bound for any channel vector.
+// Rows of partial sums of the backward.
 int64_t bwd_rows(int64_t T, int L) { return cdiv(cdiv(T, L), kRuns); }
 
 template <typename T, int NV, int WT>
-cudaError_t bwd_one(const ConvParams& p, dim3 grid, size_t smem, cudaStream_t st) {
-  auto k = ssm_conv_bwd_kernel<T, NV, WT>;
-  cudaError_t e = allow_smem(k, smem);
-  if (e != cudaSuccess) return e;
-  return launch(k, grid, dim3(32, kRuns), smem, st, p);
-}
-
-template <typename T, int NV>
-cudaError_t bwd_w(const ConvParams& p, dim3 grid, size_t smem, cudaStream_t st) {
-  if constexpr (NV > 1) {
-    switch (p.W) {
-      case 2: return bwd_one<T, NV, 2>(p, grid, smem, st);
-      case 3: return bwd_one<T, NV, 3>(p, grid, smem, st);
-      case 4: return bwd_one<T, NV, 4>(p, grid, smem, st);
-    }
-  }
-  if (p.W <= 8) return bwd_one<T, NV, -8>(p, grid, smem, st);
-  return bwd_one<T, NV, -kMaxWGeneric>(p, grid, smem, st);
-}
-
-template <typename T>
-int bwd_type(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
-  constexpr int NV = kBwdVec;
-  p.vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) && aligned(p.dout, NV * sizeof(T)) &&
-          aligned(p.dx, NV * sizeof(T));
-  const int nv = p.vec ? NV : 1;
-  p.vec_w = p.sw_d == 1 && p.sw_k % nv == 0 && aligned(p.w, nv * sizeof(T));
-  const int64_t cw = cdiv(cdiv(p.D, nv), 32);
+int bwd_one(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
+  p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
+  const int64_t cw = cdiv(cdiv(p.D, NV), 32);
   p.L = run_tokens(p.q.T, cw, kBwdMinRun, kBwdMaxRun);
   p.nblk = (int)cw;
   const int64_t rows = bwd_rows(p.q.T, p.L);
   if (rows * cw > INT_MAX) return GRETA_ERR_INVALID_ARG;
-  const size_t smem = (size_t)kRuns * (p.W + 1) * 32 * nv * sizeof(float);
-  const dim3 grid((unsigned)(rows * cw));
-  cudaError_t e = p.vec ? bwd_w<T, NV>(p, grid, smem, st) : bwd_w<T, 1>(p, grid, smem, st);
+  const size_t sums = (size_t)kRuns * (p.W + 1) * 32 * NV * sizeof(float);
+  const size_t rings = NV > 1 ? (size_t)kRuns * 2 * ConvRing<T, NV>::kBytes : 0;
+  const size_t smem = sums > rings ? sums : rings;
+  auto k = ssm_conv_bwd_kernel<T, NV, WT>;
+  cudaError_t e = allow_smem(k, smem);
+  if (e == cudaSuccess) e = launch(k, dim3((unsigned)(rows * cw)), dim3(32, kRuns), smem, st, p);
   if (e != cudaSuccess) return GRETA_ERR_LAUNCH;
   const int64_t cols = cdiv((int64_t)(p.W + 1) * p.D, 32);
   return finish(launch(ssm_conv_reduce_kernel<T>, dim3((unsigned)cols), dim3(32, 8), 0, st, (const float*)p.part,
                        reinterpret_cast<T*>(dw), reinterpret_cast<T*>(dbias), (long long)rows, p.D, p.W));
+}
+
+// Vectors of half the forward's: a thread's sums take 3 W registers a channel.
+template <typename T>
+int bwd_type(const ConvParams& p, void* dw, void* dbias, cudaStream_t st) {
+  return with_taps(p.W, [&](auto taps) {
+    constexpr int WT = decltype(taps)::value, NV = vec_of<T, WT>() >= 4 ? vec_of<T, WT>() / 2 : vec_of<T, WT>();
+    const bool vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) &&
+                     aligned(p.dout, NV * sizeof(T)) && aligned(p.dx, NV * sizeof(T));
+    return vec ? bwd_one<T, NV, WT>(p, dw, dbias, st) : bwd_one<T, 1, WT>(p, dw, dbias, st);
+  });
 }
 
 ConvParams base(const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d, const void* bias,

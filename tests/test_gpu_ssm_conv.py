@@ -211,6 +211,29 @@ def test_packed_long_and_strided():
     check_packed([50, 1, 70], [1, 0, 2], [1, 1, 0], 101, 3, torch.float16, ld=203, silu=False)
 
 
+@pytest.mark.parametrize("W", [4, 7])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_state_keeps_bits(W, dtype):
+    """Every 16-bit pattern, NaN payloads among them, goes into the slots as it
+    is: from short requests, ones inside a run and ones over several."""
+    from greta_plugin_b200 import packed_causal_conv1d
+
+    lens, D = [1, 2, 5, 200, 1], 512
+    g = torch.Generator().manual_seed(W)
+    bits = lambda *s: torch.randint(-2 ** 15, 2 ** 15, s, generator=g).to(torch.int16).to(DEV).view(dtype)  # noqa: E731
+    x, state = bits(sum(lens), D), bits(6, D, W - 1)
+    want, starts = state.clone().view(torch.int16), ragged_cu(lens)
+    slots, init = [3, 0, 5, 1, 2], [1, 1, 0, 1, 0]
+    for i, k in enumerate(slots):
+        past = want[k] if init[i] else torch.zeros_like(want[k])
+        rows = x[int(starts[i]):int(starts[i + 1])].view(torch.int16).t()
+        want[k] = torch.cat([past, rows], 1)[:, 1 - W:]
+    packed_causal_conv1d(x, torch.zeros(W, D, dtype=dtype, device=DEV), None, state, starts.to(DEV),
+                         torch.tensor(slots, dtype=torch.int32, device=DEV),
+                         torch.tensor(init, dtype=torch.int8, device=DEV))
+    assert torch.equal(state.view(torch.int16), want)
+
+
 def test_packed_slot_out_of_range():
     from greta_plugin_b200 import packed_causal_conv1d_checked
 
