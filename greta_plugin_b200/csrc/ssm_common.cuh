@@ -9,6 +9,8 @@
 // offsets is the same in all lanes.
 #pragma once
 
+#include <climits>
+
 #include "dynconv_common.cuh"
 
 namespace greta {
@@ -27,23 +29,6 @@ __device__ __forceinline__ int seq_start(const Seqs& q, int i) {
   return (int)clampll(load_idx(q.starts, i, q.is64), 0, q.T);
 }
 
-// The largest s in [-1, nseq] with seq_start(s) <= t (-1: t is ahead of the
-// first sequence, nseq: behind the last). 32 probes a round, so two rounds for
-// a thousand sequences; every lane of the warp calls it with the same t. Ends
-// on any contents of `starts`.
-__device__ __forceinline__ int warp_find(const Seqs& q, int t, int lane) {
-  int lo = -1, hi = q.nseq + 1;
-  while (hi - lo > 1) {
-    const int step = (hi - lo - 1 + 31) / 32;
-    const int idx = lo + step * (lane + 1);
-    const bool ok = idx < hi && seq_start(q, idx) <= t;
-    const int cnt = __popc(__ballot_sync(0xffffffffu, ok));
-    lo += step * cnt;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
-
 // A run of tokens [b, e) that one sequence s holds (in), or that none does
 // (ahead of the first sequence, s = -1, or behind the last, s = nseq).
 struct Seg {
@@ -51,29 +36,61 @@ struct Seg {
   bool in;
 };
 
-__device__ __forceinline__ Seg seg_make(const Seqs& q, int s, int t) {
-  Seg g;
-  g.s = s;
-  g.in = s >= 0 && s < q.nseq;
-  g.b = s >= 0 ? seq_start(q, s) : 0;
-  g.e = s < q.nseq ? seq_start(q, s + 1) : q.T;
-  if (g.e <= t) g.e = t + 1;  // offsets that fall: stay on the way forward
-  return g;
-}
+// The offsets as a warp asks for them; every lane asks the same. Up to 31
+// sequences are read once, an offset per lane (a question is then a ballot or a
+// shuffle: a lookup's loads one after another are what short runs wait for).
+struct SeqView {
+  Seqs q;
+  int lane, mine;
+  bool held;
 
-__device__ __forceinline__ Seg seg_at(const Seqs& q, int t, int lane) {
-  return seg_make(q, warp_find(q, t, lane), t);
-}
+  __device__ __forceinline__ SeqView(const Seqs& seqs, int lane_) : q(seqs), lane(lane_) {
+    held = q.nseq < 32;
+    mine = held && lane <= q.nseq ? seq_start(q, lane) : INT_MAX;
+  }
 
-// The segment that begins where `g` ends (sequences of no tokens are passed).
-__device__ __forceinline__ Seg seg_next(const Seqs& q, const Seg& g) {
-  const int t = g.e;
-  int s = g.s + 1;
-  while (s < q.nseq && seq_start(q, s + 1) <= t) ++s;
-  Seg n = seg_make(q, s, t);
-  n.b = t;
-  return n;
-}
+  __device__ __forceinline__ int start(int i) const {
+    return held ? __shfl_sync(0xffffffffu, mine, i) : seq_start(q, i);
+  }
+
+  // The largest s in [-1, nseq] with start(s) <= t (-1: t is ahead of the first
+  // sequence, nseq: behind the last). 32 probes a round, so two rounds for a
+  // thousand sequences. Ends on any contents of the offsets.
+  __device__ __forceinline__ int find(int t) const {
+    if (held) return __popc(__ballot_sync(0xffffffffu, mine <= t)) - 1;
+    int lo = -1, hi = q.nseq + 1;
+    while (hi - lo > 1) {
+      const int step = (hi - lo - 1 + 31) / 32;
+      const int idx = lo + step * (lane + 1);
+      const bool ok = idx < hi && seq_start(q, idx) <= t;
+      const int cnt = __popc(__ballot_sync(0xffffffffu, ok));
+      lo += step * cnt;
+      hi = min(hi, lo + step);
+    }
+    return lo;
+  }
+
+  __device__ __forceinline__ Seg make(int s, int t) const {
+    Seg g;
+    g.s = s;
+    g.in = s >= 0 && s < q.nseq;
+    g.b = s >= 0 ? start(s) : 0;
+    g.e = s < q.nseq ? start(s + 1) : q.T;
+    if (g.e <= t) g.e = t + 1;  // offsets that fall: stay on the way forward
+    return g;
+  }
+  __device__ __forceinline__ Seg at(int t) const { return make(find(t), t); }
+
+  // The segment that begins where `g` ends (sequences of no tokens are passed).
+  __device__ __forceinline__ Seg next(const Seg& g) const {
+    const int t = g.e;
+    int s = g.s + 1;
+    while (s < q.nseq && start(s + 1) <= t) ++s;
+    Seg n = make(s, t);
+    n.b = t;
+    return n;
+  }
+};
 
 // Where range i of L tokens begins. (Borders moved to sequence starts close by
 // save some carries, but ranges of uneven length cost more than that.)

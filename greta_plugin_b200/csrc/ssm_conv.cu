@@ -34,10 +34,15 @@ int check(int dtype, const void* x, int64_t ldx, const void* w, const void* y, c
   return GRETA_OK;
 }
 
-// Tokens per run: as many as leave each SM 16 warps (enough rows in flight to
-// fill HBM), a power of two between lo and hi.
+// Tokens beyond one per request up to which a batch is a decode batch: its
+// longest request then has at most kDecodeExtra + 1 tokens, walked one after
+// another.
+constexpr int64_t kDecodeExtra = 8;
+
+// Tokens per run: as many as leave each SM 12 warps (all of them running at
+// once, and enough rows in flight to fill HBM), a power of two between lo and hi.
 int run_tokens(int64_t T, int64_t warps_per_run, int lo, int hi) {
-  const int64_t want = T * warps_per_run / ((int64_t)sm_count() * 16);
+  const int64_t want = T * warps_per_run / ((int64_t)sm_count() * 12);
   int L = lo;
   while (L < hi && 2 * L <= want) L *= 2;
   return L;
@@ -68,8 +73,13 @@ int fwd_one(ConvParams p, cudaStream_t st) {
   p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
   if (p.state != nullptr) p.st_layout = state_layout(p.state, p.s_slot, p.s_d, p.s_h, p.W - 1, NV, sizeof(T));
   const int64_t cw = cdiv(cdiv(p.D, NV), 32);
-  p.L = run_tokens(p.q.T, cw, 1, 64);
   p.nblk = (int)cw;
+  if (PACKED && p.q.nseq > 0 && p.q.T <= p.q.nseq + kDecodeExtra) {
+    const int64_t blocks = cdiv(p.q.nseq, kRuns) * cw;
+    if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
+    return finish(launch(ssm_conv_decode_kernel<T, NV, WT>, dim3((unsigned)blocks), dim3(32, kRuns), 0, st, p));
+  }
+  p.L = run_tokens(p.q.T, cw, 1, 64);
   const int64_t blocks = cdiv(cdiv(p.q.T, p.L), kRuns) * cw;
   if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
   const size_t smem = NV > 1 ? (size_t)kRuns * ConvRing<T, NV>::kBytes : 0;

@@ -265,12 +265,8 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
   ring.ld = p.ldx;
   ring.n = n;
   Chans<NV> w[MW], bias, win[MH];
-  Seg g;
-  // one token per run: in a batch of single tokens, token t is sequence t
-  if (PACKED && p.L == 1 && t < p.q.nseq && seq_start(p.q, t) == t && seq_start(p.q, t + 1) == t + 1)
-    g = Seg{t, t, t + 1, true};
-  else
-    g = seg_at(p.q, t, lane);
+  const SeqView sv(p.q, lane);
+  Seg g = sv.at(t);
 
   int tend = t1;
   if (PACKED && H > 0) {
@@ -281,10 +277,10 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
       const int skip = min(g.b + H, g.e);
       if (skip >= t1) return;
       t = skip;
-      if (t == g.e) g = seg_next(p.q, g);
+      if (t == g.e) g = sv.next(g);
     }
     if (t1 < p.q.T && t1 != g.e) {
-      const Seg last = g.in && g.e > t1 ? g : seg_at(p.q, t1, lane);
+      const Seg last = g.in && g.e > t1 ? g : sv.at(t1);
       if (last.in && t1 > last.b && t1 - last.b < H) tend = min(last.b + H, last.e);
     }
   }
@@ -308,12 +304,12 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
     conv_zero<NV>(win);
     slot = -1;
     if (!PACKED || p.state == nullptr) return;
-    const int raw = p.slots[g.s];
+    const int raw = p.slots[g.s], initial = p.initial[g.s];
     if (raw >= p.num_slots && p.err != nullptr && c0 == 0) atomicOr(p.err, 1);
     slot = raw >= 0 && raw < p.num_slots ? raw : -1;
 #pragma unroll
     for (int h = 0; h < MH; ++h) zero(old[h]);
-    if (slot >= 0 && p.initial[g.s] != 0) {
+    if (slot >= 0 && initial != 0) {
       conv_load_state<T, NV, MH>(p, slot, c0, n, H, old, WT > 1);
 #pragma unroll
       for (int h = 0; h < MH; ++h)
@@ -376,7 +372,7 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
 #pragma unroll 1
       for (int i = 0; i < kGroup && t + i < tend; ++i) {
         const int ti = t + i;
-        if (ti >= g.e) g = seg_next(p.q, g);
+        if (ti >= g.e) g = sv.next(g);
         if (g.in) {
           if (ti == g.b) begin();
           token(ti, ring.row(group, t, i));
@@ -388,6 +384,86 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
         }
       }
     }
+  }
+}
+
+// Batches of (nearly) one token per request: a warp has the channels of one
+// request and walks its tokens, with filters and window in the element type (a
+// third of the registers, so that all of a step's warps run at once) and with
+// the metadata, the first token's row and the filters asked for together.
+template <typename T, int NV, int WT>
+__global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p) {
+  constexpr int MW = WT > 0 ? WT : -WT;
+  constexpr int MH = MW > 1 ? MW - 1 : 1;
+  const int W = WT > 0 ? WT : p.W;
+  const int H = W - 1;
+  const int lane = threadIdx.x & 31;
+  const int c0 = ((int)(blockIdx.x % p.nblk) * 32 + lane) * NV;
+  const int n = max(0, min(NV, p.D - c0));
+  const bool vec = NV > 1 && n == NV;
+  const int r = (int)(blockIdx.x / p.nblk) * blockDim.y + threadIdx.y;
+  const T* xg = reinterpret_cast<const T*>(p.x) + c0;
+  T* yg = reinterpret_cast<T*>(p.y) + c0;
+  const T* wg = reinterpret_cast<const T*>(p.w);
+  pdl_wait();
+  pdl_trigger();
+  if (r >= p.q.nseq) return;
+  const int b = seq_start(p.q, r), e = seq_start(p.q, r + 1), raw = p.slots[r], initial = p.initial[r];
+  Pack<T, NV> x, w[MW], win[MH];
+  zero(x);
+  if (r < p.q.T) x = load_part<T, NV>(xg + (long long)r * p.ldx, n, vec);  // its row, in a batch of single tokens
+  float bias[NV];
+#pragma unroll
+  for (int k = 0; k < MW; ++k) {
+    zero(w[k]);
+    const int tap = k - (MW - W);
+    if (tap < 0) continue;
+    if (p.vec_w) {
+      w[k] = load_part<T, NV>(wg + (long long)tap * p.sw_k + c0, n, n == NV);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+        if (c < n) w[k].v[c] = wg[(long long)tap * p.sw_k + (long long)(c0 + c) * p.sw_d];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+    bias[c] = p.bias != nullptr && c < n ? to_f(reinterpret_cast<const T*>(p.bias)[c0 + c]) : 0.f;
+#pragma unroll
+  for (int h = 0; h < MH; ++h) zero(win[h]);
+  int slot = -1;
+  if (p.state != nullptr && b < e) {
+    if (raw >= p.num_slots && p.err != nullptr && c0 == 0) atomicOr(p.err, 1);
+    slot = raw >= 0 && raw < p.num_slots ? raw : -1;
+    if (slot >= 0 && initial != 0) conv_load_state<T, NV, MH>(p, slot, c0, n, H, win, WT > 1);
+  }
+  for (int t = b; t < e; ++t) {
+    if (t != r) x = load_part<T, NV>(xg + (long long)t * p.ldx, n, vec);
+    Pack<T, NV> o;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      float s = bias[c];
+#pragma unroll
+      for (int k = 0; k < MW; ++k) {
+        if (k == MW - 1)
+          s = fma_io(w[k].v[c], x.v[c], s);
+        else if (k >= MW - W)
+          s = fma_io(w[k].v[c], win[k < MH ? k : 0].v[c], s);
+      }
+      o.v[c] = from_f<T>(p.silu ? s * sigmoid_t<T>(s) : s);
+    }
+    store_part<T, NV>(yg + (long long)t * p.D, o, n, vec);
+#pragma unroll
+    for (int h = 0; h < MH; ++h) win[h] = h + 1 < MH ? win[h + 1 < MH ? h + 1 : h] : x;
+  }
+  if (slot >= 0) conv_store_state<T, NV, MH>(p, slot, c0, n, H, win, WT > 1);
+  if (p.zero_rest) {
+    Pack<T, NV> z;
+    zero(z);
+    if (r == 0)
+      for (int t = 0; t < b; ++t) store_part<T, NV>(yg + (long long)t * p.D, z, n, vec);
+    if (r == p.q.nseq - 1)
+      for (int t = e; t < p.q.T; ++t) store_part<T, NV>(yg + (long long)t * p.D, z, n, vec);
   }
 }
 
@@ -455,7 +531,8 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
     conv_weights<T, NV>(p, c0, n, W, w, bias);
     conv_zero<NV>(win);
     conv_zero<NV>(acc);
-    Seg g = seg_at(p.q, t0, lane);
+    const SeqView sv(p.q, lane);
+    Seg g = sv.at(t0);
     if (g.in && t0 > g.b) {
 #pragma unroll
       for (int h = 0; h < MH; ++h)
@@ -533,7 +610,7 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
 #pragma unroll 1
         for (int i = 0; i < kGroup && t + i < t2; ++i) {
           const int ti = t + i;
-          if (ti < tin && ti >= g.e) g = seg_next(p.q, g);
+          if (ti < tin && ti >= g.e) g = sv.next(g);
           if (ti < tin && g.in) {
             if (ti == g.b) conv_zero<NV>(win);
             token(ti, rx.row(group, t, i), rd.row(group, t, i), std::false_type());

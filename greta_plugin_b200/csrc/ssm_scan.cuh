@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
   if (slice >= p.F * p.spg) return;
   const L l(p, slice, lane);
   const int ri = blockIdx.y;
+  const SeqView sv(p.q, lane);
   int t0 = range_begin(p.q, ri, p.L);
   const int t1 = range_begin(p.q, ri + 1, p.L);
   if (t0 >= t1) return;
@@ -495,7 +496,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
   int slot = -1;
   if (!kMain) {
     if (t1 >= p.q.T) return;
-    g = seg_at(p.q, t1, lane);
+    g = sv.at(t1);
     if (!g.in || g.b >= t1) return;  // the next range begins with a sequence, or outside
     load_rates(p, l, A2);
     zero_states<KD>(h);
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
       }
     }
   } else {
-    g = seg_at(p.q, t0, lane);
+    g = sv.at(t0);
     load_rates(p, l, A2);
     zero_states<KD>(h);
     if (g.in && g.b < t0) {
@@ -593,7 +594,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
         if (kMain && stop == g.e && slot >= 0) store_slot(p, slot, l, h);
       }
       t = stop;
-      if (t == g.e && t < t1) g = seg_next(p.q, g);
+      if (t == g.e && t < t1) g = sv.next(g);
     }
     __syncwarp();
     if (kMain) {

@@ -43,9 +43,9 @@ constexpr int kBwdChans = 2;  // channels per lane of the backward kernel
 struct TileSeqs {
   unsigned first, live;
 };
-__device__ __forceinline__ TileSeqs tile_seqs(const Seqs& q, int tile0, int ta, int tb, int lane, Seg& g) {
+__device__ __forceinline__ TileSeqs tile_seqs(const SeqView& sv, int tile0, int ta, int tb, Seg& g) {
   TileSeqs s{0u, 0u};
-  if (!(g.in && g.b <= ta && g.e >= tb)) g = seg_at(q, ta, lane);
+  if (!(g.in && g.b <= ta && g.e >= tb)) g = sv.at(ta);
   Seg w = g;
   int t = ta;
   while (true) {
@@ -56,7 +56,7 @@ __device__ __forceinline__ TileSeqs tile_seqs(const Seqs& q, int tile0, int ta, 
     }
     t = stop;
     if (t >= tb) return s;
-    w = seg_next(q, w);
+    w = sv.next(w);
   }
 }
 
@@ -132,10 +132,11 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   const L l(p, slice, lane);
   const int ri = blockIdx.y;
   if (ri == 0) return;
+  const SeqView sv(p.q, lane);
   const int t0 = range_begin(p.q, ri, p.L);
   int t1 = range_begin(p.q, ri + 1, p.L);
   if (t0 >= t1) return;
-  const Seg g = seg_at(p.q, t0, lane);
+  const Seg g = sv.at(t0);
   if (!g.in || g.b >= t0) return;
   const bool reset = g.e <= t1;
   if (slice == 0 && lane == 0) p.reset[ri] = reset;
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   L l(p, f * p.spg + (have ? in_group : 0), lane);
   if (!have) l.nch = 0;
   const int ri = blockIdx.y;
+  const SeqView sv(p.q, lane);
   const int t0 = range_begin(p.q, ri, p.L);
   const int t1 = range_begin(p.q, ri + 1, p.L);
   const long long DN = (long long)p.D * p.N;
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     load_rates(p, l, a);
     zero_states<KD>(r);
     if (t0 < t1 && t1 < p.q.T) {
-      const Seg g = seg_at(p.q, t1, lane);
+      const Seg g = sv.at(t1);
       if (g.in && g.b < t1) carry_back(p, l, ri, a, r);
     }
     by_states(a[0], A2);
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   int cur = 0;
   for (int tile0 = last; tile0 + kTile > t0 && tile0 >= 0; tile0 -= kTile, cur ^= 1) {
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
-    const TileSeqs q = tile_seqs(p.q, tile0, ta, tb, lane, g);
+    const TileSeqs q = tile_seqs(sv, tile0, ta, tb, g);
     copy_wait();
     const T* bc = reinterpret_cast<T*>(base + cur * S::kBC);
     f2 hs[kTile + 1][KD][2];
