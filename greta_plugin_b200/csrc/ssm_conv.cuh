@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
     if (slot >= 0 && initial != 0) conv_load_state<T, NV, MH>(p, slot, c0, n, H, win, WT > 1);
   }
   for (int t = b; t < e; ++t) {
-    if (t != r) x = load_part<T, NV>(xg + (long long)t * p.ldx, n, vec);
+    if (t != r || t != b) x = load_part<T, NV>(xg + (long long)t * p.ldx, n, vec);
     Pack<T, NV> o;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {

@@ -626,102 +626,164 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
 
 // Batches of (nearly) one token per request: bound by the states' read and
 // write, 8 D N bytes a request. A warp has the channels and states of Lanes for
-// RQ requests, all of whose states, rows and metadata it asks for before it
-// computes, with the decay rates read once; requests of more tokens (few, by
-// the host's rule) are walked token by token.
-template <typename T, int LN, int RQ>
+// a chunk of up to 32 requests, whose metadata its lanes hold and whose decay
+// rates it reads once; states and first rows of the next kAhead requests are
+// on their way in asynchronous copies while one is computed. (A warp per
+// request or two, with loads into registers, spent its time on one chain of
+// latencies after the other: 44 us for 256 requests of 4096 x 16.) Requests of
+// more tokens (few, by the host's rule) are walked token by token.
+constexpr int kAhead = 3;
+
+template <typename T, int LN>
+struct DecodeSmem {
+  static constexpr int CHW = Lanes<LN>::CHW, NP = Lanes<LN>::NP;
+  static constexpr int kStates = 32 * kFwdChans * 16;                      // [channel][lane] float4
+  static constexpr int kRows = (3 * CHW + 2 * NP) * (int)sizeof(T);        // u, delta, gate, B, C of a token
+  static constexpr int kStage = kStates + (kRows + 15) / 16 * 16;
+  static constexpr int kWarp = (kAhead + 1) * kStage;
+};
+
+template <typename T, int LN>
 __global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const ScanParams p) {
+  extern __shared__ float4 smem4[];
+  constexpr int KD = kFwdChans;
+  using L = Lanes<LN, KD>;
+  using S = DecodeSmem<T, LN>;
+  constexpr int CHW = L::CHW, NP = L::NP;
+  constexpr int V = CHW < 4 ? CHW : 4;  // elements a copy
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = blockIdx.x * (blockDim.x >> 5) + warp;
   if (slice >= p.F * p.spg) return;
-  constexpr int KD = kFwdChans;
-  const Lanes<LN, KD> l(p, slice, lane);
+  const L l(p, slice, lane);
+  char* mine = reinterpret_cast<char*>(smem4) + warp * S::kWarp;
+  auto states = [&](int q) { return reinterpret_cast<float4*>(mine + q % (kAhead + 1) * S::kStage) + lane; };
+  auto rows = [&](int q) { return reinterpret_cast<T*>(mine + q % (kAhead + 1) * S::kStage + S::kStates); };
   // the channel whose step and output this lane computes
   const int cj = l.ch(sum_channel<KD>(lane));
-  const bool mine = l.nq < KD && cj < l.nch;
+  const bool own = l.nq < KD && cj < l.nch;
   const int c = l.c0 + cj;
-  const T* ug = reinterpret_cast<const T*>(p.u);
-  const T* dg = reinterpret_cast<const T*>(p.delta);
-  const T* zg = reinterpret_cast<const T*>(p.gate);
-  const T* bg = reinterpret_cast<const T*>(p.B) + (long long)l.f * p.N + l.n0();
-  const T* cg = reinterpret_cast<const T*>(p.C) + (long long)l.f * p.N + l.n0();
-  T* og = reinterpret_cast<T*>(p.out);
   pdl_wait();
   pdl_trigger();
+  const int r0 = blockIdx.y * p.L, count = min(p.L, p.q.nseq - r0);  // (L: requests per chunk, at most 32)
+  int mb = 0, me = 0, mslot = -1, minit = 0;
+  if (lane < count) {
+    mb = seq_start(p.q, r0 + lane);
+    me = seq_start(p.q, r0 + lane + 1);
+    if (p.state != nullptr) {
+      const int raw = p.slots[r0 + lane];
+      minit = p.initial[r0 + lane];
+      if (mb < me && raw >= p.num_slots && p.err != nullptr && slice == 0) atomicOr(p.err, 1);
+      mslot = mb < me && raw >= 0 && raw < p.num_slots ? raw : -1;
+    }
+  }
   LaneStates<KD> A2;
   load_rates(p, l, A2);
-  const float bias = p.dbias != nullptr && mine ? p.dbias[c] : 0.f;
-  const float skip = p.skip != nullptr && mine ? p.skip[c] : 0.f;
-  LaneStates<KD> h[RQ];
-  int tb[RQ], te[RQ], slot[RQ];
-  struct Row {
-    T u, d, z;
-    Pack<T, 4> b, c;
-  } row[RQ];
-  auto load_row = [&](int t, Row& r) {
-    if (mine) {
-      r.u = ug[t * p.ldu + c];
-      r.d = dg[t * p.ldd + c];
-      if (zg != nullptr) r.z = zg[t * p.ldg + c];
+  const float bias = p.dbias != nullptr && own ? p.dbias[c] : 0.f;
+  const float skip = p.skip != nullptr && own ? p.skip[c] : 0.f;
+
+  // token t's rows: u, delta, gate of the channels, B and C of the states
+  auto copy_rows = [&](int q, int t) {
+    constexpr int ROW = CHW / V, ALL = 3 * ROW + 2 * LN;
+    T* s = rows(q);
+#pragma unroll
+    for (int i0 = 0; i0 < ALL; i0 += 32) {
+      const int i = i0 + lane;
+      if (i < 3 * ROW) {
+        const int op = i / ROW, at = i % ROW * V, n = l.nch - at;
+        const T* g = reinterpret_cast<const T*>(op == 0 ? p.u : op == 1 ? p.delta : p.gate);
+        const long long ld = op == 0 ? p.ldu : op == 1 ? p.ldd : p.ldg;
+        if (g != nullptr) copy_part<T, V>(s + op * CHW + at, g + t * ld + l.c0 + at, g, n, p.vec && n >= V);
+      } else if (i < ALL) {
+        const int k = i - 3 * ROW, op = k / LN, at = k % LN * 4;
+        const T* g = reinterpret_cast<const T*>(op == 0 ? p.B : p.C);
+        copy_part<T, 4>(s + 3 * CHW + op * NP + at, g + t * (op == 0 ? p.ldb : p.ldc) + (long long)l.f * p.N + at, g,
+                        p.N - at, p.vec_bc);
+      }
     }
-    const bool v = p.vec_bc && l.n0() < p.N;
-    r.b = load_part<T, 4>(bg + t * p.ldb, p.N - l.n0(), v);
-    r.c = load_part<T, 4>(cg + t * p.ldc, p.N - l.n0(), v);
+  };
+  auto issue = [&](int q) {
+    if (q < count) {
+      const int b = __shfl_sync(0xffffffffu, mb, q), e = __shfl_sync(0xffffffffu, me, q);
+      const int slot = __shfl_sync(0xffffffffu, mslot, q), initial = __shfl_sync(0xffffffffu, minit, q);
+      if (b < e) {
+        copy_rows(q, b);
+        const bool from = slot >= 0 && initial != 0;
+        if (p.st_vec || !from) {
+          const float* s = p.state + (from ? slot * p.s_slot : 0);
+#pragma unroll
+          for (int j = 0; j < KD; ++j) {
+            const bool ok = from && l.ch(j) < l.nch && l.n0() < p.N;
+            copy_async<16>(states(q) + j * 32, ok ? s + (l.c0 + l.ch(j)) * p.s_d + l.n0() : p.A, ok);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < KD; ++j)
+            states(q)[j * 32] = load_four(p.state + slot * p.s_slot + (l.c0 + l.ch(j)) * p.s_d + l.n0() * p.s_n, p.s_n,
+                                          l.ch(j) < l.nch ? p.N - l.n0() : 0, false);
+        }
+      }
+    }
+    copy_commit();
   };
 #pragma unroll
-  for (int q = 0; q < RQ; ++q) {
-    const int r = blockIdx.y * RQ + q;
-    const bool ok = r < p.q.nseq;
-    tb[q] = ok ? seq_start(p.q, r) : 0;
-    te[q] = ok ? seq_start(p.q, r + 1) : 0;
-    slot[q] = tb[q] < te[q] ? slot_of(p, r, slice == 0 && lane == 0) : -1;
-    zero_states<KD>(h[q]);
-    if (slot[q] >= 0 && p.initial[r] != 0) load_slot(p, slot[q], l, h[q]);
-    if (tb[q] < te[q]) load_row(tb[q], row[q]);
-  }
+  for (int q = 0; q < kAhead; ++q) issue(q);
+#pragma unroll 1
+  for (int q = 0; q < count; ++q) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    __syncwarp();
+    issue(q + kAhead);
+    const int b = __shfl_sync(0xffffffffu, mb, q), e = __shfl_sync(0xffffffffu, me, q);
+    const int slot = __shfl_sync(0xffffffffu, mslot, q);
+    if (b >= e) continue;
+    LaneStates<KD> h;
 #pragma unroll
-  for (int q = 0; q < RQ; ++q) {
-    for (int t = tb[q]; t < te[q]; ++t) {
-      if (t > tb[q]) load_row(t, row[q]);
-      const float u = mine ? to_f(row[q].u) : 0.f;
+    for (int j = 0; j < KD; j += 2) pack_pair(states(q)[j * 32], states(q)[(j + 1) * 32], h[j / 2]);
+    for (int t = b; t < e; ++t) {
+      if (t > b) {
+        __syncwarp();
+        copy_rows(q, t);
+        copy_commit();
+        copy_wait();
+        __syncwarp();
+      }
+      const T* s = rows(q);
+      const float u = own ? to_f(s[cj]) : 0.f;
       float dt = 0.f, other;
-      if (mine) unpack2(step_sizes(p, to_f(row[q].d) + bias, 0.f), dt, other);
+      if (own) unpack2(step_sizes(p, to_f(s[CHW + cj]) + bias, 0.f), dt, other);
       ulonglong2 d[KD / 2];
 #pragma unroll
       for (int j = 0; j < KD / 2; ++j) {
-        float s[2], x[2];
+        float x[2], y[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // that channel's lane: sum_channel is its own inverse
           const int src = l.dg * LN + sum_channel<KD>(2 * j + i);
-          s[i] = __shfl_sync(0xffffffffu, dt, src);
-          x[i] = __shfl_sync(0xffffffffu, dt * u, src);
+          x[i] = __shfl_sync(0xffffffffu, dt, src);
+          y[i] = __shfl_sync(0xffffffffu, dt * u, src);
         }
-        d[j].x = pack2(s[0], s[1]);
-        d[j].y = pack2(x[0], x[1]);
+        d[j].x = pack2(x[0], x[1]);
+        d[j].y = pack2(y[0], y[1]);
       }
       f2 b2[4], c2[4], y[KD / 2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        b2[i] = pack2(to_f(row[q].b.v[i]), to_f(row[q].b.v[i]));
-        c2[i] = pack2(to_f(row[q].c.v[i]), to_f(row[q].c.v[i]));
-      }
-      scan_step<true, KD>(h[q], A2, d, b2, c2, y);
+      read_four(s + 3 * CHW + l.n0(), b2);
+      read_four(s + 3 * CHW + NP + l.n0(), c2);
+      scan_step<true, KD>(h, A2, d, b2, c2, y);
       float o = sum_over_states<LN>(y, lane);
-      if (mine) {
+      if (own) {
         o = fmaf(skip, u, o);
-        if (zg != nullptr) o *= to_f(row[q].z) * sigmoid_t<T>(to_f(row[q].z));
-        og[(long long)t * p.D + c] = from_f<T>(o);
+        if (p.gate != nullptr) o *= to_f(s[2 * CHW + cj]) * sigmoid_t<T>(to_f(s[2 * CHW + cj]));
+        reinterpret_cast<T*>(p.out)[(long long)t * p.D + c] = from_f<T>(o);
       }
     }
-    if (slot[q] >= 0) store_slot(p, slot[q], l, h[q]);
+    if (slot >= 0) store_slot(p, slot, l, h);
   }
-  if (p.zero_rest && mine) {
+  if (p.zero_rest && own) {
+    T* og = reinterpret_cast<T*>(p.out) + c;
     const T z = from_f<T>(0.f);
     if (blockIdx.y == 0)
-      for (int t = 0; t < seq_start(p.q, 0); ++t) og[(long long)t * p.D + c] = z;
+      for (int t = 0; t < seq_start(p.q, 0); ++t) og[(long long)t * p.D] = z;
     if (blockIdx.y == gridDim.y - 1)
-      for (int t = seq_start(p.q, p.q.nseq); t < p.q.T; ++t) og[(long long)t * p.D + c] = z;
+      for (int t = seq_start(p.q, p.q.nseq); t < p.q.T; ++t) og[(long long)t * p.D] = z;
   }
 }
 

@@ -4,6 +4,6 @@
 namespace greta {
 namespace ssm {
 cudaError_t scan_fwd_bf16(const ScanParams& p, cudaStream_t st) { return scan_fwd<__nv_bfloat16>(p, st); }
-cudaError_t scan_decode_bf16(const ScanParams& p, int rq, cudaStream_t st) { return scan_decode<__nv_bfloat16>(p, rq, st); }
+cudaError_t scan_decode_bf16(const ScanParams& p, cudaStream_t st) { return scan_decode<__nv_bfloat16>(p, st); }
 }  // namespace ssm
 }  // namespace greta

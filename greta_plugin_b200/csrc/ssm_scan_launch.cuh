@@ -55,12 +55,15 @@ cudaError_t scan_fwd(const ScanParams& p, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t scan_decode(const ScanParams& p, int rq, cudaStream_t st) {
+cudaError_t scan_decode(const ScanParams& p, cudaStream_t st) {
   return with_lanes(p.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    const dim3 grid = slices_grid(p, (int)cdiv(p.q.nseq, rq)), block(kScanWarps * 32);
-    return rq == 1 ? launch(ssm_scan_decode_kernel<T, LN, 1>, grid, block, 0, st, p)
-                   : launch(ssm_scan_decode_kernel<T, LN, 2>, grid, block, 0, st, p);
+    const dim3 grid = slices_grid(p, (int)cdiv(p.q.nseq, p.L)), block(kScanWarps * 32);
+    const size_t smem = (size_t)kScanWarps * DecodeSmem<T, LN>::kWarp;
+    auto k = ssm_scan_decode_kernel<T, LN>;
+    cudaError_t e = allow_smem(k, smem);
+    if (e != cudaSuccess) return e;
+    return launch(k, grid, block, smem, st, p);
   });
 }
 
@@ -73,9 +76,9 @@ struct ScanGrads {
 cudaError_t scan_fwd_f32(const ScanParams&, cudaStream_t);
 cudaError_t scan_fwd_f16(const ScanParams&, cudaStream_t);
 cudaError_t scan_fwd_bf16(const ScanParams&, cudaStream_t);
-cudaError_t scan_decode_f32(const ScanParams&, int, cudaStream_t);
-cudaError_t scan_decode_f16(const ScanParams&, int, cudaStream_t);
-cudaError_t scan_decode_bf16(const ScanParams&, int, cudaStream_t);
+cudaError_t scan_decode_f32(const ScanParams&, cudaStream_t);
+cudaError_t scan_decode_f16(const ScanParams&, cudaStream_t);
+cudaError_t scan_decode_bf16(const ScanParams&, cudaStream_t);
 cudaError_t scan_bwd_f32(const ScanParams&, const ScanGrads&, cudaStream_t);
 cudaError_t scan_bwd_f16(const ScanParams&, const ScanGrads&, cudaStream_t);
 cudaError_t scan_bwd_bf16(const ScanParams&, const ScanGrads&, cudaStream_t);

@@ -198,6 +198,15 @@ def test_packed_decode(n, D):
     check_packed([1] * n, [int(s) for s in slots], [1] * n, D, 4, torch.bfloat16)
 
 
+def test_packed_decode_uneven():
+    """Batches of about a token per request, some of none and of several, rows
+    behind the last."""
+    for kw in (dict(tail=4), dict(tail=2, given_out=False), dict(tail=0)):
+        check_packed([1, 0, 4, 1, 0, 1], [0, 1, 2, 3, 4, 5], [1, 1, 1, 0, 1, 1], 64, 4, torch.bfloat16, **kw)
+    check_packed([0, 9], [0, 1], [1, 1], 65, 3, torch.float32)
+    check_packed([3, 1, 1], [2, 0, -1], [1, 1, 1], 64, 7, torch.float16, layout="SD")
+
+
 @pytest.mark.parametrize("extra", [0, 1, 2, 3, 5])
 def test_packed_borders_of_runs(extra):
     """Sequence starts at every offset from where one run of tokens ends and the
