@@ -128,7 +128,7 @@ def lib() -> ctypes.CDLL:
     for name, args in ssm.items():
         getattr(L, f"greta_ssm_{name}").argtypes = args
         getattr(L, f"greta_ssm_{name}").restype = I32
-    sizes = {"conv_bwd_workspace": [I64] * 3, "scan_workspace": [I64] * 5 + [I32],
+    sizes = {"conv_bwd_workspace": [I64] * 3, "scan_workspace": [I32] + [I64] * 5 + [I32],
              "scan_bwd_workspace": [I64] * 5 + [I32]}
     for name, args in sizes.items():
         getattr(L, f"greta_ssm_{name}").argtypes = args
@@ -157,6 +157,27 @@ def ptr(t):
 
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def addr(t):
+    """A tensor's address as the integer that a pointer argument takes."""
+    return None if t is None else t.data_ptr()
+
+
+def call(name: str, t: torch.Tensor, *args) -> None:
+    """The C-ABI function `name` with `args` and the current stream of t's device
+    as its last one, under that device; raises for a status other than OK.
+    (The device is switched only where it has to be: the switch costs as much
+    as the call.)"""
+    fn = getattr(lib(), name)
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st != OK:
+        check(name, st)
 
 
 def check(fn: str, status: int) -> None:

@@ -16,6 +16,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _capi
+from .causal_conv import same_device
 
 MAX_REQUESTS = 16384
 
@@ -70,31 +71,30 @@ def packed_batch_metadata(query_lens: torch.Tensor, context_lens: torch.Tensor, 
             raise ValueError("block_tables need free_blocks, a 1-d int32 tensor")
     elif free_blocks is not None:
         raise ValueError("free_blocks without block_tables")
+    same_device("query_lens", query_lens, context_lens=context_lens, block_tables=block_tables,
+                free_blocks=free_blocks)
     dev = query_lens.device
-    for name, t in (("context_lens", context_lens), ("block_tables", block_tables), ("free_blocks", free_blocks)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, query_lens on {dev}")
     if not query_lens.is_cuda:
         raise ValueError("packed_batch_metadata requires CUDA tensors")
     query_lens, context_lens = query_lens.contiguous(), context_lens.contiguous()
     free_blocks = None if free_blocks is None else free_blocks.contiguous()
     i32, i64 = torch.int32, torch.int64
-    starts = torch.empty(N + 1, dtype=i32, device=dev)
+    # int32 and int64 results share a buffer each (an allocation costs as much as
+    # the kernel's launch)
+    i32, i64 = torch.int32, torch.int64
+    starts, seq_idx, used = torch.empty(N + T + 2, dtype=i32, device=dev).split((N + 1, T, 1))
     init = torch.empty(N, dtype=torch.int8, device=dev)
-    seq_idx = torch.empty(T, dtype=i32, device=dev)
-    positions = torch.empty(T, dtype=i64, device=dev)
-    slot_map = torch.empty(T, dtype=i64, device=dev) if paged else None
-    used = torch.empty(1, dtype=i32, device=dev) if paged else None
-    p = _capi.ptr
-    width = block_tables.shape[1] if paged else 0
+    if paged:
+        positions, slot_map = torch.empty(2, T, dtype=i64, device=dev).unbind()
+    else:
+        positions, slot_map, used = torch.empty(T, dtype=i64, device=dev), None, None
+    p = _capi.addr
     # a table without entries has no address of its own
-    table = block_tables if not paged or block_tables.numel() else used
-    with torch.cuda.device(dev.index):
-        st = _capi.lib().greta_ssm_batch_metadata(
-            p(query_lens), p(context_lens), N, T, p(starts), p(init), p(seq_idx), p(positions), p(table),
-            max(block_tables.stride(0), width) if paged else 0, width, block_size if paged else 0, p(free_blocks),
-            free_blocks.numel() if paged else 0, p(slot_map), p(used), _capi.stream_of(query_lens))
-    _capi.check("greta_ssm_batch_metadata", st)
+    width = block_tables.shape[1] if paged else 0
+    table = (p(block_tables) or p(used)) if paged else None
+    _capi.call("greta_ssm_batch_metadata", query_lens, p(query_lens), p(context_lens), N, T, p(starts), p(init),
+               p(seq_idx), p(positions), table, max(block_tables.stride(0), width) if paged else 0, width,
+               block_size if paged else 0, p(free_blocks), free_blocks.numel() if paged else 0, p(slot_map), p(used))
     return PackedBatch(starts, init, seq_idx, positions, slot_map, used)
 
 

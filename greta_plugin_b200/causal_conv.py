@@ -40,8 +40,9 @@ def channel_rows(t):
     contiguous and rows do not overlap, else made contiguous. Rows that start
     on whole vectors take the vector path; others are read by element."""
     T, D = t.shape
-    if (t.stride(1) == 1 or D == 1) and (t.stride(0) >= D or T == 1):
-        return t, max(t.stride(0), D)
+    row, col = t.stride()
+    if (col == 1 or D == 1) and (row >= D or T == 1):
+        return t, max(row, D)
     return t.contiguous(), D
 
 
@@ -49,18 +50,28 @@ def _check_weight(x, weight, bias):
     D = x.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != D:
         raise ValueError(f"weight must be [W, {D}] (taps, channels), got {tuple(weight.shape)}")
-    if not 1 <= weight.shape[0] <= MAX_WIDTH:
-        raise ValueError(f"kernel size must be between 1 and {MAX_WIDTH}, got {weight.shape[0]}")
-    if bias is not None and tuple(bias.shape) != (D,):
+    W = weight.shape[0]
+    if not 1 <= W <= MAX_WIDTH:
+        raise ValueError(f"kernel size must be between 1 and {MAX_WIDTH}, got {W}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != D):
         raise ValueError(f"bias must be [{D}], got {tuple(bias.shape)}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    return weight.shape[0]
+    same_device("x", x, weight=weight, bias=bias)
+    return W
+
+
+def same_device(name, t, **others):
+    dev = t.get_device()
+    for k, o in others.items():
+        if o is not None and o.get_device() != dev:
+            raise ValueError(f"{k} is on {o.device}, {name} on {t.device}")
 
 
 def _as_type(t, dtype):
     return t if t is None or t.dtype == dtype else t.to(dtype)
+
+
+def _bias(bias, dtype):
+    return None if bias is None else _as_type(bias, dtype).contiguous()
 
 
 class CausalConv1dFunction(torch.autograd.Function):
@@ -69,16 +80,13 @@ class CausalConv1dFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, cu_seqlens, silu):
         x, ldx = channel_rows(x)
-        w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
-        b = None if b is None else b.contiguous()
         T, D = x.shape
+        w, b = _as_type(weight, x.dtype), _bias(bias, x.dtype)
         y = torch.empty(T, D, dtype=x.dtype, device=x.device)
         cu, cu64, nseq = _cu(cu_seqlens, x.device)
-        with torch.cuda.device(x.device.index):
-            st = _capi.lib().greta_ssm_conv_fwd(
-                _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
-                _capi.ptr(y), _capi.ptr(cu), cu64, nseq, T, D, w.shape[0], silu, _capi.stream_of(x))
-        _capi.check("greta_ssm_conv_fwd", st)
+        p = _capi.addr
+        _capi.call("greta_ssm_conv_fwd", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(y), p(cu), cu64,
+                   nseq, T, D, w.shape[0], silu)
         ctx.save_for_backward(x, weight, bias, cu)
         ctx.silu = silu
         return y
@@ -88,25 +96,19 @@ class CausalConv1dFunction(torch.autograd.Function):
     def backward(ctx, dout):
         x, weight, bias, cu = ctx.saved_tensors
         x, ldx = channel_rows(x)
-        w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
-        b = None if b is None else b.contiguous()
-        T, D = x.shape
-        W = w.shape[0]
-        dout = _as_type(dout, x.dtype).contiguous()
-        dev = x.device
-        dx = torch.empty(T, D, dtype=x.dtype, device=dev)
-        dw = torch.empty(W, D, dtype=x.dtype, device=dev)
-        db = None if b is None else torch.empty(D, dtype=x.dtype, device=dev)
-        L = _capi.lib()
-        ws = torch.empty(L.greta_ssm_conv_bwd_workspace(T, D, W), dtype=torch.uint8, device=dev)
+        dt, dev = x.dtype, x.device
+        w, b = _as_type(weight, dt), _bias(bias, dt)
+        (T, D), W = x.shape, w.shape[0]
+        dout = _as_type(dout, dt).contiguous()
+        dx = torch.empty(T, D, dtype=dt, device=dev)
+        dw = torch.empty(W, D, dtype=dt, device=dev)
+        db = None if b is None else torch.empty(D, dtype=dt, device=dev)
+        ws = torch.empty(_capi.lib().greta_ssm_conv_bwd_workspace(T, D, W), dtype=torch.uint8, device=dev)
         cu, cu64, nseq = _cu(cu, dev)
-        with torch.cuda.device(dev.index):
-            st = L.greta_ssm_conv_bwd(
-                _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
-                _capi.ptr(dout), _capi.ptr(dx), _capi.ptr(dw), _capi.ptr(db), _capi.ptr(cu), cu64, nseq, T, D, W,
-                ctx.silu, _capi.ptr(ws), ws.numel(), _capi.stream_of(x))
-        _capi.check("greta_ssm_conv_bwd", st)
-        return dx, _as_type(dw, weight.dtype), None if bias is None else _as_type(db, bias.dtype), None, None
+        p = _capi.addr
+        _capi.call("greta_ssm_conv_bwd", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(dout), p(dx),
+                   p(dw), p(db), p(cu), cu64, nseq, T, D, W, ctx.silu, p(ws), ws.numel())
+        return dx, _as_type(dw, weight.dtype), None if b is None else _as_type(db, bias.dtype), None, None
 
 
 @torch.compiler.disable(recursive=True)
@@ -133,6 +135,12 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     return CausalConv1dFunction.apply(x.squeeze(0), weight, bias, cu_seqlens, silu).unsqueeze(0)
 
 
+def _as_meta(t, x, dtype):
+    if t.dtype is dtype and t.get_device() == x.get_device() and t.dim() == 1 and t.is_contiguous():
+        return t
+    return t.to(device=x.device, dtype=dtype).reshape(-1).contiguous()
+
+
 def packed_metadata(x, state, starts, slots, has_initial):
     """The request tensors on x's device in the kernels' types, checked against
     one another."""
@@ -140,11 +148,9 @@ def packed_metadata(x, state, starts, slots, has_initial):
     if starts.numel() != n + 1 or has_initial.numel() != n:
         raise ValueError(f"starts must hold one offset more than slots ({n}) and has_initial as many, got "
                          f"{starts.numel()} and {has_initial.numel()}")
-    if state.device != x.device:
-        raise ValueError(f"state is on {state.device}, x on {x.device}")
-    return (starts.to(device=x.device, dtype=torch.int32).contiguous(),
-            slots.to(device=x.device, dtype=torch.int32).reshape(-1).contiguous(),
-            has_initial.to(device=x.device, dtype=torch.int8).reshape(-1).contiguous())
+    same_device("x", x, state=state)
+    return (_as_meta(starts, x, torch.int32), _as_meta(slots, x, torch.int32),
+            _as_meta(has_initial, x, torch.int8))
 
 
 def packed_out(x, out):
@@ -153,7 +159,7 @@ def packed_out(x, out):
     writes zeros to them."""
     if out is None:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device), 1
-    if out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous() or out.device != x.device:
+    if out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous() or out.get_device() != x.get_device():
         raise ValueError("out must be a contiguous tensor shaped and typed like the input, on its device")
     return out, 0
 
@@ -163,11 +169,15 @@ def check_disjoint(out, **inputs):
     a0 = out.data_ptr()
     a1 = a0 + out.numel() * out.element_size()
     for name, t in inputs.items():
-        if t is None or t.numel() == 0 or a0 == a1:
+        if t is None:
             continue
-        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
         b0 = t.data_ptr()
-        if a0 < b0 + span * t.element_size() and b0 < a1:
+        if b0 >= a1 or t.numel() == 0 or a0 == a1:
+            continue
+        span = 1
+        for n, s in zip(t.shape, t.stride()):
+            span += (n - 1) * s
+        if a0 < b0 + span * t.element_size():
             raise ValueError(f"out must not overlap {name}")
 
 
@@ -177,7 +187,7 @@ def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out,
     T, D = x.shape
     W = _check_weight(x, weight, bias)
     silu = _activation(activation)
-    if state.dim() != 3 or tuple(state.shape[1:]) != (D, W - 1):
+    if state.dim() != 3 or state.shape[1] != D or state.shape[2] != W - 1:
         raise ValueError(f"state must be [slots, {D}, {W - 1}], got {tuple(state.shape)}")
     if state.dtype != x.dtype:
         raise ValueError(f"state dtype {state.dtype} must match x dtype {x.dtype}")
@@ -188,18 +198,14 @@ def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out,
     out, new = packed_out(x, out)
     if T == 0:
         return out
-    check_disjoint(out, x=x, state=state)
+    if not new:
+        check_disjoint(out, x=x, state=state)
     x, ldx = channel_rows(x)
-    w, b = _as_type(weight, x.dtype), _as_type(bias, x.dtype)
-    b = None if b is None else b.contiguous()
-    s_slot, s_d, s_h = state.stride()
-    with torch.cuda.device(x.device.index):
-        st = _capi.lib().greta_ssm_conv_packed(
-            _capi.dtype_code(x), _capi.ptr(x), ldx, _capi.ptr(w), w.stride(0), w.stride(1), _capi.ptr(b),
-            _capi.ptr(out), _capi.ptr(state) if state.numel() else None, state.shape[0], s_slot, s_d, s_h,
-            _capi.ptr(starts), _capi.ptr(slots), _capi.ptr(has_initial), slots.numel(), T, D, W, silu,
-            new, _capi.ptr(flags), _capi.stream_of(x))
-    _capi.check("greta_ssm_conv_packed", st)
+    w, b = _as_type(weight, x.dtype), _bias(bias, x.dtype)
+    p = _capi.addr
+    _capi.call("greta_ssm_conv_packed", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(out),
+               p(state) or None, state.shape[0], *state.stride(), p(starts), p(slots), p(has_initial), slots.numel(),
+               T, D, W, silu, new, p(flags))
     return out
 
 

@@ -644,7 +644,7 @@ struct DecodeSmem {
 };
 
 template <typename T, int LN>
-__global__ void __launch_bounds__(kScanWarps * 32) ssm_scan_decode_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_decode_kernel(const ScanParams p) {
   extern __shared__ float4 smem4[];
   constexpr int KD = kFwdChans;
   using L = Lanes<LN, KD>;

@@ -23,12 +23,13 @@ There is no CPU fallback: non-CUDA tensors raise ValueError.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
 from . import _capi
-from .causal_conv import channel_rows, check_disjoint, packed_metadata, packed_out
+from .causal_conv import channel_rows, check_disjoint, packed_metadata, packed_out, same_device
 from .dynamic_conv import _cu
 
 MAX_STATES = 128
@@ -37,40 +38,43 @@ SAVE_EVERY = 8  # tokens per saved state
 
 def _check(u, delta, A, B, C, skip, gate, delta_bias):
     """Shapes, types and devices of the operands ([T, D] rows); (T, D, N, F)."""
-    T, D = u.shape
+    rows = u.shape
+    T, D = rows
+    dt = u.dtype
     _capi.dtype_code(u)
-    if tuple(delta.shape) != (T, D):
+    if delta.shape != rows:
         raise ValueError(f"delta shape {tuple(delta.shape)} must match u's {(T, D)}")
-    if gate is not None and tuple(gate.shape) != (T, D):
+    if gate is not None and gate.shape != rows:
         raise ValueError(f"gate shape {tuple(gate.shape)} must match u's {(T, D)}")
     if A.dim() != 2 or A.shape[0] != D:
         raise ValueError(f"A must be [{D}, N], got {tuple(A.shape)}")
     N = A.shape[1]
     if not 1 <= N <= MAX_STATES:
         raise ValueError(f"the number of states must be between 1 and {MAX_STATES}, got {N}")
-    if B.dim() != 3 or B.shape[0] != T or B.shape[2] != N or B.shape[1] < 1 or D % B.shape[1] != 0:
-        raise ValueError(f"B must be [{T}, F, {N}] with F dividing {D}, got {tuple(B.shape)}")
-    if tuple(C.shape) != tuple(B.shape):
-        raise ValueError(f"C shape {tuple(C.shape)} must match B's {tuple(B.shape)}")
-    for name, t in (("skip", skip), ("delta_bias", delta_bias)):
-        if t is not None and tuple(t.shape) != (D,):
-            raise ValueError(f"{name} must be [{D}], got {tuple(t.shape)}")
-    for name, t in (("delta", delta), ("gate", gate), ("B", B), ("C", C)):
-        if t is not None and t.dtype != u.dtype:
-            raise ValueError(f"{name} dtype {t.dtype} must match u dtype {u.dtype}")
-    for name, t in (("delta", delta), ("A", A), ("B", B), ("C", C), ("skip", skip), ("gate", gate),
-                    ("delta_bias", delta_bias)):
-        if t is not None and t.device != u.device:
-            raise ValueError(f"{name} is on {t.device}, u on {u.device}")
-    return T, D, N, B.shape[1]
+    groups = B.shape
+    if len(groups) != 3 or groups[0] != T or groups[2] != N or groups[1] < 1 or D % groups[1] != 0:
+        raise ValueError(f"B must be [{T}, F, {N}] with F dividing {D}, got {tuple(groups)}")
+    if C.shape != groups:
+        raise ValueError(f"C shape {tuple(C.shape)} must match B's {tuple(groups)}")
+    if skip is not None and (skip.dim() != 1 or skip.shape[0] != D):
+        raise ValueError(f"skip must be [{D}], got {tuple(skip.shape)}")
+    if delta_bias is not None and (delta_bias.dim() != 1 or delta_bias.shape[0] != D):
+        raise ValueError(f"delta_bias must be [{D}], got {tuple(delta_bias.shape)}")
+    if delta.dtype != dt or B.dtype != dt or C.dtype != dt or (gate is not None and gate.dtype != dt):
+        for name, t in (("delta", delta), ("gate", gate), ("B", B), ("C", C)):
+            if t is not None and t.dtype != dt:
+                raise ValueError(f"{name} dtype {t.dtype} must match u dtype {dt}")
+    same_device("u", u, delta=delta, A=A, B=B, C=C, skip=skip, gate=gate, delta_bias=delta_bias)
+    return T, D, N, groups[1]
 
 
 def _group_rows(t):
     """B or C [T, F, N] as (tensor, token-row stride): read in place when each
     token's F x N block is contiguous."""
     T, F, N = t.shape
-    if (t.stride(2) == 1 or N == 1) and (t.stride(1) == N or F == 1) and (t.stride(0) >= F * N or T == 1):
-        return t, max(t.stride(0), F * N)
+    row, group, state = t.stride()
+    if (state == 1 or N == 1) and (group == N or F == 1) and (row >= F * N or T == 1):
+        return t, max(row, F * N)
     return t.contiguous(), F * N
 
 
@@ -78,42 +82,50 @@ def _fp32(t):
     """fp32, contiguous and on a 16-byte boundary, as the kernels read it."""
     if t is None:
         return None
-    t = (t if t.dtype == torch.float32 else t.float()).contiguous()
+    if t.dtype is not torch.float32 or not t.is_contiguous():
+        t = t.float().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-class _Operands:
-    """The operands of a call as the kernels take them: tensors (kept alive)
-    and the leading arguments of the C calls."""
-
-    def __init__(self, u, delta, A, B, C, skip, gate, delta_bias):
-        self.u, ldu = channel_rows(u)
-        self.delta, ldd = channel_rows(delta)
-        self.gate, ldg = (None, 0) if gate is None else channel_rows(gate)
-        self.B, ldb = _group_rows(B)
-        self.C, ldc = _group_rows(C)
-        self.A, self.skip, self.delta_bias = _fp32(A), _fp32(skip), _fp32(delta_bias)
-        p = _capi.ptr
-        self.args = (_capi.dtype_code(u), p(self.u), ldu, p(self.delta), ldd, p(self.gate), ldg, p(self.B), ldb,
-                     p(self.C), ldc, p(self.A), p(self.skip), p(self.delta_bias))
+def _operands(u, delta, A, B, C, skip, gate, delta_bias):
+    """(tensors to keep alive, the leading arguments of the C calls)."""
+    u, ldu = channel_rows(u)
+    delta, ldd = channel_rows(delta)
+    gate, ldg = (None, 0) if gate is None else channel_rows(gate)
+    B, ldb = _group_rows(B)
+    C, ldc = _group_rows(C)
+    A, skip, delta_bias = _fp32(A), _fp32(skip), _fp32(delta_bias)
+    p = _capi.addr
+    return (u, delta, gate, B, C, A, skip, delta_bias), (
+        _capi.dtype_code(u), p(u), ldu, p(delta), ldd, p(gate), ldg, p(B), ldb, p(C), ldc, p(A), p(skip),
+        p(delta_bias))
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _scan_forward(ops, T, D, N, F, cu_seqlens, softplus, saved):
-    u = ops.u
-    out = torch.empty(T, D, dtype=u.dtype, device=u.device)
-    cu, cu64, nseq = _cu(cu_seqlens, u.device)
-    ranges = _capi.token_ranges()
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(kind, device, nseq, T, D, N, F, ranges):
+    """Bytes of workspace of a call on `device` (the sizes decide it alone)."""
     L = _capi.lib()
-    with torch.cuda.device(u.device.index):
-        ws = _workspace(L.greta_ssm_scan_workspace(nseq, T, D, N, F, ranges), u.device)
-        st = L.greta_ssm_scan_fwd(*ops.args, _capi.ptr(out), _capi.ptr(saved), _capi.ptr(cu), cu64, nseq, T, D, N, F,
-                                  int(softplus), ranges, _capi.ptr(ws), 0 if ws is None else ws.numel(),
-                                  _capi.stream_of(u))
-    _capi.check("greta_ssm_scan_fwd", st)
+    with torch.cuda.device(device):
+        if kind == "bwd":
+            return L.greta_ssm_scan_bwd_workspace(nseq, T, D, N, F, ranges)
+        return L.greta_ssm_scan_workspace(int(kind == "packed"), nseq, T, D, N, F, ranges)
+
+
+def _workspace(kind, device, *sizes):
+    """(workspace or None, its bytes)"""
+    n = _workspace_bytes(kind, device.index, *sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+
+
+def _scan_forward(u, args, T, D, N, F, cu_seqlens, softplus, saved):
+    dev = u.device
+    out = torch.empty(T, D, dtype=u.dtype, device=dev)
+    cu, cu64, nseq = _cu(cu_seqlens, dev)
+    ranges = _capi.token_ranges()
+    ws, n = _workspace("fwd", dev, nseq, T, D, N, F, ranges)
+    p = _capi.addr
+    _capi.call("greta_ssm_scan_fwd", u, *args, p(out), p(saved), p(cu), cu64, nseq, T, D, N, F, int(softplus), ranges,
+               p(ws), n)
     return out
 
 
@@ -123,12 +135,12 @@ class SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, softplus):
         (T, D), (_, F, N) = u.shape, B.shape
-        ops = _Operands(u, delta, A, B, C, skip, gate, delta_bias)
+        keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
         saved = None
         if any(ctx.needs_input_grad):
             saved = torch.empty(T // SAVE_EVERY + 1, D, N, dtype=torch.float32, device=u.device)
         cu, _, _ = _cu(cu_seqlens, u.device)
-        out = _scan_forward(ops, T, D, N, F, cu, softplus, saved)
+        out = _scan_forward(u, args, T, D, N, F, cu, softplus, saved)
         ctx.save_for_backward(u, delta, A, B, C, skip, gate, delta_bias, cu, saved)
         ctx.softplus = softplus
         return out
@@ -138,9 +150,9 @@ class SelectiveScanFunction(torch.autograd.Function):
     def backward(ctx, dout):
         u, delta, A, B, C, skip, gate, delta_bias, cu, saved = ctx.saved_tensors
         (T, D), (_, F, N) = u.shape, B.shape
-        ops = _Operands(u, delta, A, B, C, skip, gate, delta_bias)
-        dout = (dout if dout.dtype == u.dtype else dout.to(u.dtype)).contiguous()
+        keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
         dev, dt, f32 = u.device, u.dtype, torch.float32
+        dout = (dout if dout.dtype == dt else dout.to(dt)).contiguous()
         du, ddelta = torch.empty(T, D, dtype=dt, device=dev), torch.empty(T, D, dtype=dt, device=dev)
         dgate = None if gate is None else torch.empty(T, D, dtype=dt, device=dev)
         dB, dC = torch.empty(T, F, N, dtype=dt, device=dev), torch.empty(T, F, N, dtype=dt, device=dev)
@@ -149,14 +161,10 @@ class SelectiveScanFunction(torch.autograd.Function):
         dbias = None if delta_bias is None else torch.empty(D, dtype=f32, device=dev)
         cu, cu64, nseq = _cu(cu, dev)
         ranges = _capi.token_ranges()
-        L, p = _capi.lib(), _capi.ptr
-        with torch.cuda.device(dev.index):
-            ws = _workspace(L.greta_ssm_scan_bwd_workspace(nseq, T, D, N, F, ranges), dev)
-            st = L.greta_ssm_scan_bwd(
-                *ops.args, p(saved), p(dout), p(du), p(ddelta), p(dgate), p(dB), p(dC), p(dA), p(dskip), p(dbias),
-                p(cu), cu64, nseq, T, D, N, F, int(ctx.softplus), ranges, p(ws), 0 if ws is None else ws.numel(),
-                _capi.stream_of(u))
-        _capi.check("greta_ssm_scan_bwd", st)
+        ws, n = _workspace("bwd", dev, nseq, T, D, N, F, ranges)
+        p = _capi.addr
+        _capi.call("greta_ssm_scan_bwd", u, *args, p(saved), p(dout), p(du), p(ddelta), p(dgate), p(dB), p(dC), p(dA),
+                   p(dskip), p(dbias), p(cu), cu64, nseq, T, D, N, F, int(ctx.softplus), ranges, p(ws), n)
         like = lambda g, t: g if g is None or g.dtype == t.dtype else g.to(t.dtype)  # noqa: E731
         return (du, ddelta, like(dA, A), dB, dC, like(dskip, skip), dgate, like(dbias, delta_bias), None, None)
 
@@ -196,7 +204,7 @@ def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has
     if u.dim() != 2:
         raise ValueError(f"u must be [T, D], got {tuple(u.shape)}")
     T, D, N, F = _check(u, delta, A, B, C, skip, gate, delta_bias)
-    if state.dim() != 3 or tuple(state.shape[1:]) != (D, N):
+    if state.dim() != 3 or state.shape[1] != D or state.shape[2] != N:
         raise ValueError(f"state must be [slots, {D}, {N}], got {tuple(state.shape)}")
     if state.dtype != torch.float32:
         raise ValueError(f"state must be float32, got {state.dtype}")
@@ -206,19 +214,14 @@ def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has
     out, new = packed_out(u, out)
     if T == 0:
         return out
-    check_disjoint(out, u=u, delta=delta, gate=gate, B=B, C=C, state=state)
-    ops = _Operands(u, delta, A, B, C, skip, gate, delta_bias)
-    s_slot, s_d, s_n = state.stride()
-    ranges = _capi.token_ranges()
-    n = slots.numel()
-    L = _capi.lib()
-    with torch.cuda.device(u.device.index):
-        ws = _workspace(L.greta_ssm_scan_workspace(n, T, D, N, F, ranges), u.device)
-        st = L.greta_ssm_scan_packed(
-            *ops.args, _capi.ptr(out), _capi.ptr(state) if state.numel() else None, state.shape[0], s_slot, s_d, s_n,
-            _capi.ptr(starts), _capi.ptr(slots), _capi.ptr(has_initial), n, T, D, N, F, int(delta_softplus), new,
-            ranges, _capi.ptr(flags), _capi.ptr(ws), 0 if ws is None else ws.numel(), _capi.stream_of(u))
-    _capi.check("greta_ssm_scan_packed", st)
+    if not new:
+        check_disjoint(out, u=u, delta=delta, gate=gate, B=B, C=C, state=state)
+    keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
+    ranges, n = _capi.token_ranges(), slots.numel()
+    ws, nbytes = _workspace("packed", u.device, n, T, D, N, F, ranges)
+    p = _capi.addr
+    _capi.call("greta_ssm_scan_packed", u, *args, p(out), p(state) or None, state.shape[0], *state.stride(), p(starts),
+               p(slots), p(has_initial), n, T, D, N, F, int(delta_softplus), new, ranges, p(flags), p(ws), nbytes)
     return out
 
 

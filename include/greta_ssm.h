@@ -126,8 +126,11 @@ GRETA_API int greta_ssm_scan_bwd(int dtype, const void* u, int64_t ldu, const vo
 GRETA_API int64_t greta_ssm_scan_bwd_workspace(int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F,
                                                int ranges);
 
-/* Bytes of workspace of greta_ssm_scan_fwd and greta_ssm_scan_packed (the same `ranges`). */
-GRETA_API int64_t greta_ssm_scan_workspace(int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F, int ranges);
+/* Bytes of workspace of greta_ssm_scan_fwd and greta_ssm_scan_packed (the same `ranges`;
+ * packed: 0 for greta_ssm_scan_fwd, 1 for greta_ssm_scan_packed, which needs
+ * none for a batch of single tokens). */
+GRETA_API int64_t greta_ssm_scan_workspace(int packed, int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F,
+                                           int ranges);
 
 /*
  * Metadata of a packed serving batch in one launch, from the lengths of the

@@ -170,7 +170,7 @@ def test_scan_rejects_bad_arguments(lib):
     assert fwd(A=P(0x1004)) == C.ERR_ALIGNMENT
     assert fwd(saved=P(0x1004)) == C.ERR_ALIGNMENT
     # several ranges need a workspace
-    need = lib.greta_ssm_scan_workspace(0, 64, 64, 16, 1, 3)
+    need = lib.greta_ssm_scan_workspace(0, 0, 64, 64, 16, 1, 3)
     assert need > 0
     assert fwd(T=64, ranges=3, ws=None) == C.ERR_INVALID_ARG
     assert fwd(T=64, ranges=3, nbytes=need - 1) == C.ERR_INVALID_ARG
@@ -223,9 +223,10 @@ def test_batch_metadata_rejects_bad_arguments(lib):
 
 
 def test_workspaces_follow_the_shapes(lib):
-    assert lib.greta_ssm_scan_workspace(0, 100, 64, 16, 1, 1) == 0  # one range carries nothing
-    assert lib.greta_ssm_scan_workspace(0, 0, 64, 16, 1, 4) == 0
-    two = lib.greta_ssm_scan_workspace(0, 100, 64, 16, 1, 2)
+    assert lib.greta_ssm_scan_workspace(0, 0, 100, 64, 16, 1, 1) == 0  # one range carries nothing
+    assert lib.greta_ssm_scan_workspace(0, 0, 0, 64, 16, 1, 4) == 0
+    assert lib.greta_ssm_scan_workspace(1, 64, 70, 64, 16, 1, 0) == 0  # single tokens
+    two = lib.greta_ssm_scan_workspace(0, 0, 100, 64, 16, 1, 2)
     assert two >= 2 * (2 * 64 * 16 + 64) * 4
     assert lib.greta_ssm_scan_bwd_workspace(0, 100, 64, 16, 1, 1) >= 100 * 2 * 16 * 4 + 64 * 18 * 4
     assert lib.greta_ssm_conv_bwd_workspace(1, 64, 4) == 5 * 64 * 4
