@@ -92,11 +92,30 @@ struct SeqView {
   }
 };
 
-// Where range i of L tokens begins. (Borders moved to sequence starts close by
-// save some carries, but ranges of uneven length cost more than that.)
-__device__ __forceinline__ int range_begin(const Seqs& q, int i, int L) {
-  return (int)min((long long)i * L, (long long)q.T);
-}
+// The ranges that a packed stream is cut into. Split: by position, L tokens
+// each; a sequence over several ranges needs carries between them. Whole: range
+// i takes the sequences that begin in its L tokens, so none needs a carry, but
+// the longest sequence is one warp's walk; taken where that is at most `limit`
+// tokens (up to 31 sequences; the carries of many short ones cost little).
+struct Ranges {
+  int L;
+  bool whole;
+
+  __device__ __forceinline__ Ranges(const SeqView& v, int L_, int limit) : L(L_), whole(false) {
+    if (!v.held) return;
+    const int next = __shfl_down_sync(0xffffffffu, v.mine, 1);
+    const int longest = __reduce_max_sync(0xffffffffu, v.lane < v.q.nseq ? next - v.mine : 0);
+    whole = longest <= limit;
+  }
+
+  // The first token of range i.
+  __device__ __forceinline__ int begin(const SeqView& v, int i) const {
+    const int p = (int)min((long long)i * L, (long long)v.q.T);
+    if (!whole || i == 0) return p;
+    const unsigned m = __ballot_sync(0xffffffffu, v.lane <= v.q.nseq && v.mine >= p);
+    return m == 0 ? v.q.T : min(v.q.T, __shfl_sync(0xffffffffu, v.mine, __ffs(m) - 1));
+  }
+};
 
 // NV consecutive elements of a row as fp32. vec: the row starts on a whole
 // vector and all NV are there; else one by one, `n` of them, the rest zero.
@@ -154,6 +173,19 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 // All of this thread's copies have landed.
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// A whole aligned vector of NV elements into shared memory.
+template <typename T, int NV>
+__device__ __forceinline__ void copy_vec(T* dst, const T* src) {
+  constexpr int kBytes = sizeof(T) * NV;
+  if constexpr (kBytes <= 16) {
+    copy_async<kBytes>(dst, src, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i)
+      copy_async<16>(dst + i * (16 / sizeof(T)), src + i * (16 / sizeof(T)), true);
+  }
+}
+
 // NV elements of a row into shared memory: asynchronously when the row is
 // there in whole aligned vectors, else n of them one by one and zeros.
 template <typename T, int NV>
@@ -175,16 +207,14 @@ __device__ __forceinline__ void copy_part(T* dst, const T* src, const T* base, i
   }
 }
 
-// Four consecutive elements (aligned) in fp32. For bf16 two shifts and two
-// masks, written out.
+// Four elements in fp32. For bf16 two shifts and two masks, written out.
 template <typename T>
-__device__ __forceinline__ float4 widen4(const T* s) {
-  const Pack<T, 4> v = load_part<T, 4>(s, 4, true);
+__device__ __forceinline__ float4 widen4(const Pack<T, 4>& v) {
   return make_float4(to_f(v.v[0]), to_f(v.v[1]), to_f(v.v[2]), to_f(v.v[3]));
 }
 template <>
-__device__ __forceinline__ float4 widen4(const __nv_bfloat16* s) {
-  const uint2 w = *reinterpret_cast<const uint2*>(s);
+__device__ __forceinline__ float4 widen4(const Pack<__nv_bfloat16, 4>& v) {
+  const uint2 w = *reinterpret_cast<const uint2*>(&v);
   return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                      __uint_as_float(w.y & 0xffff0000u));
 }
@@ -226,6 +256,22 @@ __device__ __forceinline__ f2 f2_ex2(f2 x) {
   float a, b;
   unpack2(x, a, b);
   return pack2(ex2(a), ex2(b));
+}
+
+// 2^(d a) of two pairs: a decay. ex2's results are low by 0.6e-8 to 2.6e-8 of
+// their value on average between -0.1 and 0 (measured; an ulp is 6e-8), and a
+// state that remembers a thousand tokens adds that up a thousand times. kLift in
+// the exponent, which the multiplication takes for nothing, brings the average
+// to within 1.3e-8 there and leaves 2^0 at 1 (error of dA over 16384 tokens:
+// 1.8e-6 without, 0.8e-6 with it).
+constexpr float kLift = 2e-8f;
+// (Scalar, with the lift as an immediate: as a packed operation it takes a third
+// register pair, and the backward 2150 us instead of 1680.)
+__device__ __forceinline__ f2 f2_decay(f2 d, f2 a) {
+  float d0, d1, a0, a1;
+  unpack2(d, d0, d1);
+  unpack2(a, a0, a1);
+  return pack2(ex2(fmaf(d0, a0, kLift)), ex2(fmaf(d1, a1, kLift)));
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

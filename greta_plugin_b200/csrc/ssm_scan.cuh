@@ -32,7 +32,8 @@
 // S and the sum of dt; the second adds them up over the ranges back to the
 // sequence's start: h = S_j + exp(A sum dt_j) h. So the exponentials of split
 // sequences are paid twice, and the host cuts no finer than it takes to fill
-// the GPU.
+// the GPU; where the longest sequence allows it, ranges take whole sequences
+// instead (Ranges).
 #pragma once
 
 #include "ssm_common.cuh"
@@ -53,6 +54,7 @@ struct ScanParams {
   int D, N, F, Dg;  // Dg = D / F channels per group
   int spg;          // channel slices per group
   int R, L;         // ranges, tokens per range
+  int whole_limit;  // longest sequence with which ranges take whole sequences
   int softplus;
   int zero_rest;    // rows outside every sequence: zeros (else left alone)
   int vec;          // rows of u, delta, gate, out (and the backward's) are whole aligned vectors
@@ -230,6 +232,42 @@ __device__ __forceinline__ void copy_tile(const void* base, long long ld, bool v
   }
 }
 
+// A slice whose every vector is whole: its whole tiles are copied without a
+// test (most of what a tile takes beside the recurrence was such tests).
+template <int LN, int KD>
+__device__ __forceinline__ bool regular(const ScanParams& p, const Lanes<LN, KD>& l) {
+  return p.vec && p.vec_bc && l.nch == Lanes<LN, KD>::CHW;
+}
+
+// The lane's vector of row 0 of a [T, D] operand; a whole tile of it.
+template <typename T, int LN, int KD>
+__device__ __forceinline__ const T* lane_row(const void* base, long long ld, const Lanes<LN, KD>& l) {
+  using TV = TileVecs<Lanes<LN, KD>::CHW>;
+  return reinterpret_cast<const T*>(base) + TV::row(0, l.lane) * ld + l.c0 + TV::chan(l.lane);
+}
+template <typename T, int LN, int KD>
+__device__ __forceinline__ void copy_whole(const T* row0, long long ld, const Lanes<LN, KD>& l, int tile0, T* s) {
+  constexpr int CHW = Lanes<LN, KD>::CHW;
+  using TV = TileVecs<CHW>;
+  static_assert(TV::NVEC == 1, "a vector of a tile per lane");
+  if (TV::has(0, l.lane))
+    copy_vec<T, TV::V>(s + TV::row(0, l.lane) * CHW + TV::chan(l.lane), row0 + tile0 * ld);
+}
+// B and C of a whole tile (lane `at` of `lanes`); states past N stay as they are.
+template <typename T, int LN, int KD>
+__device__ __forceinline__ void copy_whole_bc(const ScanParams& p, const Lanes<LN, KD>& l, int tile0, T* s, int at,
+                                              int lanes) {
+#pragma unroll
+  for (int i0 = 0; i0 < kTile * 2 * LN; i0 += lanes) {
+    const int i = i0 + at, n = i % LN * 4;
+    if (kTile * 2 * LN % lanes != 0 && i >= kTile * 2 * LN) break;
+    const bool b = i / LN % 2 == 0;
+    if (n < p.N)
+      copy_vec<T, 4>(s + i * 4, reinterpret_cast<const T*>(b ? p.B : p.C) +
+                                    (tile0 + i / (2 * LN)) * (b ? p.ldb : p.ldc) + (long long)l.f * p.N + n);
+  }
+}
+
 // A lane's vector k of a tile in shared memory.
 template <typename T, int CHW>
 __device__ __forceinline__ Pack<T, TileVecs<CHW>::V> tile_vec(const T* s, int k, int lane) {
@@ -254,10 +292,15 @@ __device__ __forceinline__ void copy_bc(const ScanParams& p, const Lanes<LN, KD>
   }
 }
 
-// Four states of B or C in fp32, each twice (for two channels).
+// Four states of B or C (as they lie in shared memory), and in fp32, each twice
+// (for two channels).
 template <typename T>
-__device__ __forceinline__ void read_four(const T* s, f2 (&o)[4]) {
-  const float4 v = widen4(s);
+__device__ __forceinline__ Pack<T, 4> read_four(const T* s) {
+  return load_part<T, 4>(s, 4, true);
+}
+template <typename T>
+__device__ __forceinline__ void twice(const Pack<T, 4>& r, f2 (&o)[4]) {
+  const float4 v = widen4(r);
   o[0] = pack2(v.x, v.x);
   o[1] = pack2(v.y, v.y);
   o[2] = pack2(v.z, v.z);
@@ -278,7 +321,7 @@ __device__ __forceinline__ void scan_step(LaneStates<KD>& h, const LaneStates<KD
   for (int j = 0; j < KD / 2; ++j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f2 a = f2_ex2(f2_mul(dl[j].x, A2[j][i]));
+      const f2 a = f2_decay(dl[j].x, A2[j][i]);
       h[j][i] = f2_fma(a, h[j][i], f2_mul(dl[j].y, b[i]));
       if (WITH_Y) y[j] = i == 0 ? f2_mul(c[i], h[j][i]) : f2_fma(c[i], h[j][i], y[j]);
     }
@@ -337,7 +380,7 @@ __device__ __forceinline__ void carry_through(const ScanParams& p, const Lanes<L
       }
       const f2 d2 = pack2(d[0], d[1]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) h[c][k] = f2_fma(f2_ex2(f2_mul(d2, A2[c][k])), h[c][k], s[c][k]);
+      for (int k = 0; k < 4; ++k) h[c][k] = f2_fma(f2_decay(d2, A2[c][k]), h[c][k], s[c][k]);
     }
   }
 }
@@ -486,8 +529,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
   const L l(p, slice, lane);
   const int ri = blockIdx.y;
   const SeqView sv(p.q, lane);
-  int t0 = range_begin(p.q, ri, p.L);
-  const int t1 = range_begin(p.q, ri + 1, p.L);
+  const Ranges ranges(sv, p.L, p.whole_limit);
+  if (!kMain && ranges.whole) return;  // no range needs a carry
+  int t0 = ranges.begin(sv, ri);
+  const int t1 = ri + 1 < p.R ? ranges.begin(sv, ri + 1) : p.q.T;
   if (t0 >= t1) return;
 
   LaneStates<KD> A2, h;
@@ -529,32 +574,60 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
 
   int cur = 0;
   const T* bc;
+  const bool reg = regular(p, l);
+  const T* u0 = lane_row<T>(p.u, p.ldu, l);
+  const T* d0 = lane_row<T>(p.delta, p.ldd, l);
+  const T* z0 = lane_row<T>(p.gate, p.ldg, l);
   auto fetch = [&](int tile0, int s) {
-    const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
-    copy_tile<T>(p.u, p.ldu, p.vec, l, tile0, ta, tb, stage(s, 0));
-    copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
-    if (kMain && p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
-    copy_bc<T>(p, l, tile0, ta, tb, stage(s, 3), lane, 32);
+    if (reg && tile0 >= t0 && tile0 + kTile <= t1) {
+      copy_whole(u0, p.ldu, l, tile0, stage(s, 0));
+      copy_whole(d0, p.ldd, l, tile0, stage(s, 1));
+      if (kMain && p.gate != nullptr) copy_whole(z0, p.ldg, l, tile0, stage(s, 2));
+      copy_whole_bc<T>(p, l, tile0, stage(s, 3), lane, 32);
+    } else {
+      const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
+      copy_tile<T>(p.u, p.ldu, p.vec, l, tile0, ta, tb, stage(s, 0));
+      copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
+      if (kMain && p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
+      copy_bc<T>(p, l, tile0, ta, tb, stage(s, 3), lane, 32);
+    }
     copy_commit();
   };
-  // token r of the tile
-  auto step = [&](int r) {
-    ulonglong2 dv[KD / 2];
-    f2 b[4], c[4], y[KD / 2];
-    read_steps<KD>(dl, r * CHW + l.ch(0), dv);
-    read_four(bc + r * 2 * NP + l.n0(), b);
-    if (kMain) read_four(bc + (r * 2 + 1) * NP + l.n0(), c);
-    scan_step<kMain, KD>(h, A2, dv, b, c, y);
+  // states past N: B and C of both stages zero for good
+  if (p.N < NP) {
+    for (int i = lane; i < kTile * 2 * NP; i += 32) stage(0, 3)[i] = stage(1, 3)[i] = from_f<T>(0.f);
+    __syncwarp();
+  }
+  // What token r of the tile needs from shared memory; its recurrence; its sum.
+  // Whole tiles read a token ahead and sum a token behind, so that neither the
+  // reads nor the shuffles of a sum stand between two tokens' recurrences.
+  struct Operands {
+    ulonglong2 dl[KD / 2];
+    Pack<T, 4> b, c;
+  };
+  auto read = [&](int r, Operands& o) {
+    read_steps<KD>(dl, r * CHW + l.ch(0), o.dl);
+    o.b = read_four(bc + r * 2 * NP + l.n0());
+    if (kMain) o.c = read_four(bc + (r * 2 + 1) * NP + l.n0());
+  };
+  auto step = [&](const Operands& o, f2 (&y)[KD / 2]) {
+    f2 b[4], c[4];
+    twice(o.b, b);
+    if (kMain) twice(o.c, c);
+    scan_step<kMain, KD>(h, A2, o.dl, b, c, y);
+    if (!kMain) {
+#pragma unroll
+      for (int j = 0; j < KD / 2; ++j) dsum[j] = f2_add(dsum[j], o.dl[j].x);
+    }
+  };
+  auto sum = [&](int r, const f2 (&y)[KD / 2]) {
     if (kMain) {
       const float s = sum_over_states<LN>(y, lane);
       if (l.nq < KD) ys[r * CHW + l.ch(sum_channel<KD>(lane))] = s;
-    } else {
-#pragma unroll
-      for (int j = 0; j < KD / 2; ++j) dsum[j] = f2_add(dsum[j], dv[j].x);
     }
   };
 
-  // (the carry of a range begins where its last sequence does)
+  // (a carry, and a range of whole sequences, may begin inside a tile)
   const int tile_first = t0 / kTile * kTile;
   fetch(tile_first, 0);
   for (int tile0 = tile_first; tile0 < t1; tile0 += kTile, cur ^= 1) {
@@ -566,7 +639,38 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
     __syncwarp();
     // (the other stage's B and C were last read ahead of the barrier before)
     if (tile0 + kTile < t1) fetch(tile0 + kTile, cur ^ 1);
-    if (kMain && p.ckpt != nullptr) store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
+    if (kMain && p.ckpt != nullptr && ta == tile0) store_states(p.ckpt + (tile0 / kTile) * DN, l, p.N, h);
+    // out of the tile's sums, for the lane's vector
+    auto output = [&](int tt, bool in, int n, bool vec) {
+      const int r = TV::row(0, lane), c = TV::chan(lane);
+      const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), 0, lane);
+      const Pack<float, V> y = load_part<float, V>(ys + r * CHW + c, V, true);
+      Pack<T, V> z, o;
+      if (p.gate != nullptr) z = tile_vec<T, CHW>(stage(cur, 2), 0, lane);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float v = fmaf(skip[e], to_f(u.v[e]), y.v[e]);
+        if (p.gate != nullptr) v *= to_f(z.v[e]) * sigmoid_t<T>(to_f(z.v[e]));
+        o.v[e] = from_f<T>(in ? v : 0.f);
+      }
+      store_part<T, V>(reinterpret_cast<T*>(p.out) + (long long)tt * p.D + l.c0 + c, o, n, vec);
+    };
+    if (reg && g.in && g.b < ta && g.e > tb && tb - ta == kTile) {
+      // a whole tile inside a sequence
+      Operands o[2];
+      f2 y[2][KD / 2];
+      read(0, o[0]);
+#pragma unroll
+      for (int r = 0; r < kTile; ++r) {
+        if (r + 1 < kTile) read(r + 1, o[(r + 1) % 2]);
+        step(o[r % 2], y[r % 2]);
+        if (r > 0) sum(r - 1, y[(r + 1) % 2]);
+      }
+      sum(kTile - 1, y[(kTile - 1) % 2]);
+      __syncwarp();
+      if (kMain && TV::has(0, lane)) output(tile0 + TV::row(0, lane), true, V, true);
+      continue;
+    }
     unsigned live = 0;  // tokens of the tile that a sequence holds
     int t = ta;
     while (t < tb) {
@@ -584,11 +688,13 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
               load_slot(p, slot, l, h);
           }
         }
-        if (stop - t == kTile) {
-#pragma unroll
-          for (int r = 0; r < kTile; ++r) step(r);
-        } else {
-          for (int r = t - tile0; r < stop - tile0; ++r) step(r);
+#pragma unroll 1
+        for (int r = t - tile0; r < stop - tile0; ++r) {
+          Operands o;
+          f2 y[KD / 2];
+          read(r, o);
+          step(o, y);
+          sum(r, y);
         }
         live |= tile_rows(tile0, t, stop);
         if (kMain && stop == g.e && slot >= 0) store_slot(p, slot, l, h);
@@ -597,25 +703,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_fwd_kernel(const 
       if (t == g.e && t < t1) g = sv.next(g);
     }
     __syncwarp();
-    if (kMain) {
-#pragma unroll
-      for (int k = 0; k < TV::NVEC; ++k) {
-        const int r = TV::row(k, lane), c = TV::chan(lane), tt = tile0 + r, n = l.nch - c;
-        if (!TV::has(k, lane) || tt < ta || tt >= tb || n <= 0) continue;
-        const bool in = (live >> r) & 1;
-        if (!in && !p.zero_rest) continue;
-        const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane);
-        const Pack<float, V> y = load_part<float, V>(ys + r * CHW + c, V, true);
-        Pack<T, V> z, o;
-        if (p.gate != nullptr) z = tile_vec<T, CHW>(stage(cur, 2), k, lane);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float v = fmaf(skip[e], to_f(u.v[e]), y.v[e]);
-          if (p.gate != nullptr) v *= to_f(z.v[e]) * sigmoid_t<T>(to_f(z.v[e]));
-          o.v[e] = from_f<T>(in ? v : 0.f);
-        }
-        store_part<T, V>(reinterpret_cast<T*>(p.out) + (long long)tt * p.D + l.c0 + c, o, n, p.vec && n >= V);
-      }
+    if (kMain && TV::has(0, lane)) {
+      const int r = TV::row(0, lane), tt = tile0 + r, n = l.nch - TV::chan(lane);
+      const bool in = (live >> r) & 1;
+      if (tt >= ta && tt < tb && n > 0 && (in || p.zero_rest)) output(tt, in, n, p.vec && n >= V);
     }
   }
   if (!kMain) {
@@ -765,8 +856,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_decode_kernel(con
         d[j].y = pack2(y[0], y[1]);
       }
       f2 b2[4], c2[4], y[KD / 2];
-      read_four(s + 3 * CHW + l.n0(), b2);
-      read_four(s + 3 * CHW + NP + l.n0(), c2);
+      twice(read_four(s + 3 * CHW + l.n0()), b2);
+      twice(read_four(s + 3 * CHW + NP + l.n0()), c2);
       scan_step<true, KD>(h, A2, d, b2, c2, y);
       float o = sum_over_states<LN>(y, lane);
       if (own) {

@@ -133,8 +133,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   const int ri = blockIdx.y;
   if (ri == 0) return;
   const SeqView sv(p.q, lane);
-  const int t0 = range_begin(p.q, ri, p.L);
-  int t1 = range_begin(p.q, ri + 1, p.L);
+  const Ranges ranges(sv, p.L, p.whole_limit);
+  if (ranges.whole) return;  // no range needs a carry
+  const int t0 = ranges.begin(sv, ri);
+  int t1 = ranges.begin(sv, ri + 1);
   if (t0 >= t1) return;
   const Seg g = sv.at(t0);
   if (!g.in || g.b >= t0) return;
@@ -152,25 +154,40 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_bwd_carry_kernel(
   for (int j = 0; j < KD / 2; ++j) dsum[j] = 0ull;
   int cur = 0;
   const T* bc;
+  const bool reg = regular(p, l);
+  const T* g0 = lane_row<T>(p.dout, p.D, l);
+  const T* d0 = lane_row<T>(p.delta, p.ldd, l);
+  const T* z0 = lane_row<T>(p.gate, p.ldg, l);
   auto fetch = [&](int tile0, int s) {
-    const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
-    copy_tile<T>(p.dout, p.D, p.vec, l, tile0, ta, tb, stage(s, 0));
-    copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
-    if (p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
-    copy_bc<T>(p, l, tile0, ta, tb, stage(s, 3), lane, 32);
+    if (reg && tile0 >= t0 && tile0 + kTile <= t1) {
+      copy_whole(g0, p.D, l, tile0, stage(s, 0));
+      copy_whole(d0, p.ldd, l, tile0, stage(s, 1));
+      if (p.gate != nullptr) copy_whole(z0, p.ldg, l, tile0, stage(s, 2));
+      copy_whole_bc<T>(p, l, tile0, stage(s, 3), lane, 32);
+    } else {
+      const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
+      copy_tile<T>(p.dout, p.D, p.vec, l, tile0, ta, tb, stage(s, 0));
+      copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
+      if (p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
+      copy_bc<T>(p, l, tile0, ta, tb, stage(s, 3), lane, 32);
+    }
     copy_commit();
   };
+  if (p.N < NP) {  // states past N: B and C of both stages zero for good
+    for (int i = lane; i < kTile * 2 * NP; i += 32) stage(0, 3)[i] = stage(1, 3)[i] = from_f<T>(0.f);
+    __syncwarp();
+  }
   auto step = [&](int i) {
     ulonglong2 d[KD / 2];
     f2 c[4], y[KD / 2];
     read_steps<KD>(dl, i * CHW + l.ch(0), d);
-    read_four(bc + (i * 2 + 1) * NP + l.n0(), c);
+    twice(read_four(bc + (i * 2 + 1) * NP + l.n0()), c);
     read_dy<KD>(dy + i * CHW + l.ch(0), y);
 #pragma unroll
     for (int j = 0; j < KD / 2; ++j) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        r[j][k] = f2_mul(f2_ex2(f2_mul(d[j].x, A2[j][k])), f2_fma(c[k], y[j], r[j][k]));
+        r[j][k] = f2_mul(f2_decay(d[j].x, A2[j][k]), f2_fma(c[k], y[j], r[j][k]));
       dsum[j] = f2_add(dsum[j], d[j].x);
     }
   };
@@ -222,7 +239,7 @@ struct BwdSmem {
 // Four states of B or C in fp32, as pairs of states.
 template <typename T>
 __device__ __forceinline__ void read_pairs(const T* s, f2 (&o)[2]) {
-  const float4 v = widen4(s);
+  const float4 v = widen4(read_four(s));
   o[0] = pack2(v.x, v.y);
   o[1] = pack2(v.z, v.w);
 }
@@ -273,8 +290,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   if (!have) l.nch = 0;
   const int ri = blockIdx.y;
   const SeqView sv(p.q, lane);
-  const int t0 = range_begin(p.q, ri, p.L);
-  const int t1 = range_begin(p.q, ri + 1, p.L);
+  const Ranges ranges(sv, p.L, p.whole_limit);
+  const int t0 = ranges.begin(sv, ri);
+  const int t1 = ri + 1 < p.R ? ranges.begin(sv, ri + 1) : p.q.T;
   const long long DN = (long long)p.D * p.N;
   f2 A2[KD][2], dA[KD][2], rr[KD][2];
   {
@@ -304,21 +322,51 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   }
   Seg g{-1, 0, 0, false};
 
+  const bool reg = regular(p, l) && p.N % 4 == 0;
+  const T* u0 = lane_row<T>(p.u, p.ldu, l);
+  const T* d0 = lane_row<T>(p.delta, p.ldd, l);
+  const T* z0 = lane_row<T>(p.gate, p.ldg, l);
+  const T* g0 = lane_row<T>(p.dout, p.D, l);
+  const float* h0 = p.ckpt + (long long)(l.c0 + l.ch(0)) * p.N + l.n0();
   auto fetch = [&](int tile0, int s) {
+    T* bcs = reinterpret_cast<T*>(base + s * S::kBC);
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
-    copy_tile<T>(p.u, p.ldu, p.vec, l, tile0, ta, tb, stage(s, 0));
-    copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
-    if (p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
-    copy_tile<T>(p.dout, p.D, p.vec, l, tile0, ta, tb, stage(s, 3));
-    copy_bc<T>(p, l, tile0, ta, tb, reinterpret_cast<T*>(base + s * S::kBC), threadIdx.x, kScanWarps * 32);
-    const float* c = p.ckpt + (tile0 / kTile) * DN;
+    // (a range that begins inside a tile begins there with a sequence, or
+    // outside, and does not use the states saved ahead of the tile)
+    if (reg && tb - ta == kTile) {
+      copy_whole(u0, p.ldu, l, tile0, stage(s, 0));
+      copy_whole(d0, p.ldd, l, tile0, stage(s, 1));
+      if (p.gate != nullptr) copy_whole(z0, p.ldg, l, tile0, stage(s, 2));
+      copy_whole(g0, p.D, l, tile0, stage(s, 3));
+      if (l.n0() < p.N) {
+        const float* c = h0 + (tile0 / kTile) * DN;
 #pragma unroll
-    for (int j = 0; j < KD; ++j)
-      copy_part<float, 4>(reinterpret_cast<float*>(saved(s) + j * 32),
-                          c + (long long)(l.c0 + l.ch(j)) * p.N + l.n0(), p.ckpt,
-                          l.ch(j) < l.nch ? p.N - l.n0() : 0, p.N % 4 == 0);
+        for (int j = 0; j < KD; ++j) copy_async<16>(saved(s) + j * 32, c + j * p.N, true);
+      }
+    } else {
+      copy_tile<T>(p.u, p.ldu, p.vec, l, tile0, ta, tb, stage(s, 0));
+      copy_tile<T>(p.delta, p.ldd, p.vec, l, tile0, ta, tb, stage(s, 1));
+      if (p.gate != nullptr) copy_tile<T>(p.gate, p.ldg, p.vec, l, tile0, ta, tb, stage(s, 2));
+      copy_tile<T>(p.dout, p.D, p.vec, l, tile0, ta, tb, stage(s, 3));
+      const float* c = p.ckpt + (tile0 / kTile) * DN;
+#pragma unroll
+      for (int j = 0; j < KD; ++j)
+        copy_part<float, 4>(reinterpret_cast<float*>(saved(s) + j * 32),
+                            c + (long long)(l.c0 + l.ch(j)) * p.N + l.n0(), p.ckpt,
+                            l.ch(j) < l.nch ? p.N - l.n0() : 0, p.N % 4 == 0);
+    }
+    if (p.vec_bc && tb - ta == kTile)
+      copy_whole_bc<T>(p, l, tile0, bcs, threadIdx.x, kScanWarps * 32);
+    else
+      copy_bc<T>(p, l, tile0, ta, tb, bcs, threadIdx.x, kScanWarps * 32);
     copy_commit();
   };
+  if (p.N < NP) {  // states past N: B, C and saved states of both stages zero for good
+    for (int i = threadIdx.x; i < 2 * kTile * 2 * NP; i += kScanWarps * 32) reinterpret_cast<T*>(base)[i] = from_f<T>(0.f);
+#pragma unroll
+    for (int j = 0; j < 2 * KD; ++j) saved(j / KD)[j % KD * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+  }
   const int last = t1 > t0 ? (t1 - 1) / kTile * kTile : -kTile;
   if (last >= 0) fetch(last, 0);
   int cur = 0;
@@ -401,7 +449,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
           const f2 d2 = pack2(dt[j], dt[j]), du2 = pack2(du[j], du[j]);
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            hs[r + 1][j][k] = f2_fma(f2_ex2(f2_mul(d2, A2[j][k])), first ? 0ull : hs[r][j][k], f2_mul(du2, b[k]));
+            hs[r + 1][j][k] = f2_fma(f2_decay(d2, A2[j][k]), first ? 0ull : hs[r][j][k], f2_mul(du2, b[k]));
           if (p.gate != nullptr) y[j] = f2_sum(f2_fma(c[1], hs[r + 1][j][1], f2_mul(c[0], hs[r + 1][j][0])));
         }
         if (p.gate != nullptr) {
@@ -441,7 +489,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
           f2 s2 = 0ull, g2 = 0ull;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const f2 a = f2_ex2(f2_mul(d2, A2[j][k]));
+            const f2 a = f2_decay(d2, A2[j][k]);
             const f2 gg = f2_fma(c[k], y2, rr[j][k]);
             const f2 ag = first ? 0ull : f2_mul(a, gg);
             // (what is ahead of a first token is another sequence's, maybe NaN)

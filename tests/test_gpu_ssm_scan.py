@@ -101,6 +101,14 @@ def test_train_split_ranges(ranges, lens):
     check_train(lens, 40, 16, seed=ranges, ranges=ranges)
 
 
+@pytest.mark.parametrize("lens", [[24] * 20, [5, 0, 40, 1, 1, 33, 17, 8, 64, 2, 0, 30] * 2, [16] * 31, [9] * 40])
+@pytest.mark.parametrize("head, tail", [(0, 0), (13, 21)])
+def test_train_whole_sequences(lens, head, tail):
+    """Many short sequences and enough channels: ranges of whole sequences, which
+    begin inside tiles (up to 31; 40 are cut by position)."""
+    check_train(lens, 2048, 16, dtype=torch.bfloat16, head=head, tail=tail)
+
+
 @pytest.mark.parametrize("ranges", [0, 1, 4])
 def test_train_slow_decay_long(ranges):
     """Decay rates of 0.05 to 0.1 a unit step: states that remember hundreds of
@@ -342,6 +350,11 @@ def test_packed_decode(n, D, N, F, layout):
     if n > 2:
         slots[1], init[2] = -1, 0
     check_packed([1] * n, slots, init, D, N, F, torch.bfloat16, layout)
+
+
+def test_packed_whole_sequences():
+    lens = [33, 2, 40, 0, 17, 64, 1, 50, 50, 8, 31, 60]
+    check_packed(lens, list(range(12)), [1, 0] * 6, 2048, 16, tail=9)
 
 
 def test_packed_decode_uneven():
