@@ -78,16 +78,14 @@ def packed_batch_metadata(query_lens: torch.Tensor, context_lens: torch.Tensor, 
         raise ValueError("packed_batch_metadata requires CUDA tensors")
     query_lens, context_lens = query_lens.contiguous(), context_lens.contiguous()
     free_blocks = None if free_blocks is None else free_blocks.contiguous()
-    i32, i64 = torch.int32, torch.int64
     # int32 and int64 results share a buffer each (an allocation costs as much as
-    # the kernel's launch)
-    i32, i64 = torch.int32, torch.int64
-    starts, seq_idx, used = torch.empty(N + T + 2, dtype=i32, device=dev).split((N + 1, T, 1))
+    # a third of the kernel's launch)
+    starts, seq_idx, used = torch.split_with_sizes(query_lens.new_empty(N + T + 2), (N + 1, T, 1))
     init = torch.empty(N, dtype=torch.int8, device=dev)
     if paged:
-        positions, slot_map = torch.empty(2, T, dtype=i64, device=dev).unbind()
+        positions, slot_map = torch.empty((2, T), dtype=torch.int64, device=dev).unbind()
     else:
-        positions, slot_map, used = torch.empty(T, dtype=i64, device=dev), None, None
+        positions, slot_map, used = torch.empty(T, dtype=torch.int64, device=dev), None, None
     p = _capi.addr
     # a table without entries has no address of its own
     width = block_tables.shape[1] if paged else 0

@@ -61,8 +61,9 @@ def _check_weight(x, weight, bias):
 
 def same_device(name, t, **others):
     dev = t.get_device()
-    for k, o in others.items():
+    for o in others.values():
         if o is not None and o.get_device() != dev:
+            k = next(k for k, v in others.items() if v is o)
             raise ValueError(f"{k} is on {o.device}, {name} on {t.device}")
 
 
@@ -174,9 +175,11 @@ def check_disjoint(out, **inputs):
         b0 = t.data_ptr()
         if b0 >= a1 or t.numel() == 0 or a0 == a1:
             continue
-        span = 1
-        for n, s in zip(t.shape, t.stride()):
-            span += (n - 1) * s
+        span = t.numel()
+        if not t.is_contiguous():
+            span = 1
+            for n, s in zip(t.shape, t.stride()):
+                span += (n - 1) * s
         if a0 < b0 + span * t.element_size():
             raise ValueError(f"out must not overlap {name}")
 

@@ -233,15 +233,15 @@ struct BwdSmem {
   static constexpr int kStage = 4 * kRow + 32 * kBwdChans * 16;  // u, delta, gate, dout; saved states
   static constexpr int kWarp = kStage0 + 2 * kStage;
   static constexpr int kBC = kTile * 2 * NP * (int)sizeof(T);
-  static constexpr int kTotal = kScanWarps * kWarp + 2 * kBC;
+  static constexpr int kWide = sizeof(T) == 4 ? 0 : kTile * 2 * NP * 4;  // B and C in fp32
+  static constexpr int kTotal = kScanWarps * kWarp + 2 * kBC + kWide;
 };
 
-// Four states of B or C in fp32, as pairs of states.
-template <typename T>
-__device__ __forceinline__ void read_pairs(const T* s, f2 (&o)[2]) {
-  const float4 v = widen4(read_four(s));
-  o[0] = pack2(v.x, v.y);
-  o[1] = pack2(v.z, v.w);
+// Four states of B or C, as pairs of states.
+__device__ __forceinline__ void read_pairs(const float* s, f2 (&o)[2]) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(s);
+  o[0] = v.x;
+  o[1] = v.y;
 }
 
 // Pairs of channels to pairs of states.
@@ -374,7 +374,16 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
     const TileSeqs q = tile_seqs(sv, tile0, ta, tb, g);
     copy_wait();
-    const T* bc = reinterpret_cast<T*>(base + cur * S::kBC);
+    // B and C widened once for the CTA (each thread what it copied itself)
+    const float* bc = reinterpret_cast<const float*>(base + cur * S::kBC);
+    if (sizeof(T) != 4) {
+      float* wide = reinterpret_cast<float*>(base + 2 * S::kBC + kScanWarps * S::kWarp);
+      const T* bcs = reinterpret_cast<const T*>(base + cur * S::kBC);
+#pragma unroll
+      for (int i = threadIdx.x; i < kTile * 2 * LN; i += kScanWarps * 32)
+        *reinterpret_cast<float4*>(wide + i * 4) = widen4(read_four(bcs + i * 4));
+      bc = wide;
+    }
     f2 hs[kTile + 1][KD][2];
 #pragma unroll
     for (int j = 0; j < KD; ++j) {

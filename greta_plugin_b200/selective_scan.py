@@ -97,8 +97,8 @@ def _operands(u, delta, A, B, C, skip, gate, delta_bias):
     A, skip, delta_bias = _fp32(A), _fp32(skip), _fp32(delta_bias)
     p = _capi.addr
     return (u, delta, gate, B, C, A, skip, delta_bias), (
-        _capi.dtype_code(u), p(u), ldu, p(delta), ldd, p(gate), ldg, p(B), ldb, p(C), ldc, p(A), p(skip),
-        p(delta_bias))
+        _capi.dtype_code(u), u.data_ptr(), ldu, delta.data_ptr(), ldd, p(gate), ldg, B.data_ptr(), ldb, C.data_ptr(),
+        ldc, A.data_ptr(), p(skip), p(delta_bias))
 
 
 @functools.lru_cache(maxsize=4096)
