@@ -12,18 +12,25 @@ constexpr int kMinRange = 32;  // tokens
 
 int64_t slices(int64_t D, int64_t N, int64_t F) { return F * fwd_slices_per_group(D, N, F); }
 
-// Ranges the stream is cut into, none shorter than kMinRange tokens: as many as
-// run at once (kCtasPerSm CTAs an SM), so that none waits for a place; twice as
-// many where they are longer than kLongRange, so that SMs that are done early
-// find more. 16384 x 4096 x 16, forward: 18 ranges 849 us, 36 794, 19 (one CTA
-// in 38 left over) 965; 898 tokens: 18 ranges 60 us, 24 64, 36 62, 9 88.
+// Ranges the stream is cut into, none shorter than kMinRange tokens. The
+// forward: two waves of the CTAs that run at once, so that SMs that are done
+// early find more (4096 x 4096 x 16: one wave 281 us with the carries, two 253;
+// 2048 tokens 152, 146), or one where two would be shorter than kTwoWaves tokens
+// (898 tokens: 60 us, 62). The backward: four waves (one 957 us, two 764, four
+// 597), or two where four are too short (2000 x 1024 x 16: 94 us, 111 for ranges
+// of kMinRange). Twice as many where they are longer than kLongRange (30000 tokens: two
+// waves 1640 us, four 1544; backward four 4078, eight 3903). R is rounded down:
+// one CTA in 38 left over cost 965 us instead of 794.
 // Returns the tokens per range (a multiple of kTile) and sets R.
-constexpr int kCtasPerSm = 4;
-constexpr int64_t kLongRange = 512;
-int64_t plan_ranges(int64_t T, int64_t D, int64_t N, int64_t F, int asked, int& R) {
+constexpr int kFwdCtasPerSm = 4, kBwdCtasPerSm = 3;
+constexpr int64_t kTwoWaves = 48, kLongRange = 512;
+int64_t plan_ranges(int64_t T, int64_t D, int64_t N, int64_t F, int asked, bool backward, int& R) {
   int64_t r = asked;
   if (asked <= 0) {
-    r = (int64_t)sm_count() * kCtasPerSm / cdiv(slices(D, N, F), kScanWarps);
+    const int64_t ctas = cdiv(slices(D, N, F), kScanWarps);  // of a range (forward)
+    const int64_t wave = (int64_t)sm_count() * (backward ? kBwdCtasPerSm : kFwdCtasPerSm);
+    r = 2 * wave / ctas;  // four waves in the backward, which has twice the CTAs a range
+    if (backward ? T < r * kMinRange : T < r * kTwoWaves) r = wave / ctas;
     if (r < 1) r = 1;
     if (T > r * kLongRange) r *= 2;
   }
@@ -186,7 +193,7 @@ int64_t greta_ssm_scan_workspace(int packed, int64_t num_seqs, int64_t T, int64_
   if (T <= 0 || D <= 0 || N <= 0 || F <= 0 || D % F != 0 || N > kMaxStates || ranges < 0) return 0;
   if (packed != 0 && is_decode(num_seqs, T, ranges)) return 0;
   int R = 1;
-  plan_ranges(T, D, N, F, ranges, R);
+  plan_ranges(T, D, N, F, ranges, false, R);
   return Workspace(R, D, N).total;
 }
 
@@ -204,7 +211,7 @@ int greta_ssm_scan_fwd(int dtype, const void* u, int64_t ldu, const void* delta,
   p.ckpt = saved;
   p.zero_rest = 1;
   plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, out});
-  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  p.L = (int)plan_ranges(T, D, N, F, ranges, false, p.R);
   p.whole_limit = whole_limit(T, D, N, F, ranges);
   c = set_workspace(p, workspace, workspace_bytes);
   if (c != GRETA_OK) return c;
@@ -242,7 +249,7 @@ int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* del
     p.L = (int)(per > 32 ? 32 : per);
     return run_decode(dtype, p, stream);
   }
-  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  p.L = (int)plan_ranges(T, D, N, F, ranges, false, p.R);
   p.whole_limit = whole_limit(T, D, N, F, ranges);
   c = set_workspace(p, workspace, workspace_bytes);
   if (c != GRETA_OK) return c;
@@ -253,7 +260,7 @@ int64_t greta_ssm_scan_bwd_workspace(int64_t num_seqs, int64_t T, int64_t D, int
   (void)num_seqs;
   if (T <= 0 || D <= 0 || N <= 0 || F <= 0 || D % F != 0 || N > kMaxStates || ranges < 0) return 0;
   int R = 1;
-  plan_ranges(T, D, N, F, ranges, R);
+  plan_ranges(T, D, N, F, ranges, true, R);
   return BwdWorkspace(R, T, D, N, F).total;
 }
 
@@ -284,7 +291,7 @@ int greta_ssm_scan_bwd(int dtype, const void* u, int64_t ldu, const void* delta,
   p.dout = dout;
   p.du = du; p.ddelta = ddelta; p.dgate = dgate;
   plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, dout, du, ddelta, dgate});
-  p.L = (int)plan_ranges(T, D, N, F, ranges, p.R);
+  p.L = (int)plan_ranges(T, D, N, F, ranges, true, p.R);
   p.whole_limit = whole_limit(T, D, N, F, ranges);
   const BwdWorkspace w(p.R, T, D, N, F);
   if (workspace == nullptr || workspace_bytes < w.total) return GRETA_ERR_INVALID_ARG;
