@@ -169,6 +169,14 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, bool ok) 
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
+// ... to shared memory at the 32-bit address d + OFF.
+template <int BYTES, int OFF>
+__device__ __forceinline__ void copy_async_to(unsigned d, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;" ::"r"(d), "l"(src), "n"(OFF) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0+%2], [%1], %3;" ::"r"(d), "l"(src), "n"(OFF), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All of this thread's copies have landed.
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
@@ -339,6 +347,21 @@ __device__ __forceinline__ float sigmoid_t(float x) {
     return sigmoid_exact(x);
   else
     return sigmoid_fast(x);
+}
+// Two of them.
+template <typename T>
+__device__ __forceinline__ f2 sigmoid2(f2 x) {
+  float a, b;
+  if constexpr (sizeof(T) == 4) {
+    unpack2(x, a, b);
+    return pack2(sigmoid_exact(a), sigmoid_exact(b));
+  } else {
+    unpack2(f2_mul(x, pack2(-kLog2e, -kLog2e)), a, b);
+    unpack2(f2_add(pack2(ex2(a), ex2(b)), pack2(1.f, 1.f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return pack2(a, b);
+  }
 }
 
 }  // namespace greta

@@ -39,13 +39,24 @@ int check(int dtype, const void* x, int64_t ldx, const void* w, const void* y, c
 // another.
 constexpr int64_t kDecodeExtra = 8;
 
-// Tokens per run: as many as leave each SM 12 warps (all of them running at
-// once, and enough rows in flight to fill HBM), a power of two between lo and hi.
-int run_tokens(int64_t T, int64_t warps_per_run, int lo, int hi) {
-  const int64_t want = T * warps_per_run / ((int64_t)sm_count() * 12);
-  int L = lo;
-  while (L < hi && 2 * L <= want) L *= 2;
-  return L;
+// Tokens per run, whole groups of four: as few as fill every SM with the CTAs it
+// has registers for, rounded up so that none is left over, or fill it several
+// times where a run would be longer than kMaxRun. Backward of 16288 x 4096 x 4
+// taps, bf16: runs of 56 tokens (four fills) 115 us, 112 104, 228 100; 220, with
+// 16 CTAs left over, 129.
+constexpr int64_t kCtasPerSm = 4;
+constexpr int64_t kMaxRun = 256;
+int run_tokens(int64_t T, int64_t ctas_per_row, int lo) {
+  const int64_t wave = (int64_t)sm_count() * kCtasPerSm;
+  int64_t L = T;
+  for (int64_t k = cdiv(T * ctas_per_row, wave * kRuns * kMaxRun); ; ++k) {
+    const int64_t rows = wave * k / ctas_per_row;
+    if (rows < 1) continue;
+    L = cdiv(T, rows * kRuns);
+    if (L <= kMaxRun) break;
+  }
+  if (L > kGroup) L = cdiv(L, kGroup) * kGroup;
+  return (int)(L < lo ? lo : L);
 }
 
 // Elements of a thread's vector for a kernel of WT taps: 16 bytes for the small
@@ -79,7 +90,7 @@ int fwd_one(ConvParams p, cudaStream_t st) {
     if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
     return finish(launch(ssm_conv_decode_kernel<T, NV, WT>, dim3((unsigned)blocks), dim3(32, kRuns), 0, st, p));
   }
-  p.L = run_tokens(p.q.T, cw, 1, 64);
+  p.L = run_tokens(p.q.T, cw, 1);
   const int64_t blocks = cdiv(cdiv(p.q.T, p.L), kRuns) * cw;
   if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
   const size_t smem = NV > 1 ? (size_t)kRuns * ConvRing<T, NV>::kBytes : 0;
@@ -106,7 +117,7 @@ int fwd(int dtype, const ConvParams& p, void* stream) {
   }
 }
 
-constexpr int kBwdMinRun = 8, kBwdMaxRun = 64;
+constexpr int kBwdMinRun = 8;
 
 // Rows of partial sums of the backward.
 int64_t bwd_rows(int64_t T, int L) { return cdiv(cdiv(T, L), kRuns); }
@@ -115,7 +126,7 @@ template <typename T, int NV, int WT>
 int bwd_one(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
   p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
   const int64_t cw = cdiv(cdiv(p.D, NV), 32);
-  p.L = run_tokens(p.q.T, cw, kBwdMinRun, kBwdMaxRun);
+  p.L = run_tokens(p.q.T, cw, kBwdMinRun);
   p.nblk = (int)cw;
   const int64_t rows = bwd_rows(p.q.T, p.L);
   if (rows * cw > INT_MAX) return GRETA_ERR_INVALID_ARG;

@@ -52,31 +52,69 @@ struct ConvParams {
 constexpr int kGroup = 4;   // tokens at a time
 constexpr int kStages = 4;  // groups in the ring
 
+// NV channels of a row for a lane that has them (n != 0), else zeros; and back.
+// (The host takes NV > 1 only where every row is whole aligned vectors: a lane
+// has all of its channels or none.)
+template <typename T, int NV>
+__device__ __forceinline__ Pack<T, NV> get_row(const T* g, int n) {
+  Pack<T, NV> r;
+  zero(r);
+  if (n != 0) r = load_part<T, NV>(g, NV, true);
+  return r;
+}
+template <typename T, int NV>
+__device__ __forceinline__ void put_row(T* g, const Pack<T, NV>& r, int n) {
+  if (n != 0) store_part<T, NV>(g, r, NV, true);
+}
+
 // A lane's part of the ring for one operand: [stage][token][lane] vectors.
 // Single elements (rows that are not whole vectors) are loaded when the group
-// is due.
+// is due. Stages are byte offsets, rows a pointer that moves on: with products
+// of token and stride a row took as many instructions for addresses as for sums.
 template <typename T, int NV>
 struct ConvRing {
-  static constexpr int kBytes = kStages * kGroup * 32 * NV * (int)sizeof(T);  // of a warp
-  Pack<T, NV>* mine;
-  const T* g;  // the lane's first channel of row 0
+  static constexpr int kRow = 32 * NV * (int)sizeof(T), kStage = kGroup * kRow;
+  static constexpr int kBytes = kStages * kStage;  // of a warp, a power of two
+  static __device__ __forceinline__ int after(int stage) { return (stage + kStage) & (kBytes - 1); }
+  const char* mine;
+  unsigned to;    // the same in the shared window
+  const T* next;  // the lane's first channel of the next row to be fetched
+  const T* g;     // ... of row 0
   long long ld;
   int n;
-
-  // Rows t .. t + 3 that are below `end`.
-  __device__ __forceinline__ void fetch(int group, int t, int end) const {
-    if (NV > 1) {
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i)
-        if (t + i < end && n == NV)
-          copy_async<NV * (int)sizeof(T)>(mine + (group % kStages * kGroup + i) * 32, g + (long long)(t + i) * ld, true);
-      copy_commit();
+  __device__ __forceinline__ ConvRing(char* s, int lane, const void* base, long long ld_, int c0, int n_, int t) {
+    mine = s + lane * (NV * (int)sizeof(T));
+    to = (unsigned)__cvta_generic_to_shared(mine);
+    g = reinterpret_cast<const T*>(base) + c0;
+    next = g + t * ld_;
+    ld = ld_;
+    n = n_;
+  }
+  // Rows t .. t + 3 that are below `end`, the next ones, into a stage.
+  __device__ __forceinline__ void fetch(int stage, int t, int end) {
+    if constexpr (NV > 1) {
+      constexpr int B = NV * (int)sizeof(T);
+      static_assert(kGroup == 4, "written out");
+      const T *r0 = next, *r1 = r0 + ld, *r2 = r1 + ld, *r3 = r2 + ld;
+      next = r3 + ld;
+      if (n == 0) return;
+      const unsigned s = to + stage;
+      if (t + kGroup <= end) {
+        copy_async_to<B, 0>(s, r0);
+        copy_async_to<B, kRow>(s, r1);
+        copy_async_to<B, 2 * kRow>(s, r2);
+        copy_async_to<B, 3 * kRow>(s, r3);
+      } else {
+        if (t < end) copy_async_to<B, 0>(s, r0);
+        if (t + 1 < end) copy_async_to<B, kRow>(s, r1);
+        if (t + 2 < end) copy_async_to<B, 2 * kRow>(s, r2);
+      }
     }
   }
   // Row t + i of the group that begins at t.
-  __device__ __forceinline__ Pack<T, NV> row(int group, int t, int i) const {
-    if (NV > 1) return load_part<T, NV>(reinterpret_cast<const T*>(mine + (group % kStages * kGroup + i) * 32), NV, true);
-    return load_part<T, NV>(g + (long long)(t + i) * ld, n, false);
+  __device__ __forceinline__ Pack<T, NV> row(int stage, int t, int i) const {
+    if constexpr (NV > 1) return load_part<T, NV>(reinterpret_cast<const T*>(mine + stage + i * kRow), NV, true);
+    return get_row<T, NV>(g + (t + i) * ld, n);
   }
 };
 // The copies of all but the last kStages - 1 groups have landed.
@@ -89,7 +127,20 @@ using Chans = f2[(NV + 1) / 2];
 template <typename T, int NV>
 __device__ __forceinline__ void widen(const Pack<T, NV>& r, Chans<NV>& o) {
 #pragma unroll
-  for (int c = 0; c < NV; c += 2) o[c / 2] = pack2(to_f(r.v[c]), c + 1 < NV ? to_f(r.v[c + 1 < NV ? c + 1 : c]) : 0.f);
+  for (int c = 0; c < NV; c += 2) {
+    if constexpr (NV % 4 == 0) {
+      if (c % 4 == 0) {
+        Pack<T, 4> four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four.v[e] = r.v[c + e];
+        const float4 v = widen4(four);
+        o[c / 2] = pack2(v.x, v.y);
+        o[c / 2 + 1] = pack2(v.z, v.w);
+      }
+    } else {
+      o[c / 2] = pack2(to_f(r.v[c]), c + 1 < NV ? to_f(r.v[c + 1 < NV ? c + 1 : c]) : 0.f);
+    }
+  }
 }
 template <typename T, int NV>
 __device__ __forceinline__ Pack<T, NV> narrow(const Chans<NV>& v) {
@@ -231,24 +282,20 @@ template <typename T, int NV>
 __device__ __forceinline__ void conv_silu(Chans<NV>& v) {
 #pragma unroll
   for (int c = 0; c < (NV + 1) / 2; ++c) {
-    float a, b;
-    unpack2(v[c], a, b);
-    v[c] = pack2(a * sigmoid_t<T>(a), NV > 1 ? b * sigmoid_t<T>(b) : 0.f);
+    v[c] = f2_mul(v[c], sigmoid2<T>(v[c]));
   }
 }
 
 // PACKED: history from and to the requests' cache slots; else zero history.
 template <typename T, int NV, int WT, bool PACKED>
-__global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
+__global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(const ConvParams p) {
   constexpr int MW = WT > 0 ? WT : -WT;
   constexpr int MH = MW > 1 ? MW - 1 : 1;
-  constexpr bool kVec = NV > 1;  // every row is whole aligned vectors (the host's choice)
   const int W = WT > 0 ? WT : p.W;
   const int H = W - 1;
   const int lane = threadIdx.x & 31;
   const int c0 = ((int)(blockIdx.x % p.nblk) * 32 + lane) * NV;
   const int n = max(0, min(NV, p.D - c0));  // 0: a lane without channels
-  const bool vec = kVec && n == NV;
   const long long first = ((long long)(blockIdx.x / p.nblk) * blockDim.y + threadIdx.y) * p.L;
   pdl_wait();
   pdl_trigger();
@@ -256,14 +303,8 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
   int t = (int)first;
   int t1 = (int)min((long long)p.q.T, first + p.L);
   const T* xg = reinterpret_cast<const T*>(p.x) + c0;
-  T* yg = reinterpret_cast<T*>(p.y) + c0;
   extern __shared__ float4 ring_smem[];
-  ConvRing<T, NV> ring;
-  ring.mine = reinterpret_cast<Pack<T, NV>*>(reinterpret_cast<char*>(ring_smem) +
-                                             threadIdx.y * ConvRing<T, NV>::kBytes) + lane;
-  ring.g = xg;
-  ring.ld = p.ldx;
-  ring.n = n;
+  using Ring = ConvRing<T, NV>;
   Chans<NV> w[MW], bias, win[MH];
   const SeqView sv(p.q, lane);
   Seg g = sv.at(t);
@@ -284,8 +325,12 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
       if (last.in && t1 > last.b && t1 - last.b < H) tend = min(last.b + H, last.e);
     }
   }
+  Ring ring(reinterpret_cast<char*>(ring_smem) + threadIdx.y * Ring::kBytes, lane, p.x, p.ldx, c0, n, t);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) ring.fetch(i, t + i * kGroup, tend);
+  for (int i = 0; i < kStages - 1; ++i) {
+    ring.fetch(i * Ring::kStage, t + i * kGroup, tend);
+    copy_commit();
+  }
   conv_weights<T, NV>(p, c0, n, W, w, bias);
   conv_zero<NV>(win);
   // inside a sequence: the inputs ahead of the run (t - H + h >= 0 where kept)
@@ -293,7 +338,7 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
 #pragma unroll
     for (int h = 0; h < MH; ++h)
       if (h >= MH - H && t - MH + h >= g.b)
-        widen<T, NV>(load_part<T, NV>(xg + (long long)(t - MH + h) * p.ldx, n, vec), win[h]);
+        widen<T, NV>(get_row<T, NV>(xg + (long long)(t - MH + h) * p.ldx, n), win[h]);
   }
   int slot = -1;
   Pack<T, NV> old[MH];  // the slot's inputs of a request that begins here
@@ -322,7 +367,7 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
 #pragma unroll
       for (int h = 0; h < MH; ++h) {
         zero(fin[h]);
-        if (h >= MH - H) fin[h] = load_part<T, NV>(xg + (long long)(g.e - MH + h) * p.ldx, n, vec);
+        if (h >= MH - H) fin[h] = get_row<T, NV>(xg + (long long)(g.e - MH + h) * p.ldx, n);
       }
       conv_store_state<T, NV, MH>(p, slot, c0, n, H, fin, WT > 1);
       slot = -1;
@@ -339,7 +384,7 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
       zero(fin[h]);
       if (h < MH - H) continue;
       if (len - MH + h >= 0) {
-        fin[h] = load_part<T, NV>(xg + (long long)(g.e - MH + h) * p.ldx, n, vec);
+        fin[h] = get_row<T, NV>(xg + (long long)(g.e - MH + h) * p.ldx, n);
       } else {
 #pragma unroll
         for (int k = 0; k < MH; ++k)
@@ -349,25 +394,32 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
     conv_store_state<T, NV, MH>(p, slot, c0, n, H, fin, WT > 1);
     slot = -1;
   };
-  auto token = [&](int at, const Pack<T, NV>& raw) {
+  T* y = reinterpret_cast<T*>(p.y) + t * (long long)p.D + c0;  // the next token's
+  auto token = [&](const Pack<T, NV>& raw) {
     Chans<NV> x, o;
     widen<T, NV>(raw, x);
     conv_pre<NV>(w, bias, win, x, W, o);
     conv_push<NV>(win, x);
     if (p.silu) conv_silu<T, NV>(o);
-    store_part<T, NV>(yg + (long long)at * p.D, narrow<T, NV>(o), n, vec);
+    put_row<T, NV>(y, narrow<T, NV>(o), n);
+    y += p.D;
   };
 
-  for (int group = 0; t < tend; t += kGroup, ++group) {
+  // groups from `lo` + 1 up to `hi` lie in g behind its first and ahead of its
+  // last token
+  int lo = g.in ? g.b : INT_MAX, hi = min(g.e - 1, tend);
+  int get = 0, put = (kStages - 1) * Ring::kStage;
+  for (; t < tend; t += kGroup, get = Ring::after(get), put = Ring::after(put)) {
     if (NV > 1) ring_wait();
     // (into the stage of the group before this one)
-    ring.fetch(group + kStages - 1, t + (kStages - 1) * kGroup, tend);
-    if (g.in && t > g.b && t + kGroup <= min(g.e - 1, tend)) {
+    ring.fetch(put, t + (kStages - 1) * kGroup, tend);
+    if (NV > 1) copy_commit();
+    if (t > lo && t + kGroup <= hi) {
       Pack<T, NV> x[kGroup];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) x[i] = ring.row(group, t, i);
+      for (int i = 0; i < kGroup; ++i) x[i] = ring.row(get, t, i);
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) token(t + i, x[i]);
+      for (int i = 0; i < kGroup; ++i) token(x[i]);
     } else {
 #pragma unroll 1
       for (int i = 0; i < kGroup && t + i < tend; ++i) {
@@ -375,14 +427,17 @@ __global__ void __launch_bounds__(128) ssm_conv_fwd_kernel(const ConvParams p) {
         if (ti >= g.e) g = sv.next(g);
         if (g.in) {
           if (ti == g.b) begin();
-          token(ti, ring.row(group, t, i));
+          token(ring.row(get, t, i));
           if (ti + 1 == g.e) finish();
-        } else if (p.zero_rest) {
+        } else {
           Pack<T, NV> z;
           zero(z);
-          store_part<T, NV>(yg + (long long)ti * p.D, z, n, vec);
+          if (p.zero_rest) put_row<T, NV>(y, z, n);
+          y += p.D;
         }
       }
+      lo = g.in ? g.b : INT_MAX;
+      hi = min(g.e - 1, tend);
     }
   }
 }
@@ -478,7 +533,7 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
 // partial sums per block goes to `part`, which ssm_conv_reduce_kernel adds in
 // a fixed order: the same call gives the same bits.
 template <typename T, int NV, int WT>
-__global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
+__global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_bwd_kernel(const ConvParams p) {
   constexpr int MW = WT > 0 ? WT : -WT;
   constexpr int MH = MW > 1 ? MW - 1 : 1;
   constexpr int NC = (NV + 1) / 2;
@@ -489,7 +544,6 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
   const int cb = (int)(blockIdx.x % p.nblk) * 32 * NV;
   const int c0 = cb + lane * NV;
   const int n = max(0, min(NV, p.D - c0));
-  const bool vec = NV > 1 && n == NV;
   const long long first = ((long long)(blockIdx.x / p.nblk) * blockDim.y + threadIdx.y) * p.L;
   pdl_wait();
   pdl_trigger();
@@ -501,32 +555,18 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
     const int t0 = (int)first;
     const int t1 = (int)min((long long)p.q.T, first + p.L);
     const T* xg = reinterpret_cast<const T*>(p.x) + c0;
-    T* dxg = reinterpret_cast<T*>(p.dx) + c0;
     const int t2 = t1 + MW - 1;  // one behind the token that completes the run's last
     const int tin = min(t2, p.q.T);
-    ConvRing<T, NV> rx, rd;
-    char* mine = reinterpret_cast<char*>(red) + threadIdx.y * 2 * ConvRing<T, NV>::kBytes;
-    rx.mine = reinterpret_cast<Pack<T, NV>*>(mine) + lane;
-    rd.mine = reinterpret_cast<Pack<T, NV>*>(mine + ConvRing<T, NV>::kBytes) + lane;
-    rx.g = xg;
-    rd.g = reinterpret_cast<const T*>(p.dout) + c0;
-    rx.ld = p.ldx;
-    rd.ld = p.D;
-    rx.n = rd.n = n;
-    auto fetch = [&](int group, int t) {  // both operands' rows are one group of copies
-      if (NV > 1) {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i)
-          if (t + i < tin && n == NV) {
-            const int at = (group % kStages * kGroup + i) * 32;
-            copy_async<NV * (int)sizeof(T)>(rx.mine + at, rx.g + (long long)(t + i) * rx.ld, true);
-            copy_async<NV * (int)sizeof(T)>(rd.mine + at, rd.g + (long long)(t + i) * rd.ld, true);
-          }
-        copy_commit();
-      }
+    using Ring = ConvRing<T, NV>;
+    char* mine = reinterpret_cast<char*>(red) + threadIdx.y * 2 * Ring::kBytes;
+    Ring rx(mine, lane, p.x, p.ldx, c0, n, t0), rd(mine + Ring::kBytes, lane, p.dout, p.D, c0, n, t0);
+    auto fetch = [&](int stage, int t) {  // both operands' rows are one group of copies
+      rx.fetch(stage, t, tin);
+      rd.fetch(stage, t, tin);
+      if (NV > 1) copy_commit();
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(i, t0 + i * kGroup);
+    for (int i = 0; i < kStages - 1; ++i) fetch(i * Ring::kStage, t0 + i * kGroup);
     Chans<NV> w[MW], bias, win[MH], acc[MW];
     conv_weights<T, NV>(p, c0, n, W, w, bias);
     conv_zero<NV>(win);
@@ -537,7 +577,7 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
 #pragma unroll
       for (int h = 0; h < MH; ++h)
         if (h >= MH - H && t0 - MH + h >= g.b)
-          widen<T, NV>(load_part<T, NV>(xg + (long long)(t0 - MH + h) * p.ldx, n, vec), win[h]);
+          widen<T, NV>(get_row<T, NV>(xg + (long long)(t0 - MH + h) * p.ldx, n), win[h]);
     }
     // Token ti of the sequence g: its dpre, what it adds, and the window. `all`:
     // a token of the run with all its W inputs in the sequence.
@@ -551,14 +591,8 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
         conv_pre<NV>(w, bias, win, x, W, pre);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          float v[2], o[2] = {0.f, 0.f};
-          unpack2(pre[c], v[0], v[1]);
-#pragma unroll
-          for (int i = 0; i < (NV > 1 ? 2 : 1); ++i) {
-            const float s = sigmoid_t<T>(v[i]);
-            o[i] = s * fmaf(v[i], 1.f - s, 1.f);
-          }
-          d[c] = f2_mul(d[c], pack2(o[0], o[1]));
+          const f2 one = pack2(1.f, 1.f), s = sigmoid2<T>(pre[c]);
+          d[c] = f2_mul(d[c], f2_mul(s, f2_fma(pre[c], f2_fma(s, pack2(-1.f, -1.f), one), one)));
         }
       }
       const int pos = ti - g.b;
@@ -580,9 +614,11 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
       }
       conv_push<NV>(win, x);
     };
-    // dx of token `to` is complete: store it and move the sums on
-    auto complete = [&](int to, bool store) {
-      if (store) store_part<T, NV>(dxg + (long long)to * p.D, narrow<T, NV>(acc[0]), n, vec);
+    // dx of the next token is complete: store it and move the sums on
+    T* dx = reinterpret_cast<T*>(p.dx) + (t0 - (MW - 1)) * (long long)p.D + c0;
+    auto complete = [&](bool store) {
+      if (store) put_row<T, NV>(dx, narrow<T, NV>(acc[0]), n);
+      dx += p.D;
 #pragma unroll
       for (int k = 0; k < MW; ++k)
 #pragma unroll
@@ -590,21 +626,25 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
           acc[k][c] = k + 1 < MW ? acc[k + 1 < MW ? k + 1 : k][c] : 0ull;
         }
     };
-    int group = 0;
-    for (int t = t0; t < t2; t += kGroup, ++group) {
+    // groups from `lo` up to `hi` lie in g and in the run, with all their inputs,
+    // and complete tokens of the run
+    auto from = [&] { return g.in ? max(g.b + H, t0 + MW - 1) : INT_MAX; };
+    int lo = from(), hi = min(g.e, t1);
+    int get = 0, put = (kStages - 1) * Ring::kStage;
+    for (int t = t0; t < t2; t += kGroup, get = Ring::after(get), put = Ring::after(put)) {
       if (NV > 1) ring_wait();
-      fetch(group + kStages - 1, t + (kStages - 1) * kGroup);
-      if (g.in && t + kGroup <= min(g.e, t1) && t - g.b >= H && t - (MW - 1) >= t0) {
+      fetch(put, t + (kStages - 1) * kGroup);
+      if (t >= lo && t + kGroup <= hi) {
         Pack<T, NV> x[kGroup], dy[kGroup];
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
-          x[i] = rx.row(group, t, i);
-          dy[i] = rd.row(group, t, i);
+          x[i] = rx.row(get, t, i);
+          dy[i] = rd.row(get, t, i);
         }
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
           token(t + i, x[i], dy[i], std::true_type());
-          complete(t + i - (MW - 1), true);
+          complete(true);
         }
       } else {
 #pragma unroll 1
@@ -613,10 +653,12 @@ __global__ void __launch_bounds__(128) ssm_conv_bwd_kernel(const ConvParams p) {
           if (ti < tin && ti >= g.e) g = sv.next(g);
           if (ti < tin && g.in) {
             if (ti == g.b) conv_zero<NV>(win);
-            token(ti, rx.row(group, t, i), rd.row(group, t, i), std::false_type());
+            token(ti, rx.row(get, t, i), rd.row(get, t, i), std::false_type());
           }
-          complete(ti - (MW - 1), ti - (MW - 1) >= t0 && ti - (MW - 1) < t1);
+          complete(ti - (MW - 1) >= t0 && ti - (MW - 1) < t1);
         }
+        lo = from();
+        hi = min(g.e, t1);
       }
     }
   }
