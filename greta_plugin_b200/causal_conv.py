@@ -76,14 +76,15 @@ def _bias(bias, dtype):
 
 
 class CausalConv1dFunction(torch.autograd.Function):
-    """x [T, D] (rows may be strided), weight [W, D], bias [D] or None."""
+    """x [1, T, D] (rows may be strided), weight [W, D], bias [D] or None. (The
+    views to [T, D] are made in here: outside they would be nodes of their own.)"""
 
     @staticmethod
     def forward(ctx, x, weight, bias, cu_seqlens, silu):
-        x, ldx = channel_rows(x)
+        x, ldx = channel_rows(x.squeeze(0))
         T, D = x.shape
         w, b = _as_type(weight, x.dtype), _bias(bias, x.dtype)
-        y = torch.empty(T, D, dtype=x.dtype, device=x.device)
+        y = torch.empty(1, T, D, dtype=x.dtype, device=x.device)
         cu, cu64, nseq = _cu(cu_seqlens, x.device)
         p = _capi.addr
         _capi.call("greta_ssm_conv_fwd", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(y), p(cu), cu64,
@@ -101,7 +102,7 @@ class CausalConv1dFunction(torch.autograd.Function):
         w, b = _as_type(weight, dt), _bias(bias, dt)
         (T, D), W = x.shape, w.shape[0]
         dout = _as_type(dout, dt).contiguous()
-        dx = torch.empty(T, D, dtype=dt, device=dev)
+        dx = torch.empty(1, T, D, dtype=dt, device=dev)
         dw = torch.empty(W, D, dtype=dt, device=dev)
         db = None if b is None else torch.empty(D, dtype=dt, device=dev)
         ws = torch.empty(_capi.lib().greta_ssm_conv_bwd_workspace(T, D, W), dtype=torch.uint8, device=dev)
@@ -132,8 +133,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise ValueError("causal_conv1d requires CUDA tensors")
     if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
         raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
-    # squeeze, not x[0], whose gradient would be copied into zeros
-    return CausalConv1dFunction.apply(x.squeeze(0), weight, bias, cu_seqlens, silu).unsqueeze(0)
+    return CausalConv1dFunction.apply(x, weight, bias, cu_seqlens, silu)
 
 
 def _as_meta(t, x, dtype):

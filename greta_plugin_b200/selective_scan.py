@@ -37,15 +37,16 @@ SAVE_EVERY = 8  # tokens per saved state
 
 
 def _check(u, delta, A, B, C, skip, gate, delta_bias):
-    """Shapes, types and devices of the operands ([T, D] rows); (T, D, N, F)."""
+    """Shapes, types and devices of the operands ([T, D] rows, with or without a
+    leading 1); (T, D, N, F)."""
     rows = u.shape
-    T, D = rows
+    T, D = rows[-2:]
     dt = u.dtype
     _capi.dtype_code(u)
     if delta.shape != rows:
-        raise ValueError(f"delta shape {tuple(delta.shape)} must match u's {(T, D)}")
+        raise ValueError(f"delta shape {tuple(delta.shape)} must match u's {tuple(rows)}")
     if gate is not None and gate.shape != rows:
-        raise ValueError(f"gate shape {tuple(gate.shape)} must match u's {(T, D)}")
+        raise ValueError(f"gate shape {tuple(gate.shape)} must match u's {tuple(rows)}")
     if A.dim() != 2 or A.shape[0] != D:
         raise ValueError(f"A must be [{D}, N], got {tuple(A.shape)}")
     N = A.shape[1]
@@ -117,30 +118,26 @@ def _workspace(kind, device, *sizes):
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
-def _scan_forward(u, args, T, D, N, F, cu_seqlens, softplus, saved):
-    dev = u.device
-    out = torch.empty(T, D, dtype=u.dtype, device=dev)
-    cu, cu64, nseq = _cu(cu_seqlens, dev)
-    ranges = _capi.token_ranges()
-    ws, n = _workspace("fwd", dev, nseq, T, D, N, F, ranges)
-    p = _capi.addr
-    _capi.call("greta_ssm_scan_fwd", u, *args, p(out), p(saved), p(cu), cu64, nseq, T, D, N, F, int(softplus), ranges,
-               p(ws), n)
-    return out
-
-
 class SelectiveScanFunction(torch.autograd.Function):
-    """u, delta, gate [T, D]; A [D, N]; B, C [T, F, N]; skip, delta_bias [D]."""
+    """u, delta, gate [1, T, D]; A [D, N]; B, C [T, F, N]; skip, delta_bias [D].
+    (The views to [T, D] are made in here: outside they would be nodes of their
+    own.)"""
 
     @staticmethod
     def forward(ctx, u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, softplus):
+        u, delta, gate = u.squeeze(0), delta.squeeze(0), None if gate is None else gate.squeeze(0)
         (T, D), (_, F, N) = u.shape, B.shape
         keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
         saved = None
         if any(ctx.needs_input_grad):
             saved = torch.empty(T // SAVE_EVERY + 1, D, N, dtype=torch.float32, device=u.device)
-        cu, _, _ = _cu(cu_seqlens, u.device)
-        out = _scan_forward(u, args, T, D, N, F, cu, softplus, saved)
+        cu, cu64, nseq = _cu(cu_seqlens, u.device)
+        out = torch.empty(1, T, D, dtype=u.dtype, device=u.device)
+        ranges = _capi.token_ranges()
+        ws, n = _workspace("fwd", u.device, nseq, T, D, N, F, ranges)
+        p = _capi.addr
+        _capi.call("greta_ssm_scan_fwd", u, *args, p(out), p(saved), p(cu), cu64, nseq, T, D, N, F, int(softplus),
+                   ranges, p(ws), n)
         ctx.save_for_backward(u, delta, A, B, C, skip, gate, delta_bias, cu, saved)
         ctx.softplus = softplus
         return out
@@ -153,8 +150,8 @@ class SelectiveScanFunction(torch.autograd.Function):
         keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
         dev, dt, f32 = u.device, u.dtype, torch.float32
         dout = (dout if dout.dtype == dt else dout.to(dt)).contiguous()
-        du, ddelta = torch.empty(T, D, dtype=dt, device=dev), torch.empty(T, D, dtype=dt, device=dev)
-        dgate = None if gate is None else torch.empty(T, D, dtype=dt, device=dev)
+        du, ddelta = torch.empty(1, T, D, dtype=dt, device=dev), torch.empty(1, T, D, dtype=dt, device=dev)
+        dgate = None if gate is None else torch.empty(1, T, D, dtype=dt, device=dev)
         dB, dC = torch.empty(T, F, N, dtype=dt, device=dev), torch.empty(T, F, N, dtype=dt, device=dev)
         dA = torch.empty(D, N, dtype=f32, device=dev)
         dskip = None if skip is None else torch.empty(D, dtype=f32, device=dev)
@@ -186,18 +183,12 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     """
     if u.dim() != 3 or u.shape[0] != 1:
         raise ValueError(f"u must be [1, T, D], got {tuple(u.shape)}")
-    for name, t in (("delta", delta), ("gate", gate)):
-        if t is not None and tuple(t.shape) != tuple(u.shape):
-            raise ValueError(f"{name} shape {tuple(t.shape)} must match u's {tuple(u.shape)}")
-    # squeeze, not u[0], whose gradient would be copied into zeros
-    u, delta, gate = u.squeeze(0), delta.squeeze(0), None if gate is None else gate.squeeze(0)
     _check(u, delta, A, B, C, skip, gate, delta_bias)
     if not u.is_cuda:
         raise ValueError("selective_scan requires CUDA tensors")
     if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
         raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
-    return SelectiveScanFunction.apply(u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens,
-                                       delta_softplus).unsqueeze(0)
+    return SelectiveScanFunction.apply(u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, delta_softplus)
 
 
 def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has_initial, delta_softplus, out, flags):
