@@ -124,12 +124,12 @@ class SelectiveScanFunction(torch.autograd.Function):
     own.)"""
 
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, softplus):
+    def forward(ctx, u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, softplus, keep_states):
         u, delta, gate = u.squeeze(0), delta.squeeze(0), None if gate is None else gate.squeeze(0)
         (T, D), (_, F, N) = u.shape, B.shape
         keep, args = _operands(u, delta, A, B, C, skip, gate, delta_bias)
         saved = None
-        if any(ctx.needs_input_grad):
+        if keep_states and any(ctx.needs_input_grad):
             saved = torch.empty(T // SAVE_EVERY + 1, D, N, dtype=torch.float32, device=u.device)
         cu, cu64, nseq = _cu(cu_seqlens, u.device)
         out = torch.empty(1, T, D, dtype=u.dtype, device=u.device)
@@ -163,7 +163,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         _capi.call("greta_ssm_scan_bwd", u, *args, p(saved), p(dout), p(du), p(ddelta), p(dgate), p(dB), p(dC), p(dA),
                    p(dskip), p(dbias), p(cu), cu64, nseq, T, D, N, F, int(ctx.softplus), ranges, p(ws), n)
         like = lambda g, t: g if g is None or g.dtype == t.dtype else g.to(t.dtype)  # noqa: E731
-        return (du, ddelta, like(dA, A), dB, dC, like(dskip, skip), dgate, like(dbias, delta_bias), None, None)
+        return (du, ddelta, like(dA, A), dB, dC, like(dskip, skip), dgate, like(dbias, delta_bias), None, None, None)
 
 
 @torch.compiler.disable(recursive=True)
@@ -188,7 +188,9 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         raise ValueError("selective_scan requires CUDA tensors")
     if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
         raise ValueError(f"cu_seqlens must be [N + 1], got {tuple(cu_seqlens.shape)}")
-    return SelectiveScanFunction.apply(u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, delta_softplus)
+    # (inside the node gradients are always off, and needs_input_grad is set without them too)
+    return SelectiveScanFunction.apply(u, delta, A, B, C, skip, gate, delta_bias, cu_seqlens, delta_softplus,
+                                       torch.is_grad_enabled())
 
 
 def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has_initial, delta_softplus, out, flags):

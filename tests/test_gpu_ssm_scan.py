@@ -256,6 +256,22 @@ def test_no_gradient_keeps_no_states():
     assert not out.requires_grad
 
 
+def test_no_grad_block_makes_no_states():
+    """Parameters that take gradients, under no_grad: the states (2 MB) are not
+    even made."""
+    from greta_plugin_b200 import selective_scan
+
+    s, _ = make(4096, 64, 16, 1, torch.bfloat16, 1)
+    A = s["A"].clone().requires_grad_(True)
+    selective_scan(s["u"][None], s["delta"][None], s["A"], s["B"], s["C"])
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        out = selective_scan(s["u"][None], s["delta"][None], A, s["B"], s["C"])
+    assert torch.cuda.max_memory_allocated() - before < out.numel() * 2 + 513 * 64 * 16 * 4
+    assert not out.requires_grad
+
+
 def test_train_captured():
     """Forward and backward in one captured graph, replayed on new inputs."""
     s, dout = make(150, 64, 16, 1, torch.bfloat16, 11)
