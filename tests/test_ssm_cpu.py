@@ -333,6 +333,18 @@ def test_packed_selective_scan_refuses(kw, match):
         packed_selective_scan(**args)
 
 
+def test_expanded_state_is_refused():
+    """A state that several slots or channels share cannot be updated in place."""
+    from greta_plugin_b200.causal_conv import packed_metadata
+
+    meta = (_ints(0, 2, 5), _ints(0, 1), _ints(1, 1, dtype=torch.int8))
+    for state in (_t(1, 8, 3).expand(4, 8, 3), _t(4, 1, 3).expand(4, 8, 3)):
+        with pytest.raises(ValueError, match="expanded"):
+            packed_metadata(_t(5, 8), state, *meta)
+    for state in (_t(4, 8, 3), _t(1, 8, 3).expand(1, 8, 3), _t(4, 8, 0)):
+        packed_metadata(_t(5, 8), state, *meta)
+
+
 @pytest.mark.parametrize("kw, match", [
     (dict(query_lens=_ints(1, 2, dtype=torch.int64)), "query_lens"),
     (dict(context_lens=_ints(1)), "context_lens has"),
