@@ -45,7 +45,7 @@ def launch_options(kernel="auto", block_x=0, block_y=0, tokens=0, wait_limit_log
     (tests and tuning sweeps): the kernel family ("auto", "register", "rows"
     for the row-streaming bulk-copy kernels), the register kernels' CTA
     shape, the pipeline wait bound, the row-streaming kernels' channel slice,
-    token ranges and stage-ring budget. They
+    token ranges (also the selective scan's) and stage-ring budget. They
     travel with each call as its options argument; nothing is set in the
     library."""
     o = Options(ctypes.sizeof(Options), KERNELS[kernel], block_x, block_y, tokens, wait_limit_log2,
