@@ -220,14 +220,18 @@ struct BwdSmem {
   static constexpr int CHW = Lanes<LN, kBwdChans>::CHW, NP = Lanes<LN, kBwdChans>::NP, V = TileVecs<CHW>::V;
   static constexpr int kRow = kTile * CHW * (int)sizeof(T);  // a tile of an operand
   static constexpr int kRowF = kTile * CHW * 4;
+  // fp32: dy, slopes and dout SiLU' take the places of dout, delta and gate, whose
+  // values they are made of (with places of their own a third CTA had no room)
+  static constexpr bool kInPlace = sizeof(T) == 4;
   static constexpr int kDl = 0;                       // (dt, dt u)
   static constexpr int kDy = kDl + 2 * kRowF;         // dy
-  static constexpr int kSlope = kDy + kRowF;          // d(dt) / d(raw step)
-  static constexpr int kGk = kSlope + kRowF;          // dout SiLU'(gate)
-  static constexpr int kY = kGk + kRowF;              // sum C h
+  static constexpr int kSlope = kDy + (kInPlace ? 0 : kRowF);  // d(dt) / d(raw step)
+  static constexpr int kGk = kSlope + (kInPlace ? 0 : kRowF);  // dout SiLU'(gate)
+  static constexpr int kY = kGk + (kInPlace ? 0 : kRowF);      // sum C h
   static constexpr int kPair = kY + kRowF;            // (sum kept A2, sum g B)
-  static constexpr int kCols = kPair + 2 * kRowF;     // [bias | skip][lane] V floats
-  static constexpr int kSum = kCols + 2 * 32 * V * 4;  // [dskip | d(delta_bias)][lane] V floats
+  static constexpr int kCols = kPair + 2 * kRowF;     // [bias | skip][CHW]; 16-bit types: a copy per lane (1606 us, not 1623)
+  static constexpr int kColBytes = kInPlace ? (CHW * 4 + 15) / 16 * 16 : 32 * V * 4;
+  static constexpr int kSum = kCols + 2 * kColBytes;  // [dskip | d(delta_bias)][lane] V floats
   static constexpr int kPart = kSum + 2 * 32 * V * 4;  // [token][dB | dC][lane] float4
   static constexpr int kStage0 = kPart + kTile * 2 * 32 * 16;
   static constexpr int kStage = 4 * kRow + 32 * kBwdChans * 16;  // u, delta, gate, dout; saved states
@@ -267,12 +271,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   char* base = reinterpret_cast<char*>(smem4);
   char* mine = base + 2 * S::kBC + warp * S::kWarp;
   float4* dl = reinterpret_cast<float4*>(mine + S::kDl);
-  float* dys = reinterpret_cast<float*>(mine + S::kDy);
-  float* slope = reinterpret_cast<float*>(mine + S::kSlope);
-  float* gk = reinterpret_cast<float*>(mine + S::kGk);
   float* ys = reinterpret_cast<float*>(mine + S::kY);
   float2* pair = reinterpret_cast<float2*>(mine + S::kPair);
-  float* cols = reinterpret_cast<float*>(mine + S::kCols) + lane * V;
+  float* cols = reinterpret_cast<float*>(mine + S::kCols) + (S::kInPlace ? TV::chan(lane) : lane * V);
   float* sums = reinterpret_cast<float*>(mine + S::kSum) + lane * V;
   float4* part = reinterpret_cast<float4*>(mine + S::kPart) + lane;
   auto stage = [&](int s, int op) {  // u, delta, gate, dout
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     load_column<V>(p.skip, l.c0 + TV::chan(lane), l.nch - TV::chan(lane), v);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      cols[32 * V + e] = v[e];
+      cols[S::kColBytes / 4 + e] = v[e];
       sums[e] = sums[32 * V + e] = 0.f;
     }
   }
@@ -374,6 +375,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
     const int ta = max(t0, tile0), tb = min(t1, tile0 + kTile);
     const TileSeqs q = tile_seqs(sv, tile0, ta, tb, g);
     copy_wait();
+    float* dys = S::kInPlace ? reinterpret_cast<float*>(stage(cur, 3)) : reinterpret_cast<float*>(mine + S::kDy);
+    float* slope = S::kInPlace ? reinterpret_cast<float*>(stage(cur, 1)) : reinterpret_cast<float*>(mine + S::kSlope);
+    float* gk = S::kInPlace ? reinterpret_cast<float*>(stage(cur, 2)) : reinterpret_cast<float*>(mine + S::kGk);
     // B and C widened once for the CTA (each thread what it copied itself)
     const float* bc = reinterpret_cast<const float*>(base + cur * S::kBC);
     if (sizeof(T) != 4) {
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
       const bool vec = p.vec && n >= V, in = (q.live >> r) & 1;
       const Pack<T, V> u = tile_vec<T, CHW>(stage(cur, 0), k, lane);
       const Pack<float, V> sl = load_part<float, V>(slope + at, V, true), dy = load_part<float, V>(dys + at, V, true),
-                           skip = load_part<float, V>(cols + 32 * V, V, true);
+                           skip = load_part<float, V>(cols + S::kColBytes / 4, V, true);
       const Pack<float, 2 * V> sp = load_part<float, 2 * V>(reinterpret_cast<const float*>(pair + at), 2 * V, true);
       Pack<float, V> s0 = load_part<float, V>(sums, V, true), s1 = load_part<float, V>(sums + 32 * V, V, true);
       Pack<T, V> du, dd, dz;
