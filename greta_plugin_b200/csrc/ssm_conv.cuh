@@ -14,7 +14,8 @@
 // what is on its way: with loads into registers the compiler kept two to four
 // rows in flight, half of what HBM needs). Four tokens that lie inside one
 // sequence are computed without a test between them, so that the window moves
-// by renaming registers.
+// by renaming registers. 16288 x 4096, 4 taps, bf16: 53 us, 5.0 TB/s; 898 tokens
+// of 8 requests 9.1 us.
 // W is a template parameter for 2, 3 and 4 (the kernel sizes in use); WT = -8
 // and -16 take any W up to that, with narrower vectors for their windows:
 // filters and window are aligned to the current token's end (index MW-1 and
@@ -445,7 +446,8 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
 // Batches of (nearly) one token per request: a warp has the channels of one
 // request and walks its tokens, with filters and window in the element type (a
 // third of the registers, so that all of a step's warps run at once) and with
-// the metadata, the first token's row and the filters asked for together.
+// the metadata, the first token's row and the filters asked for together: three
+// latencies in a row. 256 requests of 4096 channels, 4 taps, bf16: 7.6 us.
 template <typename T, int NV, int WT>
 __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p) {
   constexpr int MW = WT > 0 ? WT : -WT;
@@ -531,7 +533,10 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
 // the sum of token t-W+1 (of t-MW+1 with a runtime W) is then complete. dw and dbias of the run stay in
 // registers, the block's four runs are added in shared memory, and one row of
 // partial sums per block goes to `part`, which ssm_conv_reduce_kernel adds in
-// a fixed order: the same call gives the same bits.
+// a fixed order: the same call gives the same bits. Four channels a thread (the
+// sums of eight do not fit 128 registers): some 100 instructions a token for 12
+// elements read and written, so issue and fp32 pipe (half of each at 16 warps an
+// SM) are ahead of HBM: 16288 x 4096, 4 taps, bf16 100 us, 4.0 TB/s.
 template <typename T, int NV, int WT>
 __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_bwd_kernel(const ConvParams p) {
   constexpr int MW = WT > 0 ? WT : -WT;
