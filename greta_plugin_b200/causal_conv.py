@@ -150,7 +150,7 @@ def packed_metadata(x, state, starts, slots, has_initial):
         raise ValueError(f"starts must hold one offset more than slots ({n}) and has_initial as many, got "
                          f"{starts.numel()} and {has_initial.numel()}")
     same_device("x", x, state=state)
-    if 0 in state.stride() and any(st == 0 and size > 1 for st, size in zip(state.stride(), state.shape)):
+    if 0 in state.stride() and state.numel() and any(st == 0 and size > 1 for st, size in zip(state.stride(), state.shape)):
         raise ValueError("state is updated in place and must not be expanded")
     return (_as_meta(starts, x, torch.int32), _as_meta(slots, x, torch.int32),
             _as_meta(has_initial, x, torch.int8))

@@ -341,7 +341,7 @@ def test_expanded_state_is_refused():
     for state in (_t(1, 8, 3).expand(4, 8, 3), _t(4, 1, 3).expand(4, 8, 3)):
         with pytest.raises(ValueError, match="expanded"):
             packed_metadata(_t(5, 8), state, *meta)
-    for state in (_t(4, 8, 3), _t(1, 8, 3).expand(1, 8, 3), _t(4, 8, 0)):
+    for state in (_t(4, 8, 3), _t(1, 8, 3).expand(1, 8, 3), _t(4, 8, 0), _t(1, 8, 0).expand(4, 8, 0)):
         packed_metadata(_t(5, 8), state, *meta)
 
 
