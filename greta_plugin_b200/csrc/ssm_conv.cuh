@@ -158,30 +158,25 @@ __device__ __forceinline__ Pack<T, NV> narrow(const Chans<NV>& v) {
 
 // The filters (tap k at index MW - W + k) and the bias of this thread's channels.
 template <typename T, int NV, int MW>
-__device__ __forceinline__ void conv_weights(const ConvParams& p, int c0, int n, int W, Chans<NV> (&w)[MW],
-                                             Chans<NV>& bias) {
+__device__ __forceinline__ void conv_weights(const ConvParams& p, int c0, int n, int W, Pack<T, NV> (&w)[MW],
+                                             float (&bias)[NV]) {
   const T* wg = reinterpret_cast<const T*>(p.w);
 #pragma unroll
   for (int k = 0; k < MW; ++k) {
-    Pack<T, NV> r;
-    zero(r);
+    zero(w[k]);
     const int tap = k - (MW - W);
-    if (tap >= 0) {
-      if (p.vec_w) {
-        r = load_part<T, NV>(wg + (long long)tap * p.sw_k + c0, n, n == NV);
-      } else {
+    if (tap < 0) continue;
+    if (p.vec_w) {
+      w[k] = load_part<T, NV>(wg + (long long)tap * p.sw_k + c0, n, n == NV);
+    } else {
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
-          if (c < n) r.v[c] = wg[(long long)tap * p.sw_k + (long long)(c0 + c) * p.sw_d];
-      }
+      for (int c = 0; c < NV; ++c)
+        if (c < n) w[k].v[c] = wg[(long long)tap * p.sw_k + (long long)(c0 + c) * p.sw_d];
     }
-    widen<T, NV>(r, w[k]);
   }
-  Pack<T, NV> r;
 #pragma unroll
   for (int c = 0; c < NV; ++c)
-    r.v[c] = p.bias != nullptr && c < n ? reinterpret_cast<const T*>(p.bias)[c0 + c] : from_f<T>(0.f);
-  widen<T, NV>(r, bias);
+    bias[c] = p.bias != nullptr && c < n ? to_f(reinterpret_cast<const T*>(p.bias)[c0 + c]) : 0.f;
 }
 
 // The slot's H = W-1 inputs of this thread's channels, oldest first, at the end
@@ -263,6 +258,32 @@ __device__ __forceinline__ void conv_pre(const Chans<NV> (&w)[MW], const Chans<N
   }
 }
 
+// The same from operands in the element type (fma_io: exact products, fp32 sums),
+// with SiLU, rounded to the output.
+template <typename T, int NV, int MW, int MH>
+__device__ __forceinline__ Pack<T, NV> conv_out(const Pack<T, NV> (&w)[MW], const float (&bias)[NV],
+                                                const Pack<T, NV> (&win)[MH], const Pack<T, NV>& x, int W, bool silu) {
+  float s[NV];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    s[c] = bias[c];
+#pragma unroll
+    for (int k = 0; k < MW; ++k) {
+      if (k == MW - 1)
+        s[c] = fma_io(w[k].v[c], x.v[c], s[c]);
+      else if (k >= MW - W)
+        s[c] = fma_io(w[k].v[c], win[k < MH ? k : 0].v[c], s[c]);
+    }
+  }
+  Chans<NV> o;
+#pragma unroll
+  for (int c = 0; c < NV; c += 2) {
+    o[c / 2] = pack2(s[c], c + 1 < NV ? s[c + 1 < NV ? c + 1 : c] : 0.f);
+    if (silu) o[c / 2] = f2_mul(o[c / 2], sigmoid2<T>(o[c / 2]));
+  }
+  return narrow<T, NV>(o);
+}
+
 template <int NV, int MH>
 __device__ __forceinline__ void conv_push(Chans<NV> (&win)[MH], const Chans<NV>& x) {
 #pragma unroll
@@ -277,14 +298,6 @@ __device__ __forceinline__ void conv_zero(Chans<NV> (&win)[MH]) {
   for (int h = 0; h < MH; ++h)
 #pragma unroll
     for (int c = 0; c < (NV + 1) / 2; ++c) win[h][c] = 0ull;
-}
-
-template <typename T, int NV>
-__device__ __forceinline__ void conv_silu(Chans<NV>& v) {
-#pragma unroll
-  for (int c = 0; c < (NV + 1) / 2; ++c) {
-    v[c] = f2_mul(v[c], sigmoid2<T>(v[c]));
-  }
 }
 
 // PACKED: history from and to the requests' cache slots; else zero history.
@@ -306,7 +319,9 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
   const T* xg = reinterpret_cast<const T*>(p.x) + c0;
   extern __shared__ float4 ring_smem[];
   using Ring = ConvRing<T, NV>;
-  Chans<NV> w[MW], bias, win[MH];
+  // filters and window in the element type: nothing to widen or to narrow
+  Pack<T, NV> w[MW], win[MH];
+  float bias[NV];
   const SeqView sv(p.q, lane);
   Seg g = sv.at(t);
 
@@ -333,13 +348,17 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
     copy_commit();
   }
   conv_weights<T, NV>(p, c0, n, W, w, bias);
-  conv_zero<NV>(win);
+  auto forget = [&] {
+#pragma unroll
+    for (int h = 0; h < MH; ++h) zero(win[h]);
+  };
+  forget();
   // inside a sequence: the inputs ahead of the run (t - H + h >= 0 where kept)
   if (g.in && t > g.b) {
 #pragma unroll
     for (int h = 0; h < MH; ++h)
       if (h >= MH - H && t - MH + h >= g.b)
-        widen<T, NV>(get_row<T, NV>(xg + (long long)(t - MH + h) * p.ldx, n), win[h]);
+        win[h] = get_row<T, NV>(xg + (long long)(t - MH + h) * p.ldx, n);
   }
   int slot = -1;
   Pack<T, NV> old[MH];  // the slot's inputs of a request that begins here
@@ -347,7 +366,7 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
   for (int h = 0; h < MH; ++h) zero(old[h]);
   // the first token of sequence g
   auto begin = [&] {
-    conv_zero<NV>(win);
+    forget();
     slot = -1;
     if (!PACKED || p.state == nullptr) return;
     const int raw = p.slots[g.s], initial = p.initial[g.s];
@@ -359,7 +378,7 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
       conv_load_state<T, NV, MH>(p, slot, c0, n, H, old, WT > 1);
 #pragma unroll
       for (int h = 0; h < MH; ++h)
-        if (h >= MH - H) widen<T, NV>(old[h], win[h]);
+        if (h >= MH - H) win[h] = old[h];
     }
     if (slot >= 0 && g.e > tend) {
       // the request ends in a later run: its last W-1 inputs (it has more
@@ -397,12 +416,9 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
   };
   T* y = reinterpret_cast<T*>(p.y) + t * (long long)p.D + c0;  // the next token's
   auto token = [&](const Pack<T, NV>& raw) {
-    Chans<NV> x, o;
-    widen<T, NV>(raw, x);
-    conv_pre<NV>(w, bias, win, x, W, o);
-    conv_push<NV>(win, x);
-    if (p.silu) conv_silu<T, NV>(o);
-    put_row<T, NV>(y, narrow<T, NV>(o), n);
+    put_row<T, NV>(y, conv_out<T, NV>(w, bias, win, raw, W, p.silu), n);
+#pragma unroll
+    for (int h = 0; h < MH; ++h) win[h] = h + 1 < MH ? win[h + 1 < MH ? h + 1 : h] : raw;
     y += p.D;
   };
 
@@ -444,8 +460,7 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
 }
 
 // Batches of (nearly) one token per request: a warp has the channels of one
-// request and walks its tokens, with filters and window in the element type (a
-// third of the registers, so that all of a step's warps run at once) and with
+// request and walks its tokens, with all of a step's warps running at once and
 // the metadata, the first token's row and the filters asked for together: three
 // latencies in a row. 256 requests of 4096 channels, 4 taps, bf16: 7.6 us.
 template <typename T, int NV, int WT>
@@ -461,7 +476,6 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
   const int r = (int)(blockIdx.x / p.nblk) * blockDim.y + threadIdx.y;
   const T* xg = reinterpret_cast<const T*>(p.x) + c0;
   T* yg = reinterpret_cast<T*>(p.y) + c0;
-  const T* wg = reinterpret_cast<const T*>(p.w);
   pdl_wait();
   pdl_trigger();
   if (r >= p.q.nseq) return;
@@ -470,22 +484,7 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
   zero(x);
   if (r < p.q.T) x = load_part<T, NV>(xg + (long long)r * p.ldx, n, vec);  // its row, in a batch of single tokens
   float bias[NV];
-#pragma unroll
-  for (int k = 0; k < MW; ++k) {
-    zero(w[k]);
-    const int tap = k - (MW - W);
-    if (tap < 0) continue;
-    if (p.vec_w) {
-      w[k] = load_part<T, NV>(wg + (long long)tap * p.sw_k + c0, n, n == NV);
-    } else {
-#pragma unroll
-      for (int c = 0; c < NV; ++c)
-        if (c < n) w[k].v[c] = wg[(long long)tap * p.sw_k + (long long)(c0 + c) * p.sw_d];
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < NV; ++c)
-    bias[c] = p.bias != nullptr && c < n ? to_f(reinterpret_cast<const T*>(p.bias)[c0 + c]) : 0.f;
+  conv_weights<T, NV>(p, c0, n, W, w, bias);
 #pragma unroll
   for (int h = 0; h < MH; ++h) zero(win[h]);
   int slot = -1;
@@ -496,19 +495,7 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
   }
   for (int t = b; t < e; ++t) {
     if (t != r || t != b) x = load_part<T, NV>(xg + (long long)t * p.ldx, n, vec);
-    Pack<T, NV> o;
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-      float s = bias[c];
-#pragma unroll
-      for (int k = 0; k < MW; ++k) {
-        if (k == MW - 1)
-          s = fma_io(w[k].v[c], x.v[c], s);
-        else if (k >= MW - W)
-          s = fma_io(w[k].v[c], win[k < MH ? k : 0].v[c], s);
-      }
-      o.v[c] = from_f<T>(p.silu ? s * sigmoid_t<T>(s) : s);
-    }
+    const Pack<T, NV> o = conv_out<T, NV>(w, bias, win, x, W, p.silu);
     store_part<T, NV>(yg + (long long)t * p.D, o, n, vec);
 #pragma unroll
     for (int h = 0; h < MH; ++h) win[h] = h + 1 < MH ? win[h + 1 < MH ? h + 1 : h] : x;
@@ -573,7 +560,15 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fetch(i * Ring::kStage, t0 + i * kGroup);
     Chans<NV> w[MW], bias, win[MH], acc[MW];
-    conv_weights<T, NV>(p, c0, n, W, w, bias);
+    {
+      Pack<T, NV> raw[MW];
+      float b[NV];
+      conv_weights<T, NV>(p, c0, n, W, raw, b);
+#pragma unroll
+      for (int k = 0; k < MW; ++k) widen<T, NV>(raw[k], w[k]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) bias[c] = pack2(b[2 * c], 2 * c + 1 < NV ? b[2 * c + 1 < NV ? 2 * c + 1 : 0] : 0.f);
+    }
     conv_zero<NV>(win);
     conv_zero<NV>(acc);
     const SeqView sv(p.q, lane);
