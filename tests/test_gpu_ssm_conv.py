@@ -292,3 +292,37 @@ def test_packed_captured():
         graph.replay()
         assert torch.equal(out, want[k])
     assert torch.equal(state, ref)
+
+
+def test_far_rows_and_slots():
+    """Rows and slots more than 2^31 elements apart give the near ones' bits."""
+    from greta_plugin_b200 import causal_conv1d, packed_causal_conv1d
+
+    lens, D, W = [9, 1, 1, 6], 64, 4
+    g = torch.Generator().manual_seed(22)
+    T, ld = sum(lens), 2 ** 28 + 8
+    x = rand(g, T, D, dtype=torch.bfloat16).to(DEV)
+    w, b = rand(g, W, D, dtype=torch.bfloat16).to(DEV), rand(g, D, dtype=torch.bfloat16).to(DEV)
+    far_x = torch.empty((T - 1) * ld + D, dtype=torch.bfloat16, device=DEV).as_strided((T, D), (ld, 1))
+    far_x.copy_(x)
+    state = rand(g, 3, D, W - 1, dtype=torch.bfloat16).to(DEV)
+    far = torch.empty(2 * (2 ** 30 + 64) + D * 3, dtype=torch.bfloat16, device=DEV).as_strided(
+        (3, D, W - 1), (2 ** 30 + 64, W - 1, 1))
+    far.copy_(state)
+    starts = ragged_cu(lens).to(DEV)
+    slots = torch.tensor([1, 0, -1, 2], dtype=torch.int32, device=DEV)
+    init = torch.ones(4, dtype=torch.int8, device=DEV)
+    cu, dout = starts, rand(g, 1, T, D, dtype=torch.bfloat16).to(DEV)
+    near = [t.detach().requires_grad_() for t in (x, w, b)]
+    wide = [t.detach().requires_grad_() for t in (far_x, w, b)]
+    outs = [causal_conv1d(t[0][None], t[1], t[2], cu, "silu") for t in (near, wide)]
+    assert torch.equal(*outs)
+    grads = [torch.autograd.grad(o, t[1:], dout) for o, t in zip(outs, (near, wide))]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    for single in (False, True):  # the prompts' kernel, then the single tokens'
+        if single:
+            starts, slots, init = starts[:0].new_tensor([0, 1, 2, 3]), slots[[0, 1, 3]].contiguous(), init[:3]
+            x, far_x = x[13:16], far_x[13:16]
+        want = packed_causal_conv1d(x, w, b, state, starts, slots, init, "silu")
+        got = packed_causal_conv1d(far_x, w, b, far, starts, slots, init, "silu")
+        assert torch.equal(got, want) and torch.equal(far, state)

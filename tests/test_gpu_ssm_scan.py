@@ -469,3 +469,29 @@ def test_two_captured_graphs_and_streams():
         assert torch.equal(out, o) and torch.equal(state, st)
     again = run_train(*make(300, 64, 16, 1, torch.bfloat16, 30), None)
     assert all(torch.equal(eager[k], again[k]) for k in again)
+
+
+def test_far_rows_and_slots():
+    """Rows and slots more than 2^31 elements apart give the near ones' bits."""
+    from greta_plugin_b200 import packed_selective_scan
+
+    lens, D, N = [9, 1, 1, 6], 64, 16
+    s, _ = make(sum(lens), D, N, 1, torch.bfloat16, 21)
+    starts, ld = ragged_cu(lens).to(DEV), 2 ** 28 + 8
+    slots = torch.tensor([1, 0, -1, 2], dtype=torch.int32, device=DEV)
+    init = torch.ones(4, dtype=torch.int8, device=DEV)
+    state = torch.randn(3, D, N, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    far = torch.empty(2 * (2 ** 30 + 64) + D * N, device=DEV).as_strided((3, D, N), (2 ** 30 + 64, N, 1))
+    far.copy_(state)
+    rows = torch.empty(16 * ld + D, dtype=torch.bfloat16, device=DEV).as_strided((17, D), (ld, 1))
+    rows.copy_(s["u"])
+    for single in (False, True):  # the prompts' kernels, then the single tokens'
+        if single:
+            starts, slots, init = starts[:0].new_tensor([0, 1, 2, 3]), slots[[0, 1, 3]].contiguous(), init[:3]
+            rows = rows[13:16]
+            s = {k: v[13:16] if v.shape[0] == 17 else v for k, v in s.items()}
+        want = packed_selective_scan(**s, state=state, starts=starts, slots=slots, has_initial=init)
+        got = packed_selective_scan(**{**s, "u": rows}, state=far, starts=starts, slots=slots, has_initial=init)
+        # (bits: without softplus some of these steps grow past what the type holds)
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+        assert torch.equal(far.contiguous().view(torch.int32), state.view(torch.int32))
