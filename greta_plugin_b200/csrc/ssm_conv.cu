@@ -35,8 +35,10 @@ int check(int dtype, const void* x, int64_t ldx, const void* w, const void* y, c
 }
 
 // Tokens beyond one per request up to which a batch is a decode batch: its
-// longest request then has at most kDecodeExtra + 1 tokens, walked one after
-// another.
+// longest request then has at most kDecodeExtra + 1 tokens (more only beside empty
+// ones, whose lengths the host does not know), walked one after another. 4, 32 and 256 requests of 4096 channels and 8 tokens more, all of one
+// request: decode kernel 6.6, 6.1, 7.9 us, runs 5.3, 5.4, 9.2; spread: 4.7, 4.4,
+// 8.1 and 5.8, 5.6, 9.2. 16 more of one request: 9.6, 9.1, 10.3 and 5.3, 5.4, 9.3.
 constexpr int64_t kDecodeExtra = 8;
 
 // Tokens per run, whole groups of four: as few as fill every SM with the CTAs it
