@@ -194,12 +194,14 @@ __device__ __forceinline__ void copy_vec(T* dst, const T* src) {
   }
 }
 
-// NV elements of a row into shared memory: asynchronously when the row is
-// there in whole aligned vectors, else n of them one by one and zeros.
+// NV elements of a row into shared memory: asynchronously when the operand's rows
+// are whole aligned vectors (vec), zeros from `base` where n <= 0; else n of them
+// one by one and zeros. An asynchronous copy of nothing, too, needs an address
+// aligned to its size, which only vec gives `base`.
 template <typename T, int NV>
 __device__ __forceinline__ void copy_part(T* dst, const T* src, const T* base, int n, bool vec) {
   constexpr int kBytes = sizeof(T) * NV;
-  if (vec || n <= 0) {
+  if (vec) {
     const bool ok = n > 0;
     const T* s = ok ? src : base;
     if constexpr (kBytes <= 16) {

@@ -231,7 +231,7 @@ __device__ __forceinline__ void copy_tile(const void* base, long long ld, bool v
     if (!TV::has(k, l.lane)) continue;
     const int r = TV::row(k, l.lane), t = tile0 + r, c = TV::chan(l.lane);
     const int n = t >= ta && t < tb ? l.nch - c : 0;
-    copy_part<T, TV::V>(s + r * CHW + c, b + t * ld + l.c0 + c, b, n, vec && n >= TV::V);
+    copy_part<T, TV::V>(s + r * CHW + c, b + t * ld + l.c0 + c, b, n, vec && (n >= TV::V || n <= 0));
   }
 }
 
@@ -787,7 +787,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_decode_kernel(con
         const int op = i / ROW, at = i % ROW * V, n = l.nch - at;
         const T* g = reinterpret_cast<const T*>(op == 0 ? p.u : op == 1 ? p.delta : p.gate);
         const long long ld = op == 0 ? p.ldu : op == 1 ? p.ldd : p.ldg;
-        if (g != nullptr) copy_part<T, V>(s + op * CHW + at, g + t * ld + l.c0 + at, g, n, p.vec && n >= V);
+        if (g != nullptr)
+          copy_part<T, V>(s + op * CHW + at, g + t * ld + l.c0 + at, g, n, p.vec && (n >= V || n <= 0));
       } else if (i < ALL) {
         const int k = i - 3 * ROW, op = k / LN, at = k % LN * 4;
         const T* g = reinterpret_cast<const T*>(op == 0 ? p.B : p.C);

@@ -1,0 +1,67 @@
+"""State-space operators on the GPU at the edges of what a call may be: operands
+on odd addresses, offsets that fall, request tables with many empty rows, mixed
+batches of many requests, token ranges chosen by hand, rows and slots past 2^31
+elements on the prompts' kernels, parameters of another type than the inputs,
+calls from two threads. The plain forms and bounds are those of
+ssm_reference.py, the cases' helpers those of the operators' own test files."""
+import pytest
+import torch
+
+import ssm_reference as R
+import test_gpu_ssm_scan as scan_tests
+from gpu_helpers import DEV, rand, ragged_cu
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def odd(t):
+    """`t` [T, ...] as a view whose rows begin on odd elements (an odd offset and
+    an odd row stride)."""
+    flat = t.reshape(t.shape[0], -1)
+    T, n = flat.shape
+    ld = n + 1 + n % 2  # odd
+    view = torch.zeros(T * ld + 2, dtype=t.dtype, device=t.device)[1:1 + T * ld].view(T, ld)[:, :n]
+    view.copy_(flat)
+    return view.unflatten(1, t.shape[1:]) if t.dim() > 2 else view
+
+
+def odd_operands(s):
+    return {k: odd(v) if v is not None and k in ("u", "delta", "gate", "B", "C") else v for k, v in s.items()}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D, N, F", [(61, 9, 1), (64, 16, 1), (40, 20, 2), (12, 65, 1)])
+def test_scan_operands_on_odd_addresses(dtype, D, N, F):
+    """Column views that start on no vector: partial tiles, slices and groups of
+    states have elements that are not there, which no copy may name an
+    unaligned address for."""
+    lens = [30, 1, 41]
+    s, dout = scan_tests.make(sum(lens), D, N, F, dtype, D)
+    s = odd_operands(s)
+    assert all(s[k].data_ptr() % 4 == 2 for k in ("u", "B")) or dtype == torch.float32
+    cu = ragged_cu(lens).to(DEV)
+    val, mag = R.scan(**s, softplus=True, cu=cu.tolist(), dout=dout)
+    got = scan_tests.run_train(s, dout, cu)
+    scan_tests.compare(got, val, mag, dtype, max(lens), sum(lens), D, F)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [[1] * 9, [50, 1, 37]])
+def test_packed_scan_operands_on_odd_addresses(dtype, lens):
+    from greta_plugin_b200 import packed_selective_scan
+
+    n, T = len(lens), sum(lens)
+    for D, N in ((61, 9), (64, 16)):
+        s, _ = scan_tests.make(T, D, N, 1, dtype, N)
+        s = odd_operands(s)
+        state = torch.randn(n, D, N, generator=torch.Generator().manual_seed(N)).to(DEV)
+        before = {i: state[i].clone() for i in range(n)}
+        starts = ragged_cu(lens)
+        out = packed_selective_scan(**s, state=state, starts=starts.to(DEV),
+                                    slots=torch.arange(n, dtype=torch.int32, device=DEV),
+                                    has_initial=torch.ones(n, dtype=torch.int8, device=DEV), delta_softplus=True)
+        val, mag = R.scan(**s, softplus=True, cu=starts.tolist(), before=before)
+        R.assert_within(out, val["out"], mag["out"], dtype, 32 * max(lens) + 64, "out")
+        for i in range(n):
+            R.assert_within(state[i], val["last"][i], mag["last"][i], torch.float32, 32 * max(lens) + 64, f"state {i}")
