@@ -170,7 +170,10 @@ extern "C" int greta_ssm_batch_metadata(const int32_t* query_lens, const int32_t
     p.used = blocks_used;
   }
   const size_t smem = sizeof(int) * 2 * (size_t)(num_reqs + 1);
-  cudaError_t e = allow_smem(batch_metadata_kernel, smem);
+  // (the limit is the kernel's, for all host threads: a call that set its own size
+  // could take away what another's launch was just allowed)
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 * 1024) e = allow_smem(batch_metadata_kernel, sizeof(int) * 2 * (kMaxRequests + 1));
   if (e != cudaSuccess) return GRETA_ERR_LAUNCH;
   const unsigned blocks = (unsigned)(T > 0 ? cdiv(T, kThreads) : 1);
   return finish(launch(batch_metadata_kernel, dim3(blocks), dim3(kThreads), smem,

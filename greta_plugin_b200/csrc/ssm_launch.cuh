@@ -36,6 +36,8 @@ cudaError_t launch(void (*k)(P...), dim3 grid, dim3 block, size_t smem, cudaStre
   return cudaLaunchKernelEx(&cfg, k, static_cast<P>(a)...);
 }
 
+// Lets a kernel's launches have `smem` bytes: the same value in every call of that
+// kernel, since a smaller one would lower the limit under another host thread.
 template <typename K>
 cudaError_t allow_smem(K kernel, size_t smem) {
   if (smem <= 48 * 1024) return cudaSuccess;

@@ -1,0 +1,58 @@
+"""Host side of the state-space operators without a GPU: what a call sets, asks
+for and passes on. Kernels do not run: launches go to a stand-in for the CUDA
+runtime's functions in a child process, or the C call is recorded."""
+import os
+import shutil
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parent.parent
+
+# What the library asks the CUDA runtime for, printed: attribute changes and
+# launches (dynamic shared memory, blocks).
+RUNTIME = r"""
+#include <stdio.h>
+#include <stddef.h>
+typedef struct { unsigned gx, gy, gz, bx, by, bz; size_t smem; } Config;
+int cudaFuncSetAttribute(const void* f, int attr, int value) {
+  printf("set %d %d\n", attr, value);
+  return 0;
+}
+int cudaLaunchKernelExC(const Config* c, const void* f, void** args) {
+  printf("launch %zu %u %u\n", c->smem, c->gx, c->gy);
+  return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def runtime(tmp_path_factory):
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    d = tmp_path_factory.mktemp("runtime")
+    (d / "runtime.c").write_text(RUNTIME)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", d / "runtime.so", d / "runtime.c"], check=True)
+    return d / "runtime.so"
+
+
+def recorded(runtime, code):
+    """Lines that the stand-in printed while `code` ran with the library as L."""
+    setup = "import ctypes; from greta_plugin_b200 import _capi; L = _capi.lib(); F = ctypes.c_void_p(0x1000)\n"
+    env = {**os.environ, "LD_PRELOAD": str(runtime), "PYTHONPATH": str(ROOT)}
+    out = subprocess.run([sys.executable, "-c", setup + code], env=env, capture_output=True, text=True, check=True)
+    return [line.split() for line in out.stdout.splitlines()]
+
+
+def test_metadata_calls_do_not_lower_each_others_limit(runtime):
+    """Two host threads with batches of different sizes: the shared memory that
+    one allows its launch may not be taken back by the other's call."""
+    lines = recorded(runtime, "for n in (16384, 8000, 100, 16384, 7000):\n"
+                     "    assert L.greta_ssm_batch_metadata(F, F, n, 8, F, F, F, F, None, 0, 0, 0, None, 0, None, None, None) == 0")
+    limits = {int(v[2]) for v in lines if v[0] == "set"}
+    launches = [int(v[1]) for v in lines if v[0] == "launch"]
+    assert len(launches) == 5
+    assert len(limits) == 1 and limits.pop() >= max(launches)
