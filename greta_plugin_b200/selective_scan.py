@@ -139,7 +139,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         _capi.call("greta_ssm_scan_fwd", u, *args, p(out), p(saved), p(cu), cu64, nseq, T, D, N, F, int(softplus),
                    ranges, p(ws), n)
         ctx.save_for_backward(u, delta, A, B, C, skip, gate, delta_bias, cu, saved)
-        ctx.softplus = softplus
+        ctx.softplus, ctx.ranges = softplus, ranges
         return out
 
     @staticmethod
@@ -157,7 +157,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         dskip = None if skip is None else torch.empty(D, dtype=f32, device=dev)
         dbias = None if delta_bias is None else torch.empty(D, dtype=f32, device=dev)
         cu, cu64, nseq = _cu(cu, dev)
-        ranges = _capi.token_ranges()
+        ranges = ctx.ranges  # the forward call's: autograd runs this on a thread of its own
         ws, n = _workspace("bwd", dev, nseq, T, D, N, F, ranges)
         p = _capi.addr
         _capi.call("greta_ssm_scan_bwd", u, *args, p(saved), p(dout), p(du), p(ddelta), p(dgate), p(dB), p(dC), p(dA),

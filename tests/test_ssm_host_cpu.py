@@ -1,6 +1,7 @@
 """Host side of the state-space operators without a GPU: what a call sets, asks
 for and passes on. Kernels do not run: launches go to a stand-in for the CUDA
 runtime's functions in a child process, or the C call is recorded."""
+import importlib
 import os
 import shutil
 import subprocess
@@ -56,3 +57,20 @@ def test_metadata_calls_do_not_lower_each_others_limit(runtime):
     launches = [int(v[1]) for v in lines if v[0] == "launch"]
     assert len(launches) == 5
     assert len(limits) == 1 and limits.pop() >= max(launches)
+
+
+def test_token_ranges_of_a_training_call_reach_its_backward(monkeypatch):
+    """launch_options holds for the calls that are made inside its block; the
+    backward of such a call runs on autograd's thread, and maybe behind it."""
+    from greta_plugin_b200 import _capi
+
+    module = importlib.import_module("greta_plugin_b200.selective_scan")  # (the package has the function's name)
+    seen = []
+    monkeypatch.setattr(module, "_workspace", lambda kind, dev, nseq, T, D, N, F, ranges: (None, 0))
+    monkeypatch.setattr(_capi, "call", lambda name, t, *a: seen.append((name, a[-3])))  # ranges, workspace, bytes
+    u = torch.zeros(1, 20, 8, requires_grad=True)
+    B = torch.zeros(20, 1, 4)
+    with _capi.launch_options(rows_ranges=5):
+        out = module.SelectiveScanFunction.apply(u, u, -torch.ones(8, 4), B, B, None, None, None, None, True, True)
+    out.backward(torch.ones_like(out))
+    assert seen == [("greta_ssm_scan_fwd", 5), ("greta_ssm_scan_bwd", 5)]
