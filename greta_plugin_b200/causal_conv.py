@@ -27,6 +27,7 @@ from . import _capi
 from .dynamic_conv import _cu
 
 MAX_WIDTH = 16
+GRADS_F32 = 0x100  # GRETA_SSM_GRADS_F32
 
 
 def _activation(activation) -> int:
@@ -103,13 +104,16 @@ class CausalConv1dFunction(torch.autograd.Function):
         (T, D), W = x.shape, w.shape[0]
         dout = _as_type(dout, dt).contiguous()
         dx = torch.empty(1, T, D, dtype=dt, device=dev)
-        dw = torch.empty(W, D, dtype=dt, device=dev)
-        db = None if b is None else torch.empty(D, dtype=dt, device=dev)
+        # parameters of another type than x's take the fp32 sums, not sums rounded to x's type
+        f32 = weight.dtype != dt or (bias is not None and bias.dtype != dt)
+        sums = torch.float32 if f32 else dt
+        dw = torch.empty(W, D, dtype=sums, device=dev)
+        db = None if b is None else torch.empty(D, dtype=sums, device=dev)
         ws = torch.empty(_capi.lib().greta_ssm_conv_bwd_workspace(T, D, W), dtype=torch.uint8, device=dev)
         cu, cu64, nseq = _cu(cu, dev)
         p = _capi.addr
         _capi.call("greta_ssm_conv_bwd", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(dout), p(dx),
-                   p(dw), p(db), p(cu), cu64, nseq, T, D, W, ctx.silu, p(ws), ws.numel())
+                   p(dw), p(db), p(cu), cu64, nseq, T, D, W, ctx.silu | (GRADS_F32 if f32 else 0), p(ws), ws.numel())
         return dx, _as_type(dw, weight.dtype), None if b is None else _as_type(db, bias.dtype), None, None
 
 
@@ -122,7 +126,9 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     offsets (None: one sequence); activation: None or "silu". Returns
     [1, T, D] contiguous. Each sequence starts with zero history; rows that no
     sequence holds give zeros and zero gradients. weight and bias are used in
-    x's type; their gradients are summed in fp32 and come back in their own.
+    x's type (fp32 ones beside 16-bit x are rounded to it, as its products are
+    taken there); their gradients are summed in fp32 and rounded once, to the
+    parameter's own type.
     """
     if x.dim() != 3 or x.shape[0] != 1:
         raise ValueError(f"x must be [1, T, D], got {tuple(x.shape)}")

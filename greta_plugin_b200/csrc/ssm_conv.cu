@@ -124,8 +124,21 @@ constexpr int kBwdMinRun = 8;
 // Rows of partial sums of the backward.
 int64_t bwd_rows(int64_t T, int L) { return cdiv(cdiv(T, L), kRuns); }
 
+// The gradients of the filters and the bias.
+struct ParamGrads {
+  void *dw, *dbias;
+  bool f32;  // fp32 arrays, else of the element type
+};
+
+template <typename T>
+int reduce(const ConvParams& p, int64_t rows, const ParamGrads& g, cudaStream_t st) {
+  const int64_t cols = cdiv((int64_t)(p.W + 1) * p.D, 32);
+  return finish(launch(ssm_conv_reduce_kernel<T>, dim3((unsigned)cols), dim3(32, 8), 0, st, (const float*)p.part,
+                       reinterpret_cast<T*>(g.dw), reinterpret_cast<T*>(g.dbias), (long long)rows, p.D, p.W));
+}
+
 template <typename T, int NV, int WT>
-int bwd_one(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
+int bwd_one(ConvParams p, const ParamGrads& g, cudaStream_t st) {
   p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
   const int64_t cw = cdiv(cdiv(p.D, NV), 32);
   p.L = run_tokens(p.q.T, cw, kBwdMinRun);
@@ -139,19 +152,17 @@ int bwd_one(ConvParams p, void* dw, void* dbias, cudaStream_t st) {
   cudaError_t e = allow_smem(k, smem);
   if (e == cudaSuccess) e = launch(k, dim3((unsigned)(rows * cw)), dim3(32, kRuns), smem, st, p);
   if (e != cudaSuccess) return GRETA_ERR_LAUNCH;
-  const int64_t cols = cdiv((int64_t)(p.W + 1) * p.D, 32);
-  return finish(launch(ssm_conv_reduce_kernel<T>, dim3((unsigned)cols), dim3(32, 8), 0, st, (const float*)p.part,
-                       reinterpret_cast<T*>(dw), reinterpret_cast<T*>(dbias), (long long)rows, p.D, p.W));
+  return g.f32 ? reduce<float>(p, rows, g, st) : reduce<T>(p, rows, g, st);
 }
 
 // Vectors of half the forward's: a thread's sums take 3 W registers a channel.
 template <typename T>
-int bwd_type(const ConvParams& p, void* dw, void* dbias, cudaStream_t st) {
+int bwd_type(const ConvParams& p, const ParamGrads& g, cudaStream_t st) {
   return with_taps(p.W, [&](auto taps) {
     constexpr int WT = decltype(taps)::value, NV = vec_of<T, WT>() >= 4 ? vec_of<T, WT>() / 2 : vec_of<T, WT>();
     const bool vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) &&
                      aligned(p.dout, NV * sizeof(T)) && aligned(p.dx, NV * sizeof(T));
-    return vec ? bwd_one<T, NV, WT>(p, dw, dbias, st) : bwd_one<T, 1, WT>(p, dw, dbias, st);
+    return vec ? bwd_one<T, NV, WT>(p, g, st) : bwd_one<T, 1, WT>(p, g, st);
   });
 }
 
@@ -200,8 +211,10 @@ int greta_ssm_conv_bwd(int dtype, const void* x, int64_t ldx, const void* w, int
   if (dw == nullptr || (bias == nullptr) != (dbias == nullptr)) return GRETA_ERR_INVALID_ARG;
   if (T > 0 && dout == nullptr) return GRETA_ERR_INVALID_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const ParamGrads g{dw, dbias, (silu & GRETA_SSM_GRADS_F32) != 0};
+  silu &= ~GRETA_SSM_GRADS_F32;
   if (T == 0) {  // sums over no tokens
-    const int es = esize(dtype);
+    const int es = g.f32 ? 4 : esize(dtype);
     cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)(W * D) * es, st);
     if (e == cudaSuccess && dbias != nullptr) e = cudaMemsetAsync(dbias, 0, (size_t)D * es, st);
     return finish(e);
@@ -213,9 +226,9 @@ int greta_ssm_conv_bwd(int dtype, const void* x, int64_t ldx, const void* w, int
   p.dx = dx;
   p.part = reinterpret_cast<float*>(workspace);
   switch (dtype) {
-    case GRETA_DT_F32: return bwd_type<float>(p, dw, dbias, st);
-    case GRETA_DT_F16: return bwd_type<__half>(p, dw, dbias, st);
-    default: return bwd_type<__nv_bfloat16>(p, dw, dbias, st);
+    case GRETA_DT_F32: return bwd_type<float>(p, g, st);
+    case GRETA_DT_F16: return bwd_type<__half>(p, g, st);
+    default: return bwd_type<__nv_bfloat16>(p, g, st);
   }
 }
 

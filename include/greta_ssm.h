@@ -47,7 +47,10 @@ GRETA_API int greta_ssm_conv_fwd(int dtype, const void* x, int64_t ldx, const vo
 
 /* Gradients of greta_ssm_conv_fwd: dx [T, D], dw [W, D] (both contiguous, of
  * the element type) and dbias [D] (NULL when bias is NULL); dout [T, D]
- * contiguous. dw and dbias are summed in fp32. */
+ * contiguous. dw and dbias are summed in fp32; with GRETA_SSM_GRADS_F32 added to
+ * `silu` they are fp32 arrays, which take the sums as they are (for parameters
+ * that are kept in fp32 beside 16-bit activations). */
+#define GRETA_SSM_GRADS_F32 0x100
 GRETA_API int greta_ssm_conv_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,
                                  const void* bias, const void* dout, void* dx, void* dw, void* dbias,
                                  const void* cu_seqlens, int cu_int64, int64_t num_seqs, int64_t T, int64_t D,

@@ -65,3 +65,38 @@ def test_packed_scan_operands_on_odd_addresses(dtype, lens):
         R.assert_within(out, val["out"], mag["out"], dtype, 32 * max(lens) + 64, "out")
         for i in range(n):
             R.assert_within(state[i], val["last"][i], mag["last"][i], torch.float32, 32 * max(lens) + 64, f"state {i}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D, W, wide", [(256, 4, "both"), (100, 3, "weight"), (64, 7, "bias")])
+def test_conv_gradients_of_fp32_parameters(dtype, D, W, wide):
+    """fp32 filters or bias beside 16-bit inputs: their gradients keep the fp32
+    sums' bits (a sum rounded to the inputs' type on the way is off by 2^-9)."""
+    from greta_plugin_b200 import causal_conv1d
+
+    g = torch.Generator().manual_seed(W)
+    lens = [150, 1, 89]
+    T = sum(lens)
+    x, dout = (rand(g, T, D, dtype=dtype).to(DEV) for _ in range(2))
+    w = rand(g, W, D, scale=W ** -0.5, dtype=torch.float32).to(DEV)
+    b = rand(g, D, dtype=torch.float32).to(DEV)
+    w, b = (w if wide != "bias" else w.to(dtype)).requires_grad_(), (b if wide != "weight" else b.to(dtype)).requires_grad_()
+    cu = ragged_cu(lens).to(DEV)
+    causal_conv1d(x[None], w, b, cu, "silu").backward(dout[None])
+    val, mag = R.conv(x, w.detach().to(dtype), b.detach().to(dtype), True, cu=cu.tolist(), dout=dout)
+    # the sums' own roundings, and the sigmoid of 16-bit inputs: 20 for arguments
+    # up to 10 (10 from the argument, 4 from the power, 3 from sum and
+    # reciprocal), twice in SiLU'
+    n = 2 * (W + 8) + T + 40
+    assert w.grad.dtype == w.dtype and b.grad.dtype == b.dtype
+    R.assert_within(w.grad, val["dw"], mag["dw"], w.dtype, n, "dw")
+    R.assert_within(b.grad, val["dbias"], mag["dbias"], b.dtype, n, "dbias")
+
+
+def test_conv_gradients_of_fp32_parameters_over_no_tokens():
+    from greta_plugin_b200 import causal_conv1d
+
+    x = torch.zeros(1, 0, 64, device=DEV, dtype=torch.bfloat16)
+    w, b = torch.ones(4, 64, device=DEV, requires_grad=True), torch.ones(64, device=DEV, requires_grad=True)
+    causal_conv1d(x, w, b, None, "silu").sum().backward()
+    assert w.grad.dtype == torch.float32 and not w.grad.any() and not b.grad.any()
