@@ -246,8 +246,9 @@ int greta_ssm_conv_packed(int dtype, const void* x, int64_t ldx, const void* w, 
   p.y = y;
   if (W > 1 && num_slots > 0) {
     p.state = state;
-    p.s_slot = s_slot; p.s_d = s_d; p.s_h = s_h; p.num_slots = num_slots;
+    p.s_slot = s_slot; p.s_d = s_d; p.s_h = s_h;
   }
+  p.num_slots = num_slots;
   p.slots = slots;
   p.initial = reinterpret_cast<const signed char*>(has_initial);
   p.err = error_flags;

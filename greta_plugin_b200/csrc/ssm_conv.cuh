@@ -368,9 +368,10 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
   auto begin = [&] {
     forget();
     slot = -1;
-    if (!PACKED || p.state == nullptr) return;
+    if (!PACKED || (p.state == nullptr && p.err == nullptr)) return;
     const int raw = p.slots[g.s], initial = p.initial[g.s];
     if (raw >= p.num_slots && p.err != nullptr && c0 == 0) atomicOr(p.err, 1);
+    if (p.state == nullptr) return;  // (no slots, or no history: asked for the check alone)
     slot = raw >= 0 && raw < p.num_slots ? raw : -1;
 #pragma unroll
     for (int h = 0; h < MH; ++h) zero(old[h]);
@@ -488,8 +489,8 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
 #pragma unroll
   for (int h = 0; h < MH; ++h) zero(win[h]);
   int slot = -1;
+  if (b < e && raw >= p.num_slots && p.err != nullptr && c0 == 0) atomicOr(p.err, 1);
   if (p.state != nullptr && b < e) {
-    if (raw >= p.num_slots && p.err != nullptr && c0 == 0) atomicOr(p.err, 1);
     slot = raw >= 0 && raw < p.num_slots ? raw : -1;
     if (slot >= 0 && initial != 0) conv_load_state<T, NV, MH>(p, slot, c0, n, H, win, WT > 1);
   }

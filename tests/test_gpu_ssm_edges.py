@@ -100,3 +100,53 @@ def test_conv_gradients_of_fp32_parameters_over_no_tokens():
     w, b = torch.ones(4, 64, device=DEV, requires_grad=True), torch.ones(64, device=DEV, requires_grad=True)
     causal_conv1d(x, w, b, None, "silu").sum().backward()
     assert w.grad.dtype == torch.float32 and not w.grad.any() and not b.grad.any()
+
+
+def meta(lens, slots, init=None):
+    """(starts, slots, has_initial) on the device."""
+    init = [1] * len(lens) if init is None else init
+    return (ragged_cu(lens).to(DEV), torch.tensor(slots, dtype=torch.int32, device=DEV),
+            torch.tensor(init, dtype=torch.int8, device=DEV))
+
+
+@pytest.mark.parametrize("lens", [[1, 1], [100, 1]])  # the single tokens' kernels, the prompts'
+@pytest.mark.parametrize("slots, bad", [([0, 5], True), ([5, 0], True), ([-1, 0], False)])
+def test_checked_calls_report_slots_out_of_range(lens, slots, bad):
+    """Also where there is no state to look at: no slots, or filters of one tap."""
+    import greta_plugin_b200 as greta
+
+    T, D, N = sum(lens), 64, 16
+    s, _ = scan_tests.make(T, D, N, 1, torch.bfloat16, 1)
+    x = s["u"]
+    for rows in (2, 0):
+        for W in (4, 1):
+            w = torch.ones(W, D, dtype=x.dtype, device=DEV)
+            state = torch.full((rows, D, W - 1), 3.0, dtype=x.dtype, device=DEV)
+            call = lambda: greta.packed_causal_conv1d_checked(x, w, None, state, *meta(lens, slots))  # noqa: E731
+            if bad or rows == 0:
+                with pytest.raises(IndexError, match="cache slot"):
+                    call()
+            else:
+                call()
+            assert rows == 0 or (state[1] == 3).all()
+        state = torch.full((rows, D, N), 3.0, device=DEV)
+        st, sl, init = meta(lens, slots)
+        call = lambda: greta.packed_selective_scan_checked(**s, state=state, starts=st, slots=sl,  # noqa: E731
+                                                           has_initial=init, delta_softplus=True)
+        if bad or rows == 0:
+            with pytest.raises(IndexError, match="cache slot"):
+                call()
+        else:
+            call()
+        assert rows == 0 or (state[1] == 3).all()
+
+
+def test_checked_calls_without_slots():
+    """Requests that have no slot need none."""
+    import greta_plugin_b200 as greta
+
+    s, _ = scan_tests.make(51, 64, 16, 1, torch.bfloat16, 1)
+    st, sl, init = meta([50, 1], [-1, -1])
+    greta.packed_selective_scan_checked(**s, state=torch.zeros(0, 64, 16, device=DEV), starts=st, slots=sl,
+                                        has_initial=init, delta_softplus=True)
+    greta.packed_causal_conv1d_checked(s["u"], s["u"][:4], None, s["u"].new_zeros(0, 64, 3), st, sl, init)
