@@ -74,3 +74,22 @@ def test_token_ranges_of_a_training_call_reach_its_backward(monkeypatch):
         out = module.SelectiveScanFunction.apply(u, u, -torch.ones(8, 4), B, B, None, None, None, None, True, True)
     out.backward(torch.ones_like(out))
     assert seen == [("greta_ssm_scan_fwd", 5), ("greta_ssm_scan_bwd", 5)]
+
+
+def test_request_tensors_of_other_types_keep_their_meaning():
+    """A count as has_initial, and offsets and slots past 32 bits: not the numbers
+    that their low bits make."""
+    from greta_plugin_b200.causal_conv import packed_metadata
+
+    x, state = torch.zeros(5, 8), torch.zeros(4, 8, 3)
+    starts = torch.tensor([0, 2, 2 ** 32 + 1], dtype=torch.int64)
+    slots = torch.tensor([2 ** 32 + 3, -(2 ** 32) + 1], dtype=torch.int64)
+    for init in (torch.tensor([256, 0]), torch.tensor([512, 0], dtype=torch.int32), torch.tensor([True, False]),
+                 torch.tensor([0.5, 0.0])):
+        st, sl, has = packed_metadata(x, state, starts, slots, init)
+        assert has.dtype == torch.int8 and (has != 0).tolist() == [True, False]
+    assert st.dtype == sl.dtype == torch.int32
+    assert st.tolist() == [0, 2, 2 ** 31 - 1]
+    assert sl[0] >= 4 and sl[1] < 0  # out of range, and none
+    st, sl, _ = packed_metadata(x, state, starts.new_tensor([0, 2, 5]), slots.new_tensor([3, -1]), init)
+    assert st.tolist() == [0, 2, 5] and sl.tolist() == [3, -1]
