@@ -56,8 +56,16 @@ def _check_weight(x, weight, bias):
         raise ValueError(f"kernel size must be between 1 and {MAX_WIDTH}, got {W}")
     if bias is not None and (bias.dim() != 1 or bias.shape[0] != D):
         raise ValueError(f"bias must be [{D}], got {tuple(bias.shape)}")
+    refuse_complex(weight=weight, bias=bias)
     same_device("x", x, weight=weight, bias=bias)
     return W
+
+
+def refuse_complex(**params):
+    """Parameters are converted to a real type, which would drop an imaginary part."""
+    for name, t in params.items():
+        if t is not None and t.is_complex():
+            raise ValueError(f"{name} must be real, got {t.dtype}")
 
 
 def same_device(name, t, **others):

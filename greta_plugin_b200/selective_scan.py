@@ -29,7 +29,7 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .causal_conv import channel_rows, check_disjoint, packed_metadata, packed_out, same_device
+from .causal_conv import channel_rows, check_disjoint, packed_metadata, packed_out, refuse_complex, same_device
 from .dynamic_conv import _cu
 
 MAX_STATES = 128
@@ -65,6 +65,7 @@ def _check(u, delta, A, B, C, skip, gate, delta_bias):
         for name, t in (("delta", delta), ("gate", gate), ("B", B), ("C", C)):
             if t is not None and t.dtype != dt:
                 raise ValueError(f"{name} dtype {t.dtype} must match u dtype {dt}")
+    refuse_complex(A=A, skip=skip, delta_bias=delta_bias)
     same_device("u", u, delta=delta, A=A, B=B, C=C, skip=skip, gate=gate, delta_bias=delta_bias)
     return T, D, N, groups[1]
 

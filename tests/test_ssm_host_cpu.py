@@ -93,3 +93,24 @@ def test_request_tensors_of_other_types_keep_their_meaning():
     assert sl[0] >= 4 and sl[1] < 0  # out of range, and none
     st, sl, _ = packed_metadata(x, state, starts.new_tensor([0, 2, 5]), slots.new_tensor([3, -1]), init)
     assert st.tolist() == [0, 2, 5] and sl.tolist() == [3, -1]
+
+
+def test_complex_parameters_are_refused():
+    """Their imaginary parts would be dropped."""
+    import greta_plugin_b200 as greta
+
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    x, B, c = z(5, 8), z(5, 1, 4), torch.complex64
+    for kw in (dict(A=z(8, 4, dtype=c)), dict(skip=z(8, dtype=c)), dict(delta_bias=z(8, dtype=c))):
+        args = {**dict(A=z(8, 4), skip=None, gate=None, delta_bias=None), **kw}
+        with pytest.raises(ValueError, match=f"{next(iter(kw))} must be real"):
+            greta.selective_scan(x[None], x[None], B=B, C=B, **args)
+        with pytest.raises(ValueError, match=f"{next(iter(kw))} must be real"):
+            greta.packed_selective_scan(x, x, B=B, C=B, **args, state=z(2, 8, 4), starts=i32(0, 5), slots=i32(0),
+                                        has_initial=i32(0))
+    for w, b, name in ((z(3, 8, dtype=c), None, "weight"), (z(3, 8), z(8, dtype=c), "bias")):
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            greta.causal_conv1d(x[None], w, b)
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            greta.packed_causal_conv1d(x, w, b, z(2, 8, 2), i32(0, 5), i32(0), i32(0))
