@@ -153,7 +153,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 def _as_meta(t, x, dtype):
     if t.dtype is dtype and t.get_device() == x.get_device() and t.dim() == 1 and t.is_contiguous():
         return t
-    if dtype is torch.int8:
+    if dtype is torch.int8 and t.dtype not in (torch.bool, torch.uint8, torch.int8):
         t = t.ne(0)  # (a count, 256 say, has no place in 8 bits)
     elif t.dtype is torch.int64:
         t = t.clamp(-1, 2 ** 31 - 1)  # (past 32 bits there is no row and no slot, and not another one's)
