@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_fwd_kernel(con
 #pragma unroll
       for (int h = 0; h < MH; ++h) {
         zero(fin[h]);
-        if (h >= MH - H) fin[h] = get_row<T, NV>(xg + (long long)(g.e - MH + h) * p.ldx, n);
+        // (offsets that fall may give it fewer: no row ahead of x all the same)
+        if (h >= MH - H) fin[h] = get_row<T, NV>(xg + (long long)max(g.e - MH + h, 0) * p.ldx, n);
       }
       conv_store_state<T, NV, MH>(p, slot, c0, n, H, fin, WT > 1);
       slot = -1;

@@ -150,3 +150,26 @@ def test_checked_calls_without_slots():
     greta.packed_selective_scan_checked(**s, state=torch.zeros(0, 64, 16, device=DEV), starts=st, slots=sl,
                                         has_initial=init, delta_softplus=True)
     greta.packed_causal_conv1d_checked(s["u"], s["u"][:4], None, s["u"].new_zeros(0, 64, 3), st, sl, init)
+
+
+@pytest.mark.parametrize("starts", [[0, 1, 10, 3], [0, 1, 2, 14, 5, 6], [0, 9, 4, 0, 0, 0], [3, 1, 12, 2, 40]])
+@pytest.mark.parametrize("W", [4, 16])
+def test_packed_conv_offsets_that_fall_read_no_other_rows(starts, W):
+    """Offsets that fall name no valid batch, but its reads stay inside x: what
+    lies around x reaches no slot and no output. (Rows that such offsets give to
+    no run stay as `out` was: of 0, 9, 4, 0, 0, 0 the search gives token 1 to
+    request 3, whose first three tokens belong to the run of its first, 0, which
+    the search gives to request 3 as well, to end at 1.)"""
+    from greta_plugin_b200 import packed_causal_conv1d
+
+    n = len(starts) - 1
+    for T, D in ((14, 64), (40, 64), (40, 8192)):  # (runs of one token, and of three)
+        around = torch.full((T + 64, D), 777.0, dtype=torch.bfloat16, device=DEV)
+        x = around[32:32 + T]
+        x.fill_(1.0)
+        state = torch.full((n, D, W - 1), 1.0, dtype=torch.bfloat16, device=DEV)
+        meta_ = (torch.tensor(starts, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV),
+                 torch.ones(n, dtype=torch.int8, device=DEV))
+        out = torch.zeros_like(x)
+        packed_causal_conv1d(x, torch.ones(W, D, dtype=torch.bfloat16, device=DEV), None, state, *meta_, out=out)
+        assert float(out.max()) <= W and float(state.max()) <= 1.0
