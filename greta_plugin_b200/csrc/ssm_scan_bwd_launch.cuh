@@ -31,7 +31,8 @@ cudaError_t scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st) {
     return launch(k, dim3((unsigned)(p.F * bpg), (unsigned)p.R), block, smem, st, m);
   });
   if (e != cudaSuccess) return e;
-  e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), (unsigned)p.F),
+  const unsigned groups = p.F < 65535 ? p.F : 65535;  // (what a grid's y dimension holds)
+  e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), groups),
              dim3(256), 0, st, (const float*)p.part_bc, (T*)g.dB, (T*)g.dC, bpg, p.q.T, p.N, p.F);
   if (e != cudaSuccess) return e;
   return launch(ssm_scan_reduce_a_kernel<4>, dim3((unsigned)cdiv((int64_t)p.D * (p.N + 2), 256)), dim3(256), 0, st,

@@ -173,3 +173,12 @@ def test_packed_conv_offsets_that_fall_read_no_other_rows(starts, W):
         out = torch.zeros_like(x)
         packed_causal_conv1d(x, torch.ones(W, D, dtype=torch.bfloat16, device=DEV), None, state, *meta_, out=out)
         assert float(out.max()) <= W and float(state.max()) <= 1.0
+
+
+def test_scan_more_groups_than_a_grid_dimension():
+    """F may be any divisor of D."""
+    lens, D = [2, 1], 70000
+    s, dout = scan_tests.make(3, D, 1, D, torch.float32, 2)
+    cu = ragged_cu(lens).to(DEV)
+    val, mag = R.scan(**s, softplus=True, cu=cu.tolist(), dout=dout)
+    scan_tests.compare(scan_tests.run_train(s, dout, cu), val, mag, torch.float32, 2, 3, D, D)
