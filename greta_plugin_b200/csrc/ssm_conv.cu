@@ -121,8 +121,18 @@ int fwd(int dtype, const ConvParams& p, void* stream) {
 
 constexpr int kBwdMinRun = 8;
 
-// Rows of partial sums of the backward.
+// Rows of partial sums of the backward, for vectors of NV channels; the most of
+// them over the vectors that bwd_type takes (the workspace is asked for by the
+// sizes alone).
 int64_t bwd_rows(int64_t T, int L) { return cdiv(cdiv(T, L), kRuns); }
+int64_t bwd_rows_most(int64_t T, int64_t D) {
+  int64_t most = 0;
+  for (int nv = 1; nv <= 4; nv *= 2) {
+    const int64_t r = bwd_rows(T, run_tokens(T, cdiv(cdiv(D, nv), 32), kBwdMinRun));
+    if (r > most) most = r;
+  }
+  return most;
+}
 
 // The gradients of the filters and the bias.
 struct ParamGrads {
@@ -139,6 +149,7 @@ int reduce(const ConvParams& p, int64_t rows, const ParamGrads& g, cudaStream_t 
 
 template <typename T, int NV, int WT>
 int bwd_one(ConvParams p, const ParamGrads& g, cudaStream_t st) {
+  static_assert(NV == 1 || NV == 2 || NV == 4, "counted by bwd_rows_most");
   p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
   const int64_t cw = cdiv(cdiv(p.D, NV), 32);
   p.L = run_tokens(p.q.T, cw, kBwdMinRun);
@@ -199,7 +210,7 @@ int greta_ssm_conv_fwd(int dtype, const void* x, int64_t ldx, const void* w, int
 
 int64_t greta_ssm_conv_bwd_workspace(int64_t T, int64_t D, int64_t W) {
   if (T <= 0 || D <= 0 || W <= 0) return 0;
-  return bwd_rows(T, kBwdMinRun) * (W + 1) * D * (int64_t)sizeof(float);
+  return bwd_rows_most(T, D) * (W + 1) * D * (int64_t)sizeof(float);
 }
 
 int greta_ssm_conv_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,

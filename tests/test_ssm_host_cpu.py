@@ -21,10 +21,12 @@ RUNTIME = r"""
 typedef struct { unsigned gx, gy, gz, bx, by, bz; size_t smem; } Config;
 int cudaFuncSetAttribute(const void* f, int attr, int value) {
   printf("set %d %d\n", attr, value);
+  fflush(stdout);
   return 0;
 }
 int cudaLaunchKernelExC(const Config* c, const void* f, void** args) {
   printf("launch %zu %u %u\n", c->smem, c->gx, c->gy);
+  fflush(stdout);
   return 0;
 }
 """
@@ -114,3 +116,24 @@ def test_complex_parameters_are_refused():
             greta.causal_conv1d(x[None], w, b)
         with pytest.raises(ValueError, match=f"{name} must be real"):
             greta.packed_causal_conv1d(x, w, b, z(2, 8, 2), i32(0, 5), i32(0), i32(0))
+
+
+def test_conv_backward_workspace_holds_the_launch_and_little_more(runtime):
+    """The workspace is what the launch's blocks write: a row of partial sums for
+    every block of runs, not for the shortest runs that there could be."""
+    shapes = [(T, D, W, dt) for T, D in ((1, 64), (9, 1), (300, 1000), (1531, 1001), (16288, 4096), (131072, 8192))
+              for W in (1, 2, 4, 8, 16) for dt in (0, 1, 2)]
+    lines = recorded(runtime, f"for T, D, W, dt in {shapes}:\n"
+                     "    n = L.greta_ssm_conv_bwd_workspace(T, D, W)\n"
+                     "    print('bytes', n, flush=True)\n"
+                     "    assert L.greta_ssm_conv_bwd(dt, F, D, F, D, 1, None, F, F, F, None, None, 0, 0, T, D, W, 0, F, n, None) == 0")
+    lines = [v for v in lines if v[0] != "set"]
+    assert len(lines) == 3 * len(shapes)  # (the second launch adds the rows up)
+    for (T, D, W, dt), (_, n), (_, _, blocks, _) in zip(shapes, lines[::3], lines[1::3]):
+        whole = 4 if dt and 2 <= W <= 4 else 2 if dt or W <= 8 else 1  # channels of a vector
+        vec = whole if D % whole == 0 else 1
+        rows = int(blocks) // -(-(-(-D // vec)) // 32)
+        wrote = rows * (W + 1) * D * 4
+        # (a grid of as many blocks has up to four times the rows with vectors of four
+        # channels that it has with one, and a row more by rounding)
+        assert wrote <= int(n) <= 5 * wrote, (T, D, W, dt)
