@@ -31,10 +31,13 @@ cudaError_t scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st) {
     return launch(k, dim3((unsigned)(p.F * bpg), (unsigned)p.R), block, smem, st, m);
   });
   if (e != cudaSuccess) return e;
-  const unsigned groups = p.F < 65535 ? p.F : 65535;  // (what a grid's y dimension holds)
-  e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), groups),
-             dim3(256), 0, st, (const float*)p.part_bc, (T*)g.dB, (T*)g.dC, bpg, p.q.T, p.N, p.F);
-  if (e != cudaSuccess) return e;
+  const int kRow = 65535;  // groups that a grid's y dimension holds
+  for (int f0 = 0; f0 < p.F; f0 += kRow) {
+    const unsigned groups = p.F - f0 < kRow ? p.F - f0 : kRow;
+    e = launch(ssm_scan_reduce_bc_kernel<T>, dim3((unsigned)cdiv((int64_t)p.q.T * 2 * p.N, 256), groups), dim3(256), 0,
+               st, (const float*)p.part_bc, (T*)g.dB, (T*)g.dC, bpg, p.q.T, p.N, p.F, f0);
+    if (e != cudaSuccess) return e;
+  }
   return launch(ssm_scan_reduce_a_kernel<4>, dim3((unsigned)cdiv((int64_t)p.D * (p.N + 2), 256)), dim3(256), 0, st,
                 (const float*)p.part_a, (const float*)p.part_d, g.dA, g.dskip, g.dbias, p.R, p.D, p.N);
 }
