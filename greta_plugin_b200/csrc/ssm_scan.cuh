@@ -198,7 +198,7 @@ __device__ __forceinline__ void store_slot(const ScanParams& p, int slot, const 
 // The request's slot, or -1 for none (negative or out of range, which is
 // flagged once).
 __device__ __forceinline__ int slot_of(const ScanParams& p, int s, bool flag) {
-  if (p.state == nullptr && p.err == nullptr) return -1;  // (no slots: none is in range)
+  if (p.state == nullptr) return -1;
   const int raw = p.slots[s];
   if (raw >= p.num_slots && p.err != nullptr && flag) atomicOr(p.err, 1);
   return raw >= 0 && raw < p.num_slots ? raw : -1;
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) ssm_scan_decode_kernel(con
   if (lane < count) {
     mb = seq_start(p.q, r0 + lane);
     me = seq_start(p.q, r0 + lane + 1);
-    if (p.state != nullptr || p.err != nullptr) {
+    if (p.state != nullptr) {
       const int raw = p.slots[r0 + lane];
       minit = p.initial[r0 + lane];
       if (mb < me && raw >= p.num_slots && p.err != nullptr && slice == 0) atomicOr(p.err, 1);
