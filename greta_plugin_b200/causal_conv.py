@@ -28,6 +28,7 @@ from .dynamic_conv import _cu
 
 MAX_WIDTH = 16
 GRADS_F32 = 0x100  # GRETA_SSM_GRADS_F32
+LONGEST_BIT = 8  # GRETA_SSM_LONGEST
 
 
 def _activation(activation) -> int:
@@ -174,6 +175,16 @@ def packed_metadata(x, state, starts, slots, has_initial):
             _as_meta(has_initial, x, torch.int8))
 
 
+def longest(max_query_len) -> int:
+    """GRETA_SSM_LONGEST of max_query_len (None: not known)."""
+    if max_query_len is None:
+        return 0
+    n = int(max_query_len)
+    if n < 0:
+        raise ValueError(f"max_query_len must not be negative, got {n}")
+    return min(max(n, 1), 2 ** 22 - 1) << LONGEST_BIT
+
+
 def packed_out(x, out):
     """(output of a packed call, whether it is new): `out`, checked, whose rows
     outside every request stay as they were, or a new tensor, where the kernel
@@ -204,12 +215,13 @@ def check_disjoint(out, **inputs):
             raise ValueError(f"out must not overlap {name}")
 
 
-def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, flags):
+def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, max_query_len, flags):
     if x.dim() != 2:
         raise ValueError(f"x must be [T, D], got {tuple(x.shape)}")
     T, D = x.shape
     W = _check_weight(x, weight, bias)
     silu = _activation(activation)
+    most = longest(max_query_len)
     if state.dim() != 3 or state.shape[1] != D or state.shape[2] != W - 1:
         raise ValueError(f"state must be [slots, {D}, {W - 1}], got {tuple(state.shape)}")
     if state.dtype != x.dtype:
@@ -228,11 +240,12 @@ def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out,
     p = _capi.addr
     _capi.call("greta_ssm_conv_packed", x, _capi.dtype_code(x), p(x), ldx, p(w), *w.stride(), p(b), p(out),
                p(state) or None, state.shape[0], *state.stride(), p(starts), p(slots), p(has_initial), slots.numel(),
-               T, D, W, silu, new, p(flags))
+               T, D, W, silu, new | most, p(flags))
     return out
 
 
-def packed_causal_conv1d(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None):
+def packed_causal_conv1d(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None,
+                         max_query_len=None):
     """Convolution of a packed serving batch with cache-slot history, in one launch.
 
     x: [T, D]; weight: [W, D]; bias: [D] or None; state: [slots, D, W-1] of x's
@@ -243,15 +256,21 @@ def packed_causal_conv1d(x, weight, bias, state, starts, slots, has_initial, act
     slot as it was, and the requests of one batch have different slots. Returns
     [T, D]: `out` when given, whose rows behind the last request stay as they
     were (they are zeros in a new tensor).
+
+    max_query_len: the most tokens of any request, where the host knows it. A
+    batch of at most 8 rows more than requests is taken for a decode step and
+    walked request by request; with this, one long request in a table of empty
+    ones is not. It has no say in the result.
     """
-    return _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, None)
+    return _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, max_query_len, None)
 
 
-def packed_causal_conv1d_checked(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None):
+def packed_causal_conv1d_checked(x, weight, bias, state, starts, slots, has_initial, activation=None, out=None,
+                                 max_query_len=None):
     """packed_causal_conv1d, reporting slots >= state.shape[0] (which the kernel
     skips) as IndexError. Waits for the device: for debugging and tests."""
     flags = torch.zeros(1, dtype=torch.int32, device=x.device)
-    out = _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, flags)
+    out = _packed(x, weight, bias, state, starts, slots, has_initial, activation, out, max_query_len, flags)
     if int(flags.item()) & 1:
         raise IndexError(f"a cache slot index is >= the number of cache slots ({state.shape[0]})")
     return out

@@ -35,10 +35,13 @@ int check(int dtype, const void* x, int64_t ldx, const void* w, const void* y, c
 }
 
 // Tokens beyond one per request up to which a batch is a decode batch: its
-// longest request then has at most kDecodeExtra + 1 tokens (more only beside empty
-// ones, whose lengths the host does not know), walked one after another. 4, 32 and 256 requests of 4096 channels and 8 tokens more, all of one
-// request: decode kernel 6.6, 6.1, 7.9 us, runs 5.3, 5.4, 9.2; spread: 4.7, 4.4,
-// 8.1 and 5.8, 5.6, 9.2. 16 more of one request: 9.6, 9.1, 10.3 and 5.3, 5.4, 9.3.
+// longest request then has at most kDecodeExtra + 1 tokens, walked one after
+// another, or more beside empty ones, whose lengths the host does not know unless
+// it is told the longest. 4, 32 and 256 requests of 4096 channels and 8 tokens
+// more, all of one request: decode kernel 6.6, 6.1, 7.9 us, runs 5.3, 5.4, 9.2;
+// spread: 4.7, 4.4, 8.1 and 5.8, 5.6, 9.2. 16 more of one request: 9.6, 9.1, 10.3
+// and 5.3, 5.4, 9.3. One request of 256 tokens beside 255 empty ones: 121 us in a
+// graph, runs 14 (256 of one token: 16).
 constexpr int64_t kDecodeExtra = 8;
 
 // Tokens per run, whole groups of four: as few as fill every SM with the CTAs it
@@ -82,12 +85,12 @@ int with_taps(int W, F f) {
 }
 
 template <typename T, int NV, int WT, bool PACKED>
-int fwd_one(ConvParams p, cudaStream_t st) {
+int fwd_one(ConvParams p, int64_t longest, cudaStream_t st) {
   p.vec_w = p.sw_d == 1 && p.sw_k % NV == 0 && aligned(p.w, NV * sizeof(T));
   if (p.state != nullptr) p.st_layout = state_layout(p.state, p.s_slot, p.s_d, p.s_h, p.W - 1, NV, sizeof(T));
   const int64_t cw = cdiv(cdiv(p.D, NV), 32);
   p.nblk = (int)cw;
-  if (PACKED && p.q.nseq > 0 && p.q.T <= p.q.nseq + kDecodeExtra) {
+  if (PACKED && p.q.nseq > 0 && p.q.T <= p.q.nseq + kDecodeExtra && longest <= kDecodeExtra + 1) {
     const int64_t blocks = cdiv(p.q.nseq, kRuns) * cw;
     if (blocks > INT_MAX) return GRETA_ERR_INVALID_ARG;
     return finish(launch(ssm_conv_decode_kernel<T, NV, WT>, dim3((unsigned)blocks), dim3(32, kRuns), 0, st, p));
@@ -101,21 +104,22 @@ int fwd_one(ConvParams p, cudaStream_t st) {
 
 // Whole vectors where every row starts on one; else single elements.
 template <typename T, bool PACKED>
-int fwd_type(const ConvParams& p, cudaStream_t st) {
+int fwd_type(const ConvParams& p, int64_t longest, cudaStream_t st) {
   return with_taps(p.W, [&](auto taps) {
     constexpr int WT = decltype(taps)::value, NV = vec_of<T, WT>();
     const bool vec = p.D % NV == 0 && p.ldx % NV == 0 && aligned(p.x, NV * sizeof(T)) && aligned(p.y, NV * sizeof(T));
-    return vec ? fwd_one<T, NV, WT, PACKED>(p, st) : fwd_one<T, 1, WT, PACKED>(p, st);
+    return vec ? fwd_one<T, NV, WT, PACKED>(p, longest, st) : fwd_one<T, 1, WT, PACKED>(p, longest, st);
   });
 }
 
+// longest: the most tokens of a request, 0 when it is not known
 template <bool PACKED>
-int fwd(int dtype, const ConvParams& p, void* stream) {
+int fwd(int dtype, const ConvParams& p, int64_t longest, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case GRETA_DT_F32: return fwd_type<float, PACKED>(p, st);
-    case GRETA_DT_F16: return fwd_type<__half, PACKED>(p, st);
-    default: return fwd_type<__nv_bfloat16, PACKED>(p, st);
+    case GRETA_DT_F32: return fwd_type<float, PACKED>(p, longest, st);
+    case GRETA_DT_F16: return fwd_type<__half, PACKED>(p, longest, st);
+    default: return fwd_type<__nv_bfloat16, PACKED>(p, longest, st);
   }
 }
 
@@ -205,7 +209,7 @@ int greta_ssm_conv_fwd(int dtype, const void* x, int64_t ldx, const void* w, int
   ConvParams p = base(x, ldx, w, sw_k, sw_d, bias, cu_seqlens, cu_int64, num_seqs, T, D, W, silu);
   p.y = y;
   p.zero_rest = 1;
-  return fwd<false>(dtype, p, stream);
+  return fwd<false>(dtype, p, 0, stream);
 }
 
 int64_t greta_ssm_conv_bwd_workspace(int64_t T, int64_t D, int64_t W) {
@@ -263,8 +267,8 @@ int greta_ssm_conv_packed(int dtype, const void* x, int64_t ldx, const void* w, 
   p.slots = slots;
   p.initial = reinterpret_cast<const signed char*>(has_initial);
   p.err = error_flags;
-  p.zero_rest = zero_rest != 0;
-  return fwd<true>(dtype, p, stream);
+  p.zero_rest = truth_of(zero_rest);
+  return fwd<true>(dtype, p, longest_of(zero_rest), stream);
 }
 
 }  // extern "C"

@@ -44,6 +44,10 @@ cudaError_t allow_smem(K kernel, size_t smem) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
 }
 
+// GRETA_SSM_LONGEST and the truth value that it was added to.
+inline int64_t longest_of(int flags) { return flags >> 8; }
+inline int truth_of(int flags) { return (flags & 0xff) != 0; }
+
 inline int finish(cudaError_t e) { return e == cudaSuccess ? GRETA_OK : GRETA_ERR_LAUNCH; }
 
 // Layout of a [slots, D, H] state from its strides for vectors of nv elements.

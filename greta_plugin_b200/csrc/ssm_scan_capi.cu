@@ -170,14 +170,18 @@ int run_bwd(int dtype, const ScanParams& p, const ScanGrads& g, void* stream) {
 }
 
 // Tokens beyond one per request up to which a batch is a decode batch: its
-// longest request then has at most kDecodeExtra + 1 tokens (more only beside empty
-// ones, whose lengths the host does not know), walked one after another. 4, 32 and 256 requests of 4096 x 16 and 32 tokens more, all of one
-// request: decode kernel 25, 27, 50 us, ranges 25, 38, 75; spread: 9, 8, 37 and
-// 23, 32, 55. 16 more: 14, 17, 38 and 12, 37, 55.
+// longest request then has at most kDecodeExtra + 1 tokens, walked one after
+// another, or more beside empty ones, whose lengths the host does not know unless
+// it is told the longest. 4, 32 and 256 requests of 4096 x 16 and 32 tokens more,
+// all of one request: decode kernel 25, 27, 50 us, ranges 25, 38, 75; spread: 9, 8,
+// 37 and 23, 32, 55. 16 more: 14, 17, 38 and 12, 37, 55. One request of 256 tokens
+// beside 255 empty ones: 266 us in a graph, ranges 35 (256 of one token: 33). Rows
+// copied ahead in that walk made it 150 us, and 29.0 us of a decode step 29.4.
 constexpr int64_t kDecodeExtra = 32;
 // (the grid has a row per chunk of up to 32 requests)
-bool is_decode(int64_t num_reqs, int64_t T, int ranges) {
-  return ranges == 0 && num_reqs > 0 && T <= num_reqs + kDecodeExtra && num_reqs <= 65535;
+bool is_decode(int64_t num_reqs, int64_t T, int ranges, int64_t longest) {
+  return ranges == 0 && num_reqs > 0 && T <= num_reqs + kDecodeExtra && longest <= kDecodeExtra + 1 &&
+         num_reqs <= 65535;
 }
 constexpr int kDecodeWarps = 16;  // per SM (20: 29.0 us instead of 27.8 at 256 requests of 4096 x 16)
 
@@ -193,7 +197,7 @@ extern "C" {
 int64_t greta_ssm_scan_workspace(int packed, int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F,
                                  int ranges) {
   if (T <= 0 || D <= 0 || N <= 0 || F <= 0 || D % F != 0 || N > kMaxStates || ranges < 0) return 0;
-  if (packed != 0 && is_decode(num_seqs, T, ranges)) return 0;
+  if (truth_of(packed) && is_decode(num_seqs, T, ranges, longest_of(packed))) return 0;
   int R = 1;
   plan_ranges(T, D, N, F, ranges, false, R);
   return Workspace(R, D, N).total;
@@ -234,7 +238,7 @@ int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* del
   if (out == nullptr || starts == nullptr || num_slots < 0) return GRETA_ERR_INVALID_ARG;
   if (num_reqs > 0 && (slots == nullptr || has_initial == nullptr)) return GRETA_ERR_INVALID_ARG;
   if (num_slots > 0 && state == nullptr) return GRETA_ERR_INVALID_ARG;
-  p.zero_rest = zero_rest != 0;
+  p.zero_rest = truth_of(zero_rest);
   if (num_slots > 0) {
     p.state = state;
     p.s_slot = s_slot; p.s_d = s_d; p.s_n = s_n; p.num_slots = num_slots;
@@ -248,7 +252,7 @@ int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* del
   p.initial = reinterpret_cast<const signed char*>(has_initial);
   p.err = error_flags;
   plan_vectors(p, esize(dtype), kFwdChans, {u, delta, gate, out});
-  if (is_decode(num_reqs, T, ranges)) {
+  if (is_decode(num_reqs, T, ranges, longest_of(zero_rest))) {
     // chunks of requests that leave every SM kDecodeWarps warps
     const int64_t chunks = (int64_t)sm_count() * kDecodeWarps / slices(D, N, F);
     int64_t per = cdiv(num_reqs, chunks < 1 ? 1 : chunks);

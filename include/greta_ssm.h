@@ -63,7 +63,14 @@ GRETA_API int64_t greta_ssm_conv_bwd_workspace(int64_t T, int64_t D, int64_t W);
  * copies), in one launch. state, slots, has_initial, starts (int32) and
  * error_flags as in greta_dynconv_packed_state; a request without tokens
  * leaves its slot as it was. Requests of one batch have different slots.
+ *
+ * A batch of few rows more than requests is taken for a decode step, whose
+ * requests are walked token by token. A table of mostly empty requests may hide a
+ * long one in as many rows: GRETA_SSM_LONGEST(n) added to `zero_rest` tells that
+ * no request has more than n tokens (below 2^22; 0: not known), and the choice
+ * goes by that. Results do not depend on it.
  */
+#define GRETA_SSM_LONGEST(n) ((n) << 8)
 GRETA_API int greta_ssm_conv_packed(int dtype, const void* x, int64_t ldx, const void* w, int64_t sw_k, int64_t sw_d,
                                     const void* bias, void* y, void* state, int64_t num_slots, int64_t s_slot,
                                     int64_t s_d, int64_t s_h, const int32_t* starts, const int32_t* slots,
@@ -102,7 +109,7 @@ GRETA_API int greta_ssm_scan_fwd(int dtype, const void* u, int64_t ldu, const vo
  * [num_slots, D, N] through element strides; starts (int32), slots,
  * has_initial, error_flags as in greta_dynconv_packed_state. A request without
  * tokens leaves its slot as it was. Requests of one batch have different
- * slots.
+ * slots. zero_rest with GRETA_SSM_LONGEST as in greta_ssm_conv_packed.
  */
 GRETA_API int greta_ssm_scan_packed(int dtype, const void* u, int64_t ldu, const void* delta, int64_t ldd,
                                     const void* gate, int64_t ldg, const void* B, int64_t ldb, const void* C,
@@ -131,7 +138,7 @@ GRETA_API int64_t greta_ssm_scan_bwd_workspace(int64_t num_seqs, int64_t T, int6
 
 /* Bytes of workspace of greta_ssm_scan_fwd and greta_ssm_scan_packed (the same `ranges`;
  * packed: 0 for greta_ssm_scan_fwd, 1 for greta_ssm_scan_packed, which needs
- * none for a batch of single tokens). */
+ * none for a batch of single tokens; with the GRETA_SSM_LONGEST of that call). */
 GRETA_API int64_t greta_ssm_scan_workspace(int packed, int64_t num_seqs, int64_t T, int64_t D, int64_t N, int64_t F,
                                            int ranges);
 

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import ssm_reference as R
+import test_gpu_ssm_conv as conv_tests
 import test_gpu_ssm_scan as scan_tests
 from gpu_helpers import DEV, rand, ragged_cu
 
@@ -80,7 +81,8 @@ def test_conv_gradients_of_fp32_parameters(dtype, D, W, wide):
     x, dout = (rand(g, T, D, dtype=dtype).to(DEV) for _ in range(2))
     w = rand(g, W, D, scale=W ** -0.5, dtype=torch.float32).to(DEV)
     b = rand(g, D, dtype=torch.float32).to(DEV)
-    w, b = (w if wide != "bias" else w.to(dtype)).requires_grad_(), (b if wide != "weight" else b.to(dtype)).requires_grad_()
+    w, b = w.to(dtype if wide == "bias" else w.dtype), b.to(dtype if wide == "weight" else b.dtype)
+    w, b = w.requires_grad_(), b.requires_grad_()
     cu = ragged_cu(lens).to(DEV)
     causal_conv1d(x[None], w, b, cu, "silu").backward(dout[None])
     val, mag = R.conv(x, w.detach().to(dtype), b.detach().to(dtype), True, cu=cu.tolist(), dout=dout)
@@ -182,3 +184,35 @@ def test_scan_more_groups_than_a_grid_dimension():
     cu = ragged_cu(lens).to(DEV)
     val, mag = R.scan(**s, softplus=True, cu=cu.tolist(), dout=dout)
     scan_tests.compare(scan_tests.run_train(s, dout, cu), val, mag, torch.float32, 2, 3, D, D)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("table, at, n", [(256, 128, 256), (300, 0, 301), (64, 63, 60)])
+def test_request_tables_with_many_empty_rows(dtype, table, at, n):
+    """A long request in a table of empty ones has the rows of a batch of single
+    tokens, and is walked by the kernels of those, or, with max_query_len, not."""
+    from greta_plugin_b200 import packed_causal_conv1d, packed_selective_scan
+
+    lens = [0] * table
+    lens[at] = n
+    if n < 100:
+        lens[5], lens[40] = 1, 3
+    T, D, N, W = sum(lens), 72, 16, 4
+    slots = [int(v) for v in torch.randperm(table + 2, generator=torch.Generator().manual_seed(n))[:table]]
+    scan_tests.check_packed(lens, slots, [1] * table, D, N, 1, dtype, seed=n)
+    conv_tests.check_packed(lens, slots, [1] * table, D, W, dtype, seed=n)
+    s, _ = scan_tests.make(T, D, N, 1, dtype, n)
+    st, sl, init = meta(lens, slots)
+    state = torch.randn(table + 2, D, N, generator=torch.Generator().manual_seed(n)).to(DEV)
+    before = {i: state[k].clone() for i, k in enumerate(slots)}
+    val, mag = R.scan(**s, softplus=True, cu=st.tolist(), before=before)
+    for most in (n, 10 ** 6):
+        now = state.clone()
+        out = packed_selective_scan(**s, state=now, starts=st, slots=sl, has_initial=init, delta_softplus=True,
+                                    max_query_len=most)
+        R.assert_within(out, val["out"], mag["out"], dtype, 32 * n + 64, "out")
+        for i in val["last"]:
+            R.assert_within(now[slots[i]], val["last"][i], mag["last"][i], torch.float32, 32 * n + 64, f"state {i}")
+    w, history = s["u"][:W], torch.ones(table + 2, D, W - 1, dtype=dtype, device=DEV)
+    want = packed_causal_conv1d(s["u"], w, None, history.clone(), st, sl, init)
+    assert torch.equal(want, packed_causal_conv1d(s["u"], w, None, history, st, sl, init, max_query_len=n))

@@ -54,7 +54,8 @@ def test_metadata_calls_do_not_lower_each_others_limit(runtime):
     """Two host threads with batches of different sizes: the shared memory that
     one allows its launch may not be taken back by the other's call."""
     lines = recorded(runtime, "for n in (16384, 8000, 100, 16384, 7000):\n"
-                     "    assert L.greta_ssm_batch_metadata(F, F, n, 8, F, F, F, F, None, 0, 0, 0, None, 0, None, None, None) == 0")
+                     "    assert L.greta_ssm_batch_metadata(F, F, n, 8, F, F, F, F, None, 0, 0, 0, None, 0, None, None,\n"
+                     "                                      None) == 0")
     limits = {int(v[2]) for v in lines if v[0] == "set"}
     launches = [int(v[1]) for v in lines if v[0] == "launch"]
     assert len(launches) == 5
@@ -126,7 +127,8 @@ def test_conv_backward_workspace_holds_the_launch_and_little_more(runtime):
     lines = recorded(runtime, f"for T, D, W, dt in {shapes}:\n"
                      "    n = L.greta_ssm_conv_bwd_workspace(T, D, W)\n"
                      "    print('bytes', n, flush=True)\n"
-                     "    assert L.greta_ssm_conv_bwd(dt, F, D, F, D, 1, None, F, F, F, None, None, 0, 0, T, D, W, 0, F, n, None) == 0")
+                     "    assert L.greta_ssm_conv_bwd(dt, F, D, F, D, 1, None, F, F, F, None, None, 0, 0, T, D, W, 0, F, n,\n"
+                     "                                None) == 0")
     lines = [v for v in lines if v[0] != "set"]
     assert len(lines) == 3 * len(shapes)  # (the second launch adds the rows up)
     for (T, D, W, dt), (_, n), (_, _, blocks, _) in zip(shapes, lines[::3], lines[1::3]):
@@ -137,3 +139,44 @@ def test_conv_backward_workspace_holds_the_launch_and_little_more(runtime):
         # (a grid of as many blocks has up to four times the rows with vectors of four
         # channels that it has with one, and a row more by rounding)
         assert wrote <= int(n) <= 5 * wrote, (T, D, W, dt)
+
+
+def test_a_long_request_beside_empty_ones_is_no_decode_step(runtime):
+    """A table of 256 requests with one prompt has the rows of 256 single tokens;
+    where the host knows the longest request, the choice of the kernels goes by it."""
+    lines = recorded(runtime, """
+for T, n, most in ((256, 256, 0), (256, 256, 1), (256, 256, 256), (300, 256, 1), (10, 4, 7), (10, 4, 40)):
+    flag = most << 8
+    need = L.greta_ssm_scan_workspace(1 | flag, n, T, 4096, 16, 1, 0)
+    print("bytes", need, flush=True)
+    assert L.greta_ssm_scan_packed(2, F, 4096, F, 4096, None, 0, F, 16, F, 16, F, None, None, F, F, n, 65536, 16, 1, F,
+                                   F, F, n, T, 4096, 16, 1, 0, 1 | flag, 0, None, F, need, None) == 0
+    assert L.greta_ssm_conv_packed(2, F, 4096, F, 4096, 1, None, F, F, n, 12288, 3, 1, F, F, F, n, T, 4096, 4, 0,
+                                   1 | flag, None, None) == 0
+    print("end", flush=True)
+""")
+    lines = [v for v in lines if v[0] != "set"]
+    calls, at = [], 0
+    for _ in range(6):
+        end = lines.index(["end"], at)
+        calls.append(lines[at:end])
+        at = end + 1
+    # decode: a scan launch of its own, without a workspace; else carries and outputs
+    launches = [len(c) - 1 for c in calls]
+    assert launches == [2, 2, 3, 3, 2, 2]
+    assert [int(c[0][1]) > 0 for c in calls] == [False, False, True, True, False, False]
+    # the convolution's decode kernel has 16 blocks of channels for four requests each
+    conv = [int(c[-1][2]) for c in calls]
+    assert conv[0] == conv[1] == 64 * 16 and conv[2] != conv[0]
+
+
+def test_max_query_len_reaches_the_calls(monkeypatch):
+    from greta_plugin_b200 import _capi
+    from greta_plugin_b200.causal_conv import longest
+
+    assert longest(None) == 0 and longest(0) == 1 << 8 and longest(33) == 33 << 8
+    assert longest(10 ** 9) == (2 ** 22 - 1) << 8 < 2 ** 31
+    with pytest.raises(ValueError, match="max_query_len"):
+        longest(-1)
+    assert _capi.lib().greta_ssm_scan_workspace(1, 64, 70, 64, 16, 1, 0) == 0
+    assert _capi.lib().greta_ssm_scan_workspace(1 | longest(64), 64, 70, 64, 16, 1, 0) > 0
