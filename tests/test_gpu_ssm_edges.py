@@ -216,3 +216,273 @@ def test_request_tables_with_many_empty_rows(dtype, table, at, n):
     w, history = s["u"][:W], torch.ones(table + 2, D, W - 1, dtype=dtype, device=DEV)
     want = packed_causal_conv1d(s["u"], w, None, history.clone(), st, sl, init)
     assert torch.equal(want, packed_causal_conv1d(s["u"], w, None, history, st, sl, init, max_query_len=n))
+
+
+# ---------------------------------------------------------------------------
+# which kernels run: the prompts' (ranges, with a workspace) or the single tokens'
+# ---------------------------------------------------------------------------
+@pytest.fixture
+def calls(monkeypatch):
+    """The scan's packed calls, as the bytes of workspace that they took: 0 is the
+    single tokens' kernel (or one range, which these cases do not have)."""
+    from greta_plugin_b200 import _capi
+
+    taken, call = [], _capi.call
+
+    def record(name, t, *args):
+        if name == "greta_ssm_scan_packed":
+            taken.append(args[-1])
+        return call(name, t, *args)
+
+    monkeypatch.setattr(_capi, "call", record)
+    return taken
+
+
+def mixed_batch(n, seed):
+    """n requests: single tokens, idle ones, and four prompts of up to 90 tokens;
+    distinct slots, some requests without one, some that start anew."""
+    g = torch.Generator().manual_seed(seed)
+    draw = lambda lo, hi, k: torch.randint(lo, hi, (k,), generator=g).tolist()  # noqa: E731
+    lens = [int(v > 0) for v in draw(0, 8, n)]
+    for at, m in zip(draw(0, n, 4), (90, 33, 17, 64)):
+        lens[at] = m
+    slots = torch.randperm(n + 3, generator=g)[:n].tolist()
+    for at in draw(0, n, 1 + n // 10):
+        slots[at] = -1
+    return lens, slots, [int(v > 0) for v in draw(0, 4, n)]
+
+
+@pytest.mark.parametrize("n", [40, 300, 1000])
+@pytest.mark.parametrize("ranges", [0, 1, 7])
+def test_packed_scan_prompts_beside_many_single_tokens(n, ranges, calls):
+    """32 requests and more (the offsets come from memory, not from a lane)."""
+    lens, slots, init = mixed_batch(n, n)
+    scan_tests.check_packed(lens, slots, init, 72, 16, 1, torch.bfloat16, ranges=ranges, tail=5, seed=n)
+    assert sum(lens) + 5 > n + 32 and (ranges == 1 or calls[-1] > 0)
+
+
+@pytest.mark.parametrize("n", [40, 300, 1000])
+@pytest.mark.parametrize("D, W, dtype", [(72, 4, torch.bfloat16), (512, 4, torch.float32), (61, 7, torch.float16)])
+def test_packed_conv_prompts_beside_many_single_tokens(n, D, W, dtype):
+    lens, slots, init = mixed_batch(n, n + 1)
+    assert sum(lens) + 5 > n + 8
+    conv_tests.check_packed(lens, slots, init, D, W, dtype, tail=5, seed=n)
+
+
+def test_packed_scan_in_long_chunks_continues_like_one_call(calls):
+    """A prompt in chunks of both kernels' lengths leaves what one call leaves."""
+    from greta_plugin_b200 import packed_selective_scan
+
+    chunks = [60, 1, 90, 33, 120, 1, 1]
+    total = sum(chunks)
+    s, _ = scan_tests.make(total, 64, 16, 1, torch.float32, 13)
+    rows, rest = ("u", "delta", "B", "C", "gate"), {k: s[k] for k in ("A", "skip", "delta_bias")}
+    val, mag = R.scan(**s, softplus=True)
+    state = torch.full((1, 64, 16), 9.0, device=DEV)
+    got, at = [], 0
+    for n in chunks:
+        st, sl, init = meta([n], [0], [int(at > 0)])
+        got.append(packed_selective_scan(**{k: s[k][at:at + n] for k in rows}, **rest, state=state, starts=st, slots=sl,
+                                         has_initial=init, delta_softplus=True))
+        at += n
+    assert [n > 0 for n in calls] == [n > 33 for n in chunks]
+    base = 32 * total + 64
+    R.assert_within(torch.cat(got), val["out"], mag["out"], torch.float32, base, "out")
+    R.assert_within(state[0], val["last"][0], mag["last"][0], torch.float32, base, "state")
+
+
+def test_packed_scan_slot_out_of_range_on_a_long_request(calls):
+    """The prompts' kernels skip the slot and flag it, split over ranges or not."""
+    from greta_plugin_b200 import _capi, packed_selective_scan_checked
+
+    lens = [100, 1, 60]
+    s, _ = scan_tests.make(161, 32, 16, 1, torch.bfloat16, 0)
+    state = torch.ones(2, 32, 16, device=DEV)
+    for ranges in (0, 6):
+        for slots in ([5, 0, -1], [0, -1, 2]):
+            st, sl, init = meta(lens, slots)
+            with _capi.launch_options(rows_ranges=ranges), pytest.raises(IndexError, match="cache slot"):
+                packed_selective_scan_checked(**s, state=state, starts=st, slots=sl, has_initial=init)
+            assert (state[1] == 1).all() and calls[-1] > 0
+
+
+def test_serving_steps_in_long_chunks_equal_one_training_call(calls):
+    """Metadata, convolution and scan together in steps past the single tokens'
+    kernels, against the formulas on the whole sequences."""
+    import greta_plugin_b200 as greta
+
+    D, N, W, total, f32 = 64, 16, 4, [170, 83, 121], torch.float32
+    g = torch.Generator().manual_seed(0)
+    seqs = [{k: rand(g, n, *s, dtype=f32).to(DEV) for k, s in
+             (("x", (D,)), ("delta", (D,)), ("gate", (D,)), ("B", (1, N)), ("C", (1, N)))} for n in total]
+    w, b = rand(g, W, D, scale=0.5, dtype=f32).to(DEV), rand(g, D, dtype=f32).to(DEV)
+    A = -(torch.rand(D, N, generator=g) * 2 + 0.05).to(DEV)
+    skip, bias = rand(g, D, dtype=f32).to(DEV), (rand(g, D, dtype=f32) - 2).to(DEV)
+    conv_state, scan_state = torch.full((5, D, W - 1), 3.0, device=DEV), torch.full((5, D, N), 3.0, device=DEV)
+    slots, context, got = torch.tensor([4, 0, 2], dtype=torch.int32, device=DEV), [0, 0, 0], [[], [], []]
+    for step in ([70, 0, 40], [1, 80, 1], [98, 1, 79], [1, 2, 1]):
+        T = sum(step) + 3
+        rows = {k: torch.cat([s[k][c:c + n] for s, c, n in zip(seqs, context, step)] +
+                             [torch.full_like(seqs[0][k][:3], float("nan"))]) for k in seqs[0]}
+        m = greta.packed_batch_metadata(torch.tensor(step, dtype=torch.int32, device=DEV),
+                                        torch.tensor(context, dtype=torch.int32, device=DEV), T)
+        xc = greta.packed_causal_conv1d(rows["x"], w, b, conv_state, m.starts, slots, m.has_initial, "silu")
+        y = greta.packed_selective_scan(xc, rows["delta"], A, rows["B"], rows["C"], skip, rows["gate"], bias,
+                                        scan_state, m.starts, slots, m.has_initial, True)
+        assert not y[sum(step):].any()
+        at = 0
+        for i, n in enumerate(step):
+            got[i].append(y[at:at + n])
+            at += n
+            context[i] += n
+    assert context == total and [n > 0 for n in calls] == [True, True, True, False]
+    cu = ragged_cu(total).tolist()
+    whole = {k: torch.cat([s[k] for s in seqs]) for k in seqs[0]}
+    u, umag = R.conv(whole["x"], w, b, True, cu=cu)
+    val, mag = R.scan(u["out"], whole["delta"], A, whole["B"], whole["C"], skip, whole["gate"], bias, True, cu)
+    # the scan is linear in u, whose own error is W + 8 roundings of its magnitude
+    _, by_u = R.scan(umag["out"], whole["delta"], A, whole["B"], whole["C"], skip, whole["gate"], bias, True, cu)
+    n = 32 * max(total) + 64
+    R.assert_within(torch.cat([torch.cat(v) for v in got]), val["out"], torch.maximum(mag["out"], by_u["out"]), f32,
+                    n + W + 8, "serving")
+
+
+def far_rows(s, T, ld):
+    """The operands of `s` as column blocks of one buffer whose rows lie `ld`
+    elements apart."""
+    wide = {k: v for k, v in s.items() if v is not None and k in ("u", "delta", "gate", "B", "C")}
+    sizes = {k: v[0].numel() for k, v in wide.items()}
+    dt = s["u"].dtype
+    buf = torch.empty((T - 1) * ld + sum(sizes.values()), dtype=dt, device=DEV)
+    buf = buf.as_strided((T, sum(sizes.values())), (ld, 1))
+    out, at = dict(s), 0
+    for k, v in wide.items():
+        view = buf[:, at:at + sizes[k]]
+        view.copy_(v.reshape(T, -1))
+        out[k] = view.unflatten(1, v.shape[1:]) if v.dim() > 2 else view
+        at += sizes[k]
+    return out
+
+
+def test_scan_far_rows_and_slots_on_the_prompts_kernels(calls):
+    """Rows of all operands and slots more than 2^31 elements apart give the near
+    ones' bits: in split ranges, as the test before the single tokens' kernel."""
+    from greta_plugin_b200 import _capi, packed_selective_scan
+
+    lens, D, N = [9, 1, 1, 7], 64, 16
+    T = sum(lens)
+    s, _ = scan_tests.make(T, D, N, 1, torch.bfloat16, 21)
+    far = far_rows(s, T, 2 ** 28 + 8)
+    starts, slots, init = meta(lens, [1, 0, -1, 2])
+    state = torch.randn(3, D, N, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    far_state = torch.empty(2 * (2 ** 30 + 64) + D * N, device=DEV).as_strided((3, D, N), (2 ** 30 + 64, N, 1))
+    far_state.copy_(state)
+    kw = dict(starts=starts, slots=slots, has_initial=init, delta_softplus=True)
+    with _capi.launch_options(rows_ranges=3):
+        want = packed_selective_scan(**s, state=state, **kw)
+        got = packed_selective_scan(**far, state=far_state, **kw)
+    assert all(n > 0 for n in calls)
+    assert torch.equal(got, want) and torch.equal(far_state, state)
+
+
+def test_scan_training_far_rows():
+    """Forward and backward with rows more than 2^31 elements apart."""
+    from greta_plugin_b200 import _capi
+
+    lens, D, N = [9, 1, 8], 64, 16
+    T = sum(lens)
+    s, dout = scan_tests.make(T, D, N, 1, torch.bfloat16, 22)
+    far, cu = far_rows(s, T, 2 ** 28 + 8), ragged_cu(lens).to(DEV)
+    for ranges in (1, 3):
+        with _capi.launch_options(rows_ranges=ranges):
+            want = scan_tests.run_train(s, dout, cu)
+            got = far_train(far, dout, cu)
+        for k in got:
+            assert torch.equal(got[k], want[k]), (k, ranges)
+
+
+def far_train(s, dout, cu):
+    """Outputs and gradients through the autograd node itself, which keeps the
+    operands as they lie."""
+    from greta_plugin_b200 import selective_scan
+
+    leaf = {k: v.detach().requires_grad_() for k, v in s.items()}
+    a = {**leaf, **{k: leaf[k][None] for k in ("u", "delta", "gate")}}
+    out = selective_scan(**a, delta_softplus=True, cu_seqlens=cu)
+    names = ("u", "delta", "gate", "A", "B", "C", "skip", "delta_bias")
+    grads = torch.autograd.grad(out, [a[k] for k in names], dout[None])
+    return {"out": out[0].detach(), **{"d" + k: g[0] if k in ("u", "delta", "gate") else g
+                                       for k, g in zip(names, grads)}}
+
+
+# ---------------------------------------------------------------------------
+# ranges of whole sequences, and wide states
+# ---------------------------------------------------------------------------
+def takes_whole(lens, D, N, T):
+    """The host's rule (ranges of whole sequences): the longest is at most 0.4 of
+    what each scheduler has to walk in all."""
+    lanes = 4 if N <= 16 else 8 if N <= 32 else 16 if N <= 64 else 32
+    slices = -(-D // (32 // lanes * 4))
+    return len(lens) < 32 and max(lens) <= int(0.4 * T * slices / (4 * torch.cuda.get_device_properties(0)
+                                                                    .multi_processor_count))
+
+
+WHOLE = [([23] * 20, 4096), ([5, 0, 40, 1, 1, 33, 17, 8, 64, 2, 0, 30] * 2, 8192), ([9, 31, 14, 1, 22] * 6, 4096)]
+
+
+@pytest.mark.parametrize("lens, D", WHOLE)
+@pytest.mark.parametrize("head, tail", [(0, 0), (13, 21)])
+def test_train_ranges_of_whole_sequences(lens, D, head, tail):
+    assert takes_whole(lens, D, 16, sum(lens) + head + tail)
+    scan_tests.check_train(lens, D, 16, dtype=torch.bfloat16, head=head, tail=tail)
+
+
+@pytest.mark.parametrize("lens, D", WHOLE)
+def test_packed_ranges_of_whole_sequences(lens, D):
+    assert takes_whole(lens, D, 16, sum(lens) + 9)
+    n = len(lens)
+    slots = [(7 * i) % n if i % 5 else -1 for i in range(n)] if n % 7 else list(range(n))
+    scan_tests.check_packed(lens, slots, [1, 0] * (n // 2), D, 16, tail=9)
+
+
+def test_ranges_of_whole_sequences_do_not_mix():
+    """Two ranges share a tile where one ends and the next begins inside it: NaN in
+    a sequence and in the rows outside change no bit of the others, forward and
+    backward (sums over tokens apart)."""
+    lens, D, tail = [23] * 20, 4096, 9
+    T = sum(lens) + tail
+    assert takes_whole(lens, D, 16, T)
+    s, dout = scan_tests.make(T, D, 16, 1, torch.bfloat16, 5)
+    cu = ragged_cu(lens).to(DEV)
+    clean = scan_tests.run_train(s, dout, cu)
+    for bad in (1, 6, 19):
+        a, b = 23 * bad, 23 * (bad + 1)
+        t = {k: v.clone() if v is not None else None for k, v in s.items()}
+        for k in ("u", "delta", "B", "C", "gate"):
+            t[k][a:b] = float("nan")
+            t[k][-tail:] = float("nan")
+        t["u"][a + 5] = float("inf")
+        d = dout.clone()
+        d[a:b] = float("nan")
+        got = scan_tests.run_train(t, d, cu)
+        for k in ("out", "du", "ddelta", "dgate", "dB", "dC"):
+            assert torch.equal(got[k][:a], clean[k][:a]) and torch.equal(got[k][b:], clean[k][b:]), (k, bad)
+            assert got[k][a:b].isnan().any(), (k, bad)
+
+
+@pytest.mark.parametrize("N, F", [(64, 1), (128, 2)])
+def test_train_wide_states_over_many_blocks(N, F):
+    """Wide states beside many channels: hundreds of parts of dB and dC a token."""
+    scan_tests.check_train([150, 1, 90], 2048, N, F, torch.bfloat16, seed=N)
+
+
+@pytest.mark.parametrize("ranges", [1, 2, 5, 25])
+@pytest.mark.parametrize("lens", [[200], [90, 1, 109], [1] * 40 + [150, 3]])
+def test_train_ranges_reach_the_backward(ranges, lens, monkeypatch):
+    """The forward's ranges in the backward too: adjoints carried over each."""
+    from greta_plugin_b200 import _capi
+
+    seen, call = [], _capi.call
+    monkeypatch.setattr(_capi, "call", lambda name, t, *a: (seen.append((name, a[-3])), call(name, t, *a))[1])
+    scan_tests.check_train(lens, 40, 16, seed=ranges, ranges=ranges)
+    assert seen == [("greta_ssm_scan_fwd", ranges), ("greta_ssm_scan_bwd", ranges)]
