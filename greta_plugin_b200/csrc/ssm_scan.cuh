@@ -77,7 +77,8 @@ struct ScanParams {
   // backward
   const void* dout;
   void *du, *ddelta, *dgate;
-  float *part_bc;  // [D blocks][T][2][N]
+  int b0;          // first of the launch's D blocks
+  float *part_bc;  // [the launch's D blocks][T][2][N]
   float *part_a;   // [R][D][N]
   float *part_d;   // [R][2][D]: dskip, d(delta_bias)
 };

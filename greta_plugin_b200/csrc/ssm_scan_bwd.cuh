@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   pdl_wait();
   pdl_trigger();
   const int bpg = (p.spg + kScanWarps - 1) / kScanWarps;  // CTAs per group
-  const int f = blockIdx.x / bpg, in_group = blockIdx.x % bpg * kScanWarps + warp;
+  const int block = p.b0 + blockIdx.x;
+  const int f = block / bpg, in_group = block % bpg * kScanWarps + warp;
   const bool have = in_group < p.spg;  // else a warp without channels, which only keeps the CTA's steps
   L l(p, f * p.spg + (have ? in_group : 0), lane);
   if (!have) l.nch = 0;
@@ -638,20 +639,28 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) ssm_scan_bwd_kernel(const 
   }
 }
 
-// dB[t, f, n], dC[t, f, n] = sums over the CTAs of group f, from f0 on. (A loop over
-// the groups in here takes 57 us instead of 27 with one of them.)
+// dB[t, f, n], dC[t, f, n] = sums over the CTAs of group f, of which a launch of the
+// main kernel left blocks [lo, hi); a group's sums over the launches before are
+// in `acc` [F][T][2][N]. One addition after the other, so the launches make no
+// difference to the bits. (A loop over the groups in here takes 57 us instead of
+// 27 with one of them.)
 template <typename T>
-__global__ void __launch_bounds__(256) ssm_scan_reduce_bc_kernel(const float* part, T* dB, T* dC, int bpg, int T_,
-                                                                 int N, int F, int f0) {
+__global__ void __launch_bounds__(256) ssm_scan_reduce_bc_kernel(const float* part, float* acc, T* dB, T* dC, int bpg,
+                                                                 int lo, int hi, int T_, int N, int F, int f0) {
   pdl_wait();
   pdl_trigger();
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x, per = (long long)T_ * 2 * N;
   const int f = f0 + blockIdx.y;
   if (i >= per) return;
-  const float* s = part + (long long)f * bpg * per + i;
-  float v = 0.f;
+  const int b0 = max(lo - f * bpg, 0), b1 = min(hi - f * bpg, bpg);
+  const float* s = part + ((long long)f * bpg - lo) * per + i;
+  float v = b0 > 0 ? acc[f * per + i] : 0.f;
 #pragma unroll 8
-  for (int b = 0; b < bpg; ++b) v += s[b * per];
+  for (int b = b0; b < b1; ++b) v += s[b * per];
+  if (b1 < bpg) {
+    acc[f * per + i] = v;
+    return;
+  }
   const long long t = i / (2 * N);
   const int k = (int)(i / N % 2), n = (int)(i % N);
   (k == 0 ? dB : dC)[(t * F + f) * N + n] = from_f<T>(v);

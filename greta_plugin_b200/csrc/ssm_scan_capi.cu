@@ -148,13 +148,30 @@ int run_decode(int dtype, const ScanParams& p, void* stream) {
   }
 }
 
+// Blocks of the backward's main kernel that one launch takes. Each leaves a row of
+// 2 N sums for every token, and a block has 64 channels for up to 16 states but 8
+// for 128, so the rows of all of them grow with T D N: 8.6 GB for 16384 x 4096 x
+// 128. Where that is more than kPartBytes, as many blocks as keep to it, in whole
+// waves of CTAs, or one wave: 1.3 GB, in seven launches (backward 19.6 ms, 19.1 in one).
+constexpr int64_t kPartBytes = int64_t(2) << 30;
+int64_t bwd_blocks(int64_t blocks, int64_t R, int64_t T, int64_t N) {
+  int64_t most = kPartBytes / (T * 2 * N * 4);
+  if (blocks <= most) return blocks;
+  int64_t wave = (int64_t)sm_count() * kBwdCtasPerSm / R;
+  if (wave < 1) wave = 1;
+  most = most < wave ? wave : most / wave * wave;
+  return most < blocks ? most : blocks;
+}
+
 // The backward's workspace: the carries', then the parts of the sums.
 struct BwdWorkspace {
-  int64_t bc, a, d, total;
+  int64_t blocks, bc, acc, a, d, total;
   BwdWorkspace(int64_t R, int64_t T, int64_t D, int64_t N, int64_t F) {
-    const int64_t blocks = F * cdiv(bwd_slices_per_group(D, N, F), kScanWarps);
+    const int64_t per_group = cdiv(bwd_slices_per_group(D, N, F), kScanWarps), all = F * per_group;
+    blocks = bwd_blocks(all, R, T, N);
     bc = a16(Workspace(R, D, N).total);
-    a = bc + a16(blocks * T * 2 * N * 4);
+    acc = bc + a16(blocks * T * 2 * N * 4);
+    a = acc + (blocks < all && per_group > 1 ? a16(F * T * 2 * N * 4) : 0);
     d = a + a16(R * D * N * 4);
     total = d + a16(R * 2 * D * 4);
   }
@@ -312,7 +329,8 @@ int greta_ssm_scan_bwd(int dtype, const void* u, int64_t ldu, const void* delta,
   p.part_bc = reinterpret_cast<float*>(b + w.bc);
   p.part_a = reinterpret_cast<float*>(b + w.a);
   p.part_d = reinterpret_cast<float*>(b + w.d);
-  return run_bwd(dtype, p, ScanGrads{dA, dskip, ddelta_bias, dB, dC}, stream);
+  return run_bwd(dtype, p,
+                 ScanGrads{dA, dskip, ddelta_bias, dB, dC, (int)w.blocks, reinterpret_cast<float*>(b + w.acc)}, stream);
 }
 
 }  // extern "C"

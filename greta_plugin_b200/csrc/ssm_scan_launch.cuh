@@ -67,10 +67,14 @@ cudaError_t scan_decode(const ScanParams& p, cudaStream_t st) {
   });
 }
 
-// dA, dskip, ddbias and dB, dC: null where there is no such gradient.
+// dA, dskip, ddbias and dB, dC: null where there is no such gradient. blocks: those
+// of the main kernel that one launch takes, and acc: the groups' sums between
+// launches.
 struct ScanGrads {
   float *dA, *dskip, *dbias;
   void *dB, *dC;
+  int blocks;
+  float* acc;
 };
 
 cudaError_t scan_fwd_f32(const ScanParams&, cudaStream_t);

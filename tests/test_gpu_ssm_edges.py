@@ -486,3 +486,32 @@ def test_train_ranges_reach_the_backward(ranges, lens, monkeypatch):
     monkeypatch.setattr(_capi, "call", lambda name, t, *a: (seen.append((name, a[-3])), call(name, t, *a))[1])
     scan_tests.check_train(lens, 40, 16, seed=ranges, ranges=ranges)
     assert seen == [("greta_ssm_scan_fwd", ranges), ("greta_ssm_scan_bwd", ranges)]
+
+
+def test_train_wide_states_in_several_launches():
+    """So many tokens, channels and states that the backward takes its blocks of
+    channels in several launches: channels have their halves' bits, and the sums
+    over all channels those of the halves but for rounding. (Positive operands: no
+    sum is smaller than its parts, of which 512 are added.)"""
+    from greta_plugin_b200 import _capi, selective_scan
+
+    T, D, N, ranges = 4200, 4096, 128, 6
+    assert _capi.lib().greta_ssm_scan_bwd_workspace(1, T, D, N, 1, ranges) < T * 2 * N * 4 * 512  # rows of all blocks
+    g = torch.Generator(DEV).manual_seed(0)
+    one = lambda *s: torch.rand(*s, generator=g, device=DEV)  # noqa: E731
+    u, dt, dout = one(1, T, D), one(1, T, D) * 0.2, one(1, T, D)
+    A, B, C = -one(D, N) * 4 - 0.05, one(T, 1, N), one(T, 1, N)
+    cu = torch.tensor([0, 1800, 1801, T], dtype=torch.int32, device=DEV)
+
+    def grads(c):
+        leaf = [v.contiguous().requires_grad_() for v in (u[..., c], dt[..., c], A[c], B.clone(), C.clone())]
+        with _capi.launch_options(rows_ranges=ranges):
+            out = selective_scan(*leaf, cu_seqlens=cu)
+        return torch.autograd.grad(out, leaf, dout[..., c].contiguous())
+
+    whole, halves = grads(slice(0, D)), [grads(slice(0, D // 2)), grads(slice(D // 2, D))]
+    for i, dim in ((0, 2), (1, 2), (2, 0)):
+        assert torch.equal(whole[i], torch.cat([h[i] for h in halves], dim))
+    for i in (3, 4):
+        want = halves[0][i].double() + halves[1][i].double()
+        assert ((whole[i].double() - want).abs() <= 2 * 520 * R.ROUNDING * want).all()

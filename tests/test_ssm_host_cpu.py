@@ -180,3 +180,39 @@ def test_max_query_len_reaches_the_calls(monkeypatch):
         longest(-1)
     assert _capi.lib().greta_ssm_scan_workspace(1, 64, 70, 64, 16, 1, 0) == 0
     assert _capi.lib().greta_ssm_scan_workspace(1 | longest(64), 64, 70, 64, 16, 1, 0) > 0
+
+
+def test_scan_backward_parts_are_bounded(runtime):
+    """A row of sums of dB and dC for every token and block of channels is as much as
+    the inputs times the states: 8.6 GB in one launch of 16384 x 4096 x 128. Launches
+    of some of the blocks after one another, whole waves of CTAs, keep it to 2 GB,
+    or to what one wave leaves."""
+    shapes = [(16384, 4096, 128, 1), (16384, 4096, 128, 3), (16384, 4096, 16, 1), (131072, 4096, 128, 1),
+              (16384, 4096, 128, 512), (65536, 8192, 64, 8)]
+    shapes = [(T, D // F * F, N, F) for T, D, N, F in shapes]
+    lines = recorded(runtime, f"""
+for T, D, N, F_ in {shapes}:
+    n = L.greta_ssm_scan_bwd_workspace(1, T, D, N, F_, 0)
+    print("bytes", n, flush=True)
+    assert L.greta_ssm_scan_bwd(2, F, D, F, D, None, 0, F, F_ * N, F, F_ * N, F, None, None, F, F, F, F, None, F, F, F,
+                                None, None, None, 0, 0, T, D, N, F_, 0, 0, F, n, None) == 0
+    print("end", flush=True)
+""")
+    lines = [v for v in lines if v[0] != "set"]
+    at = 0
+    for T, D, N, F in shapes:
+        end = lines.index(["end"], at)
+        need, launches = int(lines[at][1]), [(int(v[2]), int(v[3])) for v in lines[at + 1:end]]
+        at = end + 1
+        lanes = 4 if N <= 16 else 8 if N <= 32 else 16 if N <= 64 else 32
+        blocks = F * -(-(-(-(D // F) // (32 // lanes * 2))) // 4)
+        R = launches[0][1]  # (the carries first)
+        main = [x for x, y in launches[1:-1] if y == R and x <= blocks]
+        sums = [x for x, y in launches[1:-1] if x == -(-T * 2 * N // 256)]
+        assert sum(main) == blocks and len(sums) == len(main) and len(launches) == 2 + 2 * len(main)
+        row, wave = T * 2 * N * 4, 148 * 3 // R
+        most = max(main) * row
+        assert most <= max(2 << 30, wave * row)
+        assert len(main) == 1 or max(main) % wave == 0
+        # what else there is: the carries and parts of the ranges, and the sums between the launches
+        assert need <= most + R * D * N * 4 * 3 + 3 * R * D * 4 + F * row + 4096
