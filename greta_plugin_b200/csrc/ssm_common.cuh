@@ -95,8 +95,9 @@ struct SeqView {
 // The ranges that a packed stream is cut into. Split: by position, L tokens
 // each; a sequence over several ranges needs carries between them. Whole: range
 // i takes the sequences that begin in its L tokens, so none needs a carry, but
-// the longest sequence is one warp's walk; taken where that is at most `limit`
-// tokens (up to 31 sequences; the carries of many short ones cost little).
+// the longest sequence is one warp's walk, as are the rows ahead of the first and
+// behind the last; taken where each is at most `limit` tokens (up to 31
+// sequences; the carries of many short ones cost little).
 struct Ranges {
   int L;
   bool whole;
@@ -104,8 +105,9 @@ struct Ranges {
   __device__ __forceinline__ Ranges(const SeqView& v, int L_, int limit) : L(L_), whole(false) {
     if (!v.held) return;
     const int next = __shfl_down_sync(0xffffffffu, v.mine, 1);
-    const int longest = __reduce_max_sync(0xffffffffu, v.lane < v.q.nseq ? next - v.mine : 0);
-    whole = longest <= limit;
+    int run = v.lane < v.q.nseq ? next - v.mine : v.lane == v.q.nseq ? v.q.T - v.mine : 0;
+    if (v.lane == 0) run = max(run, v.mine);
+    whole = __reduce_max_sync(0xffffffffu, run) <= limit;
   }
 
   // The first token of range i.

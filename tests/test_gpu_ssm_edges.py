@@ -515,3 +515,17 @@ def test_train_wide_states_in_several_launches():
     for i in (3, 4):
         want = halves[0][i].double() + halves[1][i].double()
         assert ((whole[i].double() - want).abs() <= 2 * 520 * R.ROUNDING * want).all()
+
+
+@pytest.mark.parametrize("head, tail", [(0, 3000), (2500, 0), (900, 2100)])
+def test_short_sequences_among_many_rows_outside(head, tail):
+    """Short sequences beside long runs of rows that none holds, which are dealt to
+    the ranges as a long sequence would be."""
+    lens, D = [60, 100, 3, 80], 1024
+    T = sum(lens) + head + tail
+    got = scan_tests.check_train(lens, D, 16, dtype=torch.bfloat16, head=head, tail=tail)
+    for k in ("out", "du", "ddelta", "dgate", "dB", "dC"):
+        assert not got[k][:head].any() and not got[k][T - tail:].any(), k
+    if head == 0:
+        scan_tests.check_packed(lens, [2, 0, -1, 1], [1, 0, 1, 1], D, 16, tail=tail)
+        scan_tests.check_packed(lens, [2, 0, -1, 1], [1, 0, 1, 1], D, 16, tail=tail, given_out=False)
