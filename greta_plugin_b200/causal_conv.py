@@ -57,16 +57,8 @@ def _check_weight(x, weight, bias):
         raise ValueError(f"kernel size must be between 1 and {MAX_WIDTH}, got {W}")
     if bias is not None and (bias.dim() != 1 or bias.shape[0] != D):
         raise ValueError(f"bias must be [{D}], got {tuple(bias.shape)}")
-    refuse_complex(weight=weight, bias=bias)
     same_device("x", x, weight=weight, bias=bias)
     return W
-
-
-def refuse_complex(**params):
-    """Parameters are converted to a real type, which would drop an imaginary part."""
-    for name, t in params.items():
-        if t is not None and t.is_complex():
-            raise ValueError(f"{name} must be real, got {t.dtype}")
 
 
 def same_device(name, t, **others):
@@ -77,8 +69,15 @@ def same_device(name, t, **others):
             raise ValueError(f"{k} is on {o.device}, {name} on {t.device}")
 
 
+def to_real(t, dtype):
+    """t.to(dtype) for a real type, which would drop an imaginary part."""
+    if t.is_complex():
+        raise ValueError(f"parameters must be real, got {t.dtype}")
+    return t.to(dtype)
+
+
 def _as_type(t, dtype):
-    return t if t is None or t.dtype == dtype else t.to(dtype)
+    return t if t is None or t.dtype == dtype else to_real(t, dtype)
 
 
 def _bias(bias, dtype):
@@ -176,9 +175,7 @@ def packed_metadata(x, state, starts, slots, has_initial):
 
 
 def longest(max_query_len) -> int:
-    """GRETA_SSM_LONGEST of max_query_len (None: not known)."""
-    if max_query_len is None:
-        return 0
+    """GRETA_SSM_LONGEST of max_query_len."""
     n = int(max_query_len)
     if n < 0:
         raise ValueError(f"max_query_len must not be negative, got {n}")
@@ -221,7 +218,7 @@ def _packed(x, weight, bias, state, starts, slots, has_initial, activation, out,
     T, D = x.shape
     W = _check_weight(x, weight, bias)
     silu = _activation(activation)
-    most = longest(max_query_len)
+    most = 0 if max_query_len is None else longest(max_query_len)
     if state.dim() != 3 or state.shape[1] != D or state.shape[2] != W - 1:
         raise ValueError(f"state must be [slots, {D}, {W - 1}], got {tuple(state.shape)}")
     if state.dtype != x.dtype:

@@ -29,8 +29,7 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .causal_conv import (channel_rows, check_disjoint, longest, packed_metadata, packed_out, refuse_complex,
-                          same_device)
+from .causal_conv import channel_rows, check_disjoint, longest, packed_metadata, packed_out, same_device, to_real
 from .dynamic_conv import _cu
 
 MAX_STATES = 128
@@ -66,7 +65,6 @@ def _check(u, delta, A, B, C, skip, gate, delta_bias):
         for name, t in (("delta", delta), ("gate", gate), ("B", B), ("C", C)):
             if t is not None and t.dtype != dt:
                 raise ValueError(f"{name} dtype {t.dtype} must match u dtype {dt}")
-    refuse_complex(A=A, skip=skip, delta_bias=delta_bias)
     same_device("u", u, delta=delta, A=A, B=B, C=C, skip=skip, gate=gate, delta_bias=delta_bias)
     return T, D, N, groups[1]
 
@@ -86,7 +84,7 @@ def _fp32(t):
     if t is None:
         return None
     if t.dtype is not torch.float32 or not t.is_contiguous():
-        t = t.float().contiguous()
+        t = to_real(t, torch.float32).contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -202,7 +200,7 @@ def _packed(u, delta, A, B, C, skip, gate, delta_bias, state, starts, slots, has
     if u.dim() != 2:
         raise ValueError(f"u must be [T, D], got {tuple(u.shape)}")
     T, D, N, F = _check(u, delta, A, B, C, skip, gate, delta_bias)
-    most = longest(max_query_len)
+    most = 0 if max_query_len is None else longest(max_query_len)
     if state.dim() != 3 or state.shape[1] != D or state.shape[2] != N:
         raise ValueError(f"state must be [slots, {D}, {N}], got {tuple(state.shape)}")
     if state.dtype != torch.float32:

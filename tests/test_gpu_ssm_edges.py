@@ -529,3 +529,24 @@ def test_short_sequences_among_many_rows_outside(head, tail):
     if head == 0:
         scan_tests.check_packed(lens, [2, 0, -1, 1], [1, 0, 1, 1], D, 16, tail=tail)
         scan_tests.check_packed(lens, [2, 0, -1, 1], [1, 0, 1, 1], D, 16, tail=tail, given_out=False)
+
+
+def test_complex_parameters_are_refused():
+    import greta_plugin_b200 as greta
+
+    s, _ = scan_tests.make(5, 8, 4, 1, torch.bfloat16, 0)
+    rows = {k: v[None] if k in ("u", "delta", "gate") else v for k, v in s.items()}
+    st, sl, init = meta([5], [0])
+    for k in ("A", "skip", "delta_bias"):
+        z = s[k].to(torch.complex64)
+        with pytest.raises(ValueError, match="must be real"):
+            greta.selective_scan(**{**rows, k: z})
+        with pytest.raises(ValueError, match="must be real"):
+            greta.packed_selective_scan(**{**s, k: z}, state=torch.zeros(2, 8, 4, device=DEV), starts=st, slots=sl,
+                                        has_initial=init)
+    x, w, b = s["u"], s["u"][:3], s["u"][0]
+    for kw in (dict(weight=w.to(torch.complex64), bias=b), dict(weight=w, bias=b.to(torch.complex64))):
+        with pytest.raises(ValueError, match="must be real"):
+            greta.causal_conv1d(x[None], **kw)
+        with pytest.raises(ValueError, match="must be real"):
+            greta.packed_causal_conv1d(x, **kw, state=x.new_zeros(2, 8, 2), starts=st, slots=sl, has_initial=init)
