@@ -38,14 +38,18 @@ def packed_batch_metadata(query_lens: torch.Tensor, context_lens: torch.Tensor, 
 
     query_lens, context_lens: [N] int32; negative lengths count as 0.
     num_tokens: rows T of the packed tensors, at least the sum of query_lens;
-    tokens past it are dropped (the offsets end at T).
+    tokens past it are dropped (the offsets end at T), though their blocks are
+    asked for like the others'.
 
     With block_tables ([N, M] int32, contiguous rows, updated in place) the
     requests' tables grow by the blocks that their new tokens begin, taken from
     the front of free_blocks ([K] int32) in request order, and every token gets
     its slot: block * block_size + position % block_size. blocks_used is the
     number of blocks asked for: above K, the list ran out, and the entries and
-    slots without a block are -1, as are slots past the table's width M.
+    slots without a block are -1, as are slots past the table's width M. It counts
+    the blocks of all query_lens: those that only dropped tokens would begin, and
+    those past the table's width, stand in no table, so a caller whose T may be
+    below the sum clamps query_lens first, or those blocks are lost to it.
     """
     for name, t in (("query_lens", query_lens), ("context_lens", context_lens)):
         if t.dim() != 1 or t.dtype != torch.int32:

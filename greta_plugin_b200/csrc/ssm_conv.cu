@@ -170,7 +170,8 @@ int bwd_one(ConvParams p, const ParamGrads& g, cudaStream_t st) {
   return g.f32 ? reduce<float>(p, rows, g, st) : reduce<T>(p, rows, g, st);
 }
 
-// Vectors of half the forward's: a thread's sums take 3 W registers a channel.
+// Vectors of half the forward's: with the filters and the window in fp32, as they
+// are here, a thread has 4 W - 1 registers a channel, 2 W of them sums.
 template <typename T>
 int bwd_type(const ConvParams& p, const ParamGrads& g, cudaStream_t st) {
   return with_taps(p.W, [&](auto taps) {

@@ -522,10 +522,11 @@ __global__ void __launch_bounds__(128) ssm_conv_decode_kernel(const ConvParams p
 // the sum of token t-W+1 (of t-MW+1 with a runtime W) is then complete. dw and dbias of the run stay in
 // registers, the block's four runs are added in shared memory, and one row of
 // partial sums per block goes to `part`, which ssm_conv_reduce_kernel adds in
-// a fixed order: the same call gives the same bits. Four channels a thread (the
-// sums of eight do not fit 128 registers): some 100 instructions a token for 12
-// elements read and written, so issue and fp32 pipe (half of each at 16 warps an
-// SM) are ahead of HBM: 16288 x 4096, 4 taps, bf16 100 us, 4.0 TB/s.
+// a fixed order: the same call gives the same bits. Four channels a thread (sums,
+// filters and windows of eight in fp32 do not fit 128 registers): 102 instructions
+// a token for 12 elements read and written, so issue and fp32 pipe (45 and 44 %
+// busy at 16 warps an SM) are ahead of HBM: 16288 x 4096, 4 taps, bf16 100 us,
+// 4.0 TB/s.
 template <typename T, int NV, int WT>
 __global__ void __launch_bounds__(128, WT > -16 ? 4 : 2) ssm_conv_bwd_kernel(const ConvParams p) {
   constexpr int MW = WT > 0 ? WT : -WT;

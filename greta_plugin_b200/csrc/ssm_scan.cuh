@@ -34,9 +34,9 @@
 // sequences are paid twice, and the host cuts no finer than it takes to fill
 // the GPU; where the longest sequence allows it, ranges take whole sequences
 // instead (Ranges).
-// 16288 tokens of nine sequences, 4096 x 16, bf16: carries 328 us (72 % of the
-// exponentials' rate), outputs and saved states 446 us (53 %; 168 instructions a
-// warp and token, seven in ten issue slots). 8000 x 2048 x 64, fp16: 320 + 415 us.
+// 16288 tokens of nine sequences, 4096 x 16, bf16: carries 330 us (71 % of the
+// exponentials' rate), outputs and saved states 465 us (50 %; 168 instructions a
+// warp and token, six in ten issue slots). 8000 x 2048 x 64, fp16: 327 + 431 us.
 #pragma once
 
 #include "ssm_common.cuh"

@@ -29,9 +29,9 @@
 // A range that ends inside a sequence needs a g of the next token: the carry
 // kernel runs g alone over the part of each range up to the first sequence end
 // in it, as the forward's does for h.
-// 16288 tokens of nine sequences, 4096 x 16, bf16: carries 328 us, 1605 us, sums
-// over CTAs and ranges 50 us. The main kernel has the shared memory 69 % busy
-// (74 rows of 128 bytes a warp and token) and issues in 52 % of the slots, at
+// 16288 tokens of nine sequences, 4096 x 16, bf16: carries 338 us, 1592 us, sums
+// over CTAs and ranges 38 us. The main kernel has the shared memory 64 % busy
+// (74 rows of 128 bytes a warp and token) and issues in 50 % of the slots, at
 // three warps a scheduler: its registers leave room for no more.
 #pragma once
 

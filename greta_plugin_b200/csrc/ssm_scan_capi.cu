@@ -42,11 +42,15 @@ int64_t plan_ranges(int64_t T, int64_t D, int64_t N, int64_t F, int asked, bool 
   return L;
 }
 
-// The longest sequence with which ranges take whole sequences: kWholeShare of
+// The longest sequence with which ranges take whole sequences (Ranges): kWholeShare of
 // the tokens that each scheduler has to walk in all (four an SM). Measured at
 // 4096 x 16, forward and backward: 16 sequences of 128 tokens (0.29) 106 + 298 us
 // split, 73 + 263 whole; 12 of 1365 (0.39) 715 + 2038, 681 + 1882; 8 of 256 (0.58)
-// 116 + 297, 108 + 322; 8 of 2048 (0.58) 749 + 2039, 1014 + 2320.
+// 116 + 297, 108 + 322; 8 of 2048 (0.58) 749 + 2039, 1014 + 2320. With more states
+// the same lengths are a smaller share: 4096 x 64, 3 of 683 tokens (0.39) 409 + 1315, 392 + 1241; 4096 x 128, 2 of 1024 (0.29) 767 +
+// 2516, 643 + 2585, 9 of 227 (0.06) 732 + 2445, 605 + 2375. (Rows that no sequence
+// holds count like one: 8192 rows of four sequences of 100 tokens and no others,
+// 4096 x 16, forward: 1014 us whole, 111 split.)
 constexpr double kWholeShare = 0.4;
 int whole_limit(int64_t T, int64_t D, int64_t N, int64_t F, int asked) {
   if (asked > 0) return 0;

@@ -158,7 +158,9 @@ GRETA_API int64_t greta_ssm_scan_workspace(int packed, int64_t num_seqs, int64_t
  *   slot_map    [T] block * block_size + position % block_size, -1 where there
  *               is no block (behind the last token, past the table's width, or
  *               the list ran out; such table entries become -1)
- *   blocks_used [1] blocks asked for (above num_free: the list ran out)
+ *   blocks_used [1] blocks asked for (above num_free: the list ran out), for all
+ *               of query_lens: blocks that only tokens past T would begin, or that
+ *               lie past the table's width, are counted and stand in no table
  * At most 16384 requests.
  */
 GRETA_API int greta_ssm_batch_metadata(const int32_t* query_lens, const int32_t* context_lens, int64_t num_reqs,
