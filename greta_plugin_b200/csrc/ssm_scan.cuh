@@ -363,6 +363,15 @@ __device__ __forceinline__ int sum_channel(int lane) {
   return KD == 4 ? (lane & 1) * 2 + ((lane >> 1) & 1) : lane & 1;
 }
 
+// Factors of a state: of one that is zero, 0 (a range's growth may be past what fp32
+// holds where no token's is, and inf times 0 would be NaN).
+__device__ __forceinline__ f2 f2_keep(f2 a, f2 h) {
+  float a0, a1, h0, h1;
+  unpack2(a, a0, a1);
+  unpack2(h, h0, h1);
+  return pack2(h0 == 0.f ? 0.f : a0, h1 == 0.f ? 0.f : a1);
+}
+
 // A state (or adjoint) brought through the ranges `from`, .., `to` (in that
 // direction): the first one's carry, then carry + exp(A sum dt) times what came.
 template <int LN, int KD>
@@ -384,7 +393,7 @@ __device__ __forceinline__ void carry_through(const ScanParams& p, const Lanes<L
       }
       const f2 d2 = pack2(d[0], d[1]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) h[c][k] = f2_fma(f2_decay(d2, A2[c][k]), h[c][k], s[c][k]);
+      for (int k = 0; k < 4; ++k) h[c][k] = f2_fma(f2_keep(f2_decay(d2, A2[c][k]), h[c][k]), h[c][k], s[c][k]);
     }
   }
 }

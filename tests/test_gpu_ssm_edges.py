@@ -550,3 +550,28 @@ def test_complex_parameters_are_refused():
             greta.causal_conv1d(x[None], **kw)
         with pytest.raises(ValueError, match="must be real"):
             greta.packed_causal_conv1d(x, **kw, state=x.new_zeros(2, 8, 2), starts=st, slots=sl, has_initial=init)
+
+
+def test_growing_states_that_are_zero_for_ranges():
+    """Positive rates: over a range the growth is past what fp32 holds, but the
+    state that it multiplies is zero until the first input. (Gradients are not
+    looked at: theirs go back to the first token, e^100 and more.)"""
+    from greta_plugin_b200 import _capi, packed_selective_scan, selective_scan
+
+    T, D, N = 104, 32, 16
+    s, _ = scan_tests.make(T, D, N, 1, torch.float32, 3, options=("skip", "gate"))
+    s["A"] = s["A"].abs() * 2 + 1  # up to 5, steps of 1: e^5 a token
+    s["delta"] = torch.ones_like(s["delta"])
+    s["u"][:100] = 0
+    val, mag = R.scan(**s)
+    # |dt A| of 5 takes 8 * 5 + 8 roundings a token, over the four tokens with a state
+    n = 4 * 48 + 64
+    st, sl, init = meta([T], [0], [0])
+    for ranges in (0, 1, 6):
+        state = torch.zeros(1, D, N, device=DEV)
+        with _capi.launch_options(rows_ranges=ranges):
+            out = selective_scan(**{k: v[None] if k in ("u", "delta", "gate") else v for k, v in s.items()})
+            packed = packed_selective_scan(**s, state=state, starts=st, slots=sl, has_initial=init)
+        R.assert_within(out[0], val["out"], mag["out"], torch.float32, n, f"out {ranges}")
+        R.assert_within(packed, val["out"], mag["out"], torch.float32, n, f"packed {ranges}")
+        R.assert_within(state[0], val["last"][0], mag["last"][0], torch.float32, n, f"state {ranges}")
